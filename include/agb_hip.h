@@ -421,6 +421,28 @@ int agb_layernorm_fwd(const float* X, int ldx, int n, int C, const float* gamma,
 int agb_layernorm_bwd(const float* X, int ldx, const float* dY, int ldy, int n, int C, const float* gamma,
                       const float* stats, float* dX, int lddx, float* part, float* dgamma, float* dbeta, void* stream);
 
+/* Row norms around a residual block (layer: rms = 0, centred; rms = 1: not), fused with what touches the same rows:
+ *   Y = act(R + keep[p] gate[p] scale norm(Z)),  norm(z) = zhat w + b, p = the plot of the row;  H = norm(Y) w2 + b2 (rms and
+ *   layer alike; from the unrounded Y).
+ * Rows are float (bf16 = 0) or bf16 bit patterns (bf16 = 1), ld* in elements; everything else is float.  NULL: R (nothing is
+ * added), w / scale / gate / keep / w2 (ones), b / b2 (zeros), Y or H (not written; not both).  gate [B][C] and keep [B] need ptr
+ * int32 [B + 1], the plots' row ranges; rows behind ptr[B] belong to no plot: Y = act(R), dZ = 0.  act: 0 none, 1 ReLU, 2 GELU.
+ * C <= 4096.
+ * _bwd recomputes from Z and R.  dY, dH: either may be NULL (zeros); dZ, dR and the parameter gradients (dw, db, dscale, dw2,
+ * db2 [C], dgate [B][C]) may be NULL.  Sums over rows are folded in a fixed order through `workspace`
+ * (agb_rownorm_bwd_workspace_bytes: B = 0 without plots; next = dH is given). */
+int agb_rownorm_fwd(const void* Z, long long ldz, const void* R, long long ldr, int n, int C, const float* w, const float* b,
+                    float eps, int rms, int act, const float* gate, const float* keep, const int32_t* ptr, int B,
+                    const float* scale, const float* w2, const float* b2, float eps2, void* Y, long long ldy, void* H,
+                    long long ldh, int bf16, void* stream);
+size_t agb_rownorm_bwd_workspace_bytes(int n, int C, int B, int next);      /* host helper */
+int agb_rownorm_bwd(const void* Z, long long ldz, const void* R, long long ldr, const void* dY, long long lddy, const void* dH,
+                    long long lddh, int n, int C, const float* w, const float* b, float eps, int rms, int act,
+                    const float* gate, const float* keep, const int32_t* ptr, int B, const float* scale, const float* w2,
+                    const float* b2, float eps2, void* dZ, long long lddz, void* dR, long long lddr, float* dw, float* db,
+                    float* dgate, float* dscale, float* dw2, float* db2, void* workspace, size_t workspace_bytes, int bf16,
+                    void* stream);
+
 /* ---------------------------------------------------------------------------------------------------------
  * KPConv index path.  Replaces the CPython extensions behind modules/KPConv/common.py:
  *   radius_neighbors.batch_query   cpp_wrappers/cpp_neighbors/wrapper.cpp:58-238 -> neighbors/neighbors.cpp:211-333

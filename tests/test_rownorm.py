@@ -1,0 +1,384 @@
+"""Row norms around a residual block (norm_ops.row_norm_act / row_norm_join, csrc/rownorm.hip) against the formulas in 64 bits:
+values and every gradient, over widths that take each lane layout, ragged and empty plots, strided and misaligned rows, rows
+behind the last plot, both storage types; repeatability, streams, captured graphs, and the refusals."""
+import math
+
+import pytest
+import torch
+
+EPS = 1e-6
+
+
+def normed(x, kind, eps=EPS):
+    if kind == "layer":
+        x = x - x.mean(1, keepdim=True)
+    return x / torch.sqrt((x * x).mean(1, keepdim=True) + eps)
+
+
+def reference(t, kind, act, want_h):
+    """The definition, differentiable, in the type of its arguments (float64 here)."""
+    c = t["z"].shape[1]
+    n = normed(t["z"], kind) * t["w"] + (t["b"] if t.get("b") is not None else 0)
+    u = n
+    if t.get("r") is not None:
+        f = torch.ones_like(n)
+        if t.get("scale") is not None:
+            f = f * t["scale"]
+        if t.get("plot") is not None:
+            live = (t["plot"] < t["plots"])[:, None]
+            at = t["plot"].clamp(max=t["plots"] - 1)
+            if t.get("gate") is not None:
+                f = f * t["gate"][at]
+            if t.get("keep") is not None:
+                f = f * t["keep"][at][:, None]
+            n = torch.where(live, n, torch.zeros_like(n))
+            f = f * live
+        u = t["r"] + f * n
+    y = u if act == "none" else torch.relu(u) if act == "relu" else 0.5 * u * (1 + torch.erf(u / math.sqrt(2)))
+    h = normed(y, kind) * t["w2"] + t["b2"] if want_h else None
+    assert y.shape[1] == c
+    return y, h
+
+
+def make(n, c, dtype, device, join=True, plots=None, want_h=False, seed=0, bias=True, behind=0):
+    g = torch.Generator().manual_seed(seed)
+    rn = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    t = dict(z=(rn(n, c) * 1.5 + 0.7).to(dtype), w=1 + 0.2 * rn(c), b=0.3 * rn(c) if bias else None)
+    if join:
+        t.update(r=rn(n, c).to(dtype), scale=0.5 + 0.1 * rn(c))
+    if plots:
+        cut = torch.sort(torch.randint(0, n - behind + 1, (plots - 1,), generator=g))[0]
+        ptr = torch.cat([torch.zeros(1, dtype=torch.long), cut, torch.tensor([n - behind])])
+        t.update(ptr=ptr.to(torch.int32), plots=plots, gate=torch.sigmoid(rn(plots, c)),
+                 keep=(torch.rand(plots, generator=g) > 0.25).float() / 0.75)
+        t["plot"] = torch.bucketize(torch.arange(n), ptr[1:].contiguous(), right=True)
+    if want_h:
+        t.update(w2=1 + 0.2 * rn(c), b2=0.1 * rn(c))
+    t["dy"], t["dh"] = rn(n, c).to(dtype), rn(n, c).to(dtype)
+    return {k: v.to(device) if torch.is_tensor(v) else v for k, v in t.items()}
+
+
+LEAVES = ("z", "r", "w", "b", "gate", "scale", "w2", "b2")
+
+
+def call(t, kind, act, want_h):
+    from dpcr_agb_amd import norm_ops
+    if t.get("r") is None:
+        return norm_ops.row_norm_act(t["z"], t["w"], t["b"], EPS, kind, act), None
+    out = norm_ops.row_norm_join(t["z"], t["r"], t["w"], t["b"], EPS, kind, act, gate=t.get("gate"), keep=t.get("keep"),
+                                 ptr=t.get("ptr"), scale=t.get("scale"), next_norm=(t["w2"], t["b2"]) if want_h else None)
+    return out if want_h else (out, None)
+
+
+def with_grads(f, t, kind, act, want_h):
+    t = dict(t)
+    keys = [k for k in LEAVES if t.get(k) is not None]
+    for k in keys:
+        t[k] = t[k].detach().requires_grad_()
+    y, h = f(t, kind, act, want_h)
+    outs, douts = ([y], [t["dy"]]) if h is None else ([y, h], [t["dy"], t["dh"]])
+    grads = torch.autograd.grad(outs, [t[k] for k in keys], [d.to(o.dtype) for d, o in zip(douts, outs)])
+    return dict(y=y.detach(), **({} if h is None else {"h": h.detach()}), **{"d" + k: g for k, g in zip(keys, grads)})
+
+
+def check(t, kind, act, want_h):
+    got = with_grads(call, t, kind, act, want_h)
+    t64 = {k: v.double() if torch.is_tensor(v) and v.is_floating_point() else v for k, v in t.items()}
+    ref = with_grads(reference, t64, kind, act, want_h)
+    assert got.keys() == ref.keys()
+    # Rows are rounded once on store: half a step of their type.  Before it, fp32: a handful of operations and the pairwise sums
+    # of a row, 8 steps of 2^-24 of the terms' size.  What a norm does to an error: x - mean loses max|x| rstd (relative to
+    # xhat), a gradient through it is multiplied by rstd; `cond` is that, per row, for the norm and the next one.  Terms: |dy|,
+    # |w|, ... stay below 8 together with the value itself.
+    def cond(x):
+        d = x - x.mean(1, keepdim=True) if kind == "layer" else x
+        rstd = 1 / torch.sqrt((d * d).mean(1, keepdim=True) + EPS)
+        return (1 + rstd * x.abs().amax(1, keepdim=True)) * (1 + rstd)
+
+    k64 = cond(t64["z"]) if t["z"].numel() else None
+    if want_h and k64 is not None:
+        k64 = k64 * cond(ref["y"])
+    for k, v in got.items():
+        assert v.dtype == (t["z"].dtype if k in ("y", "h", "dz", "dr") else torch.float32), k
+        r = ref[k]
+        assert torch.isfinite(v.double()).all(), k
+        if not r.numel():
+            continue
+        unit = 8 * 2.0 ** -24
+        if k in ("y", "h", "dz", "dr"):
+            tol = torch.finfo(v.dtype).eps / 2 * r.abs() + unit * k64 * (r.abs().amax(1, keepdim=True) + 8)
+        else:         # errors of the rows add up as their squares; the folds' own roundings are of the sum's size
+            tol = unit * (8 * k64.square().sum().sqrt() + r.abs())
+        bad = (v.double() - r).abs() > tol
+        assert not bad.any(), (k, float((v.double() - r).abs().max()), float(r.abs().max()))
+
+
+WIDTHS = [1, 3, 4, 31, 32, 33, 64, 100, 128, 203, 256, 511, 512, 1000, 1024, 1025, 2048, 2051, 4096]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("c", WIDTHS)
+def test_norm_act_all_widths(device, c, dtype):
+    for i, (n, kind, act) in enumerate([(1, "layer", "gelu"), (37, "rms", "relu"), (150, "layer", "none")]):
+        check(make(n, c, dtype, device, join=False, seed=i, bias=i != 1), kind if c > 1 else "rms", act, False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("c", WIDTHS)
+def test_join_all_widths(device, c, dtype):
+    kind = ("layer", "rms")[c % 2] if c > 1 else "rms"
+    check(make(257, c, dtype, device, plots=5, seed=c), kind, ("none", "gelu")[c % 2], False)
+    check(make(100, c, dtype, device, seed=c), kind, "none", False)                       # no plots
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c", [4, 64, 203, 512, 1024, 2048, 4096])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_join_with_next_norm(device, c, dtype):
+    check(make(131, c, dtype, device, plots=3, seed=c, want_h=True), "layer", "gelu", True)
+    check(make(66, c, dtype, device, seed=c + 1, want_h=True), "rms", "none", True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,plots", [(1, 1), (2, 7), (64, 64), (5000, 3), (9001, 130), (70000, 32)])
+def test_join_ragged_plots(device, n, plots):
+    """More plots than rows (most of them empty), plots shorter than a workgroup's turn, runs that hold several plots and plots
+    that span many runs."""
+    check(make(n, 96, torch.float32, device, plots=plots, seed=n), "layer", "gelu", False)
+    check(make(n, 61, torch.bfloat16, device, plots=plots, seed=n, want_h=True), "rms", "relu", True)
+
+
+@pytest.mark.gpu
+def test_rows_behind_the_last_plot_are_handed_on(device):
+    t = make(300, 64, torch.float32, device, plots=4, behind=40, seed=3)
+    check(t, "layer", "gelu", False)
+    t["z"][-5:] = float("nan")          # (whatever they hold)
+    got = with_grads(call, t, "layer", "none", False)
+    assert torch.equal(got["y"][-40:], t["r"][-40:])
+    assert torch.equal(got["dz"][-40:], torch.zeros_like(got["dz"][-40:]))
+    assert all(torch.isfinite(v).all() for v in got.values())
+
+
+@pytest.mark.gpu
+def test_no_rows(device):
+    t = make(0, 32, torch.float32, device, want_h=True)
+    got = with_grads(call, t, "layer", "gelu", True)
+    assert got["y"].shape == (0, 32) and got["dz"].shape == (0, 32)
+    for k in ("dw", "db", "dscale", "dw2", "db2"):
+        assert torch.equal(got[k], torch.zeros(32, device=device)), k
+    t = make(0, 32, torch.float32, device, plots=3)
+    assert torch.equal(with_grads(call, t, "rms", "none", False)["dgate"], torch.zeros(3, 32, device=device))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_strides_and_alignment(device, dtype):
+    """Rows cut out of wider matrices (aligned, misaligned), transposed and expanded ones give the contiguous result."""
+    t = make(90, 64, dtype, device, plots=4, seed=1)
+    want = with_grads(call, t, "layer", "gelu", False)
+    wide = torch.zeros(90, 200, dtype=dtype, device=device)
+    for off in (0, 64, 1, 6):
+        s = dict(t)
+        a, b = wide.clone(), wide.clone()
+        a[:, off:off + 64], b[:, off:off + 64] = t["z"], t["r"]
+        s["z"], s["r"] = a[:, off:off + 64], b[:, off:off + 64]
+        got = with_grads(call, s, "layer", "gelu", False)
+        for k in want:
+            if off % 4 == 0:
+                assert torch.equal(got[k], want[k]), (off, k)
+            else:         # (another lane layout: another order of the fp32 sums)
+                assert torch.allclose(got[k].float(), want[k].float(), rtol=2.0 ** -7 if got[k].dtype == torch.bfloat16 else 1e-4,
+                                      atol=1e-4), (off, k)
+    s = dict(t, z=t["z"].t().contiguous().t(), dy=t["dy"].t().contiguous().t())
+    got = with_grads(call, s, "layer", "gelu", False)
+    assert all(torch.equal(got[k], want[k]) for k in want)
+    s = dict(t, dy=t["dy"][:1].expand(90, 64))
+    check(s, "layer", "gelu", False)
+
+
+@pytest.mark.gpu
+def test_only_what_is_asked_for(device):
+    """Gradients of single leaves, of y alone and of h alone."""
+    from dpcr_agb_amd import norm_ops
+    t = make(120, 48, torch.float32, device, plots=3, seed=5, want_h=True)
+    want = with_grads(call, t, "layer", "gelu", True)
+    for k in LEAVES:
+        s = {q: (v.detach().requires_grad_() if q == k else v) for q, v in t.items()}
+        y, h = call(s, "layer", "gelu", True)
+        (g,) = torch.autograd.grad([y, h], [s[k]], [t["dy"], t["dh"]])
+        assert torch.equal(g, want["d" + k]), k
+    zero = torch.zeros_like(t["dy"])
+    for used in ("y", "h"):
+        s = dict(t, z=t["z"].detach().requires_grad_(), r=t["r"].detach().requires_grad_())
+        y, h = call(s, "layer", "gelu", True)
+        got = torch.autograd.grad([y if used == "y" else h], [s["z"], s["r"]], [t["dy"] if used == "y" else t["dh"]])
+        q = dict(t, **{"dh" if used == "y" else "dy": zero})
+        ref = with_grads(call, q, "layer", "gelu", True)
+        for g, k in zip(got, ("dz", "dr")):
+            assert torch.allclose(g, ref[k], rtol=1e-5, atol=1e-5), (used, k)
+    # z also as its own shortcut: both gradients arrive
+    z = t["z"].detach().double().requires_grad_()
+    ref = torch.autograd.grad(z + normed(z, "rms"), z, t["dy"].double())[0]
+    zz = t["z"].detach().requires_grad_()
+    got = torch.autograd.grad(norm_ops.row_norm_join(zz, zz, None, None, EPS, "rms"), zz, t["dy"])[0]
+    assert float((got - ref).abs().max()) < 64 * 2.0 ** -24 * float(ref.abs().max() + 1)
+
+
+@pytest.mark.gpu
+def test_gradients_against_differences(device):
+    """The formula's gradient against central differences of the 64-bit definition."""
+    t = make(12, 20, torch.float32, device, plots=3, seed=8, want_h=True)
+    got = with_grads(call, t, "layer", "gelu", True)
+    t64 = {k: v.double() if torch.is_tensor(v) and v.is_floating_point() else v for k, v in t.items()}
+
+    def loss(s):
+        y, h = reference(s, "layer", "gelu", True)
+        return float((y * t64["dy"]).sum() + (h * t64["dh"]).sum())
+
+    g = torch.Generator().manual_seed(1)
+    for k in LEAVES:
+        d = torch.randn(t[k].shape, generator=g).double().to(device)
+        e = 1e-5
+        slope = (loss(dict(t64, **{k: t64[k] + e * d})) - loss(dict(t64, **{k: t64[k] - e * d}))) / (2 * e)
+        mine = float((got["d" + k].double() * d).sum())
+        assert abs(mine - slope) < 1e-4 * (abs(slope) + float(got["d" + k].double().norm())), (k, mine, slope)
+
+
+@pytest.mark.gpu
+def test_non_finite_rows_stay_in_their_rows(device):
+    t = make(40, 64, torch.float32, device, plots=2, seed=2)
+    clean = with_grads(call, t, "layer", "gelu", False)
+    t["z"][7, 3], t["z"][20, 0] = float("nan"), float("inf")
+    got = with_grads(call, t, "layer", "gelu", False)
+    rows = [i for i in range(40) if i not in (7, 20)]
+    for k in ("y", "dz", "dr"):
+        assert torch.equal(got[k][rows], clean[k][rows]), k
+
+
+@pytest.mark.gpu
+def test_repeats_bit_for_bit_and_on_another_stream(device):
+    t = make(20011, 128, torch.bfloat16, device, plots=9, seed=4)
+    a = with_grads(call, t, "layer", "gelu", False)
+    b = with_grads(call, t, "layer", "gelu", False)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        c = with_grads(call, t, "layer", "gelu", False)
+    torch.cuda.current_stream().wait_stream(side)
+    for k in a:
+        assert torch.equal(a[k], b[k]) and torch.equal(a[k], c[k]), k
+
+
+@pytest.mark.gpu
+def test_captured_and_replayed(device):
+    """Forward and backward captured once, replayed on new inputs between eager work; two graphs do not share anything."""
+    t = make(700, 64, torch.float32, device, plots=5, seed=6, want_h=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        with_grads(call, t, "layer", "gelu", True)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = with_grads(call, t, "layer", "gelu", True)
+        graphs.append((g, out))
+    for step in range(4):
+        new = make(700, 64, torch.float32, device, plots=5, seed=60 + step, want_h=True)
+        for k in ("z", "r", "gate", "dy", "dh", "w"):
+            t[k].copy_(new[k])
+        eager = with_grads(call, t, "layer", "gelu", True)
+        torch.cuda.synchronize()
+        for g, out in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for g, out in graphs:
+            for k in eager:
+                assert torch.equal(out[k], eager[k]), (step, k)
+
+
+@pytest.mark.gpu
+def test_long_offsets(device):
+    """Rows whose offsets pass 2^31 elements."""
+    from dpcr_agb_amd import norm_ops
+    n, c = 3, 64
+    big = torch.empty((1 << 31) // 2 * 3, dtype=torch.bfloat16, device=device)
+    ld = (1 << 31) // 2 + 64
+    z = big.as_strided((n, c), (ld, 1))
+    z.copy_(torch.randn(n, c))
+    y = norm_ops.row_norm_act(z)
+    assert torch.equal(y, norm_ops.row_norm_act(z.contiguous()))
+
+
+def test_refusals():
+    from dpcr_agb_amd import _lib, norm_ops
+    z = torch.zeros(4, 8)
+    with pytest.raises(_lib.AgbError):
+        norm_ops.row_norm_act(z)                                               # host rows
+    with pytest.raises(_lib.AgbError):
+        norm_ops.row_norm_act(z.half())
+    with pytest.raises(ValueError, match="kind"):
+        norm_ops.row_norm_act(z, kind="batch")
+    with pytest.raises(ValueError, match="act"):
+        norm_ops.row_norm_act(z, act="tanh")
+    with pytest.raises(ValueError):
+        norm_ops.row_norm_act(torch.zeros(4, 4097))
+    with pytest.raises(ValueError):
+        norm_ops.row_norm_act(torch.zeros(4, 0))
+    with pytest.raises(ValueError):
+        norm_ops.row_norm_act(torch.zeros(2, 4, 8))
+    with pytest.raises(ValueError, match="weight"):
+        norm_ops.row_norm_act(z, torch.ones(7))
+    with pytest.raises(_lib.AgbError, match="fp32"):
+        norm_ops.row_norm_act(z, torch.ones(8).bfloat16())
+    with pytest.raises(ValueError):
+        norm_ops.row_norm_join(z, None)
+    with pytest.raises(ValueError):
+        norm_ops.row_norm_join(z, torch.zeros(5, 8))
+    with pytest.raises(_lib.AgbError):
+        norm_ops.row_norm_join(z, z.bfloat16())
+    with pytest.raises(ValueError, match="ptr"):
+        norm_ops.row_norm_join(z, z, gate=torch.ones(2, 8))
+    ptr = torch.tensor([0, 2, 4], dtype=torch.int32)
+    with pytest.raises(ValueError, match="int32"):
+        norm_ops.row_norm_join(z, z, gate=torch.ones(2, 8), ptr=ptr.long())
+    with pytest.raises(ValueError, match="gate"):
+        norm_ops.row_norm_join(z, z, gate=torch.ones(3, 8), ptr=ptr)
+    with pytest.raises(ValueError, match="keep"):
+        norm_ops.row_norm_join(z, z, keep=torch.ones(3), ptr=ptr)
+    with pytest.raises(ValueError, match="drawn"):
+        norm_ops.row_norm_join(z, z, keep=torch.ones(2, requires_grad=True), ptr=ptr)
+    with pytest.raises(ValueError, match="next_norm"):
+        norm_ops.row_norm_join(z, z, next_norm=(torch.ones(9), None))
+
+
+def test_entry_points_validate_before_any_launch():
+    import ctypes
+    from dpcr_agb_amd import _lib, norm_ops  # noqa: F401
+    L = _lib.load()
+    p, f = ctypes.c_void_p(256), ctypes.c_float(1e-6)
+
+    def fwd(n=4, c=8, ldz=8, rms=0, act=0, gate=None, keep=None, ptr=None, B=0, z=p, y=p, bf16=0):
+        return L.agb_rownorm_fwd(z, ldz, None, 0, n, c, None, None, f, rms, act, gate, keep, ptr, B, None, None, None, f, y, 8,
+                                 None, 8, bf16, None)
+
+    for kw, word in (({"c": 0}, b"bad shape"), ({"c": 4097}, b"bad shape"), ({"n": -1}, b"bad shape"), ({"act": 3}, b"act"),
+                     ({"rms": 2}, b"rms"), ({"bf16": 2}, b"bf16"), ({"gate": p}, b"row ranges"), ({"keep": p}, b"row ranges"),
+                     ({"ptr": p, "B": 0}, b"row ranges"), ({"z": None}, b"null pointer"), ({"y": None}, b"null pointer"),
+                     ({"ldz": 7}, b"row stride")):
+        assert fwd(**kw) == -1 and word in L.agb_last_error(), kw
+    assert fwd(n=0, z=None, y=None) == 0
+    size = _lib.size_call("agb_rownorm_bwd_workspace_bytes", 1000, 64, 4, 0)
+    assert size >= (1000 // 64 // 8 + 5) * 2 * 64 * 4 and _lib.size_call("agb_rownorm_bwd_workspace_bytes", 1000, 64, 4, 1) == 2 * size
+
+    def bwd(ws=p, nbytes=size, dy=p, dgate=None, dw2=None, ptr=p, gate=p):
+        return L.agb_rownorm_bwd(p, 64, p, 64, dy, 64, None, 0, 1000, 64, None, None, f, 0, 0, gate, None, ptr, 4, None, None,
+                                 None, f, p, 64, None, 0, None, None, dgate, None, dw2, None, ws, ctypes.c_size_t(nbytes), 0,
+                                 None)
+
+    for kw, word in (({"ws": None}, b"workspace"), ({"nbytes": size - 1}, b"workspace"), ({"dy": None}, b"null pointer"),
+                     ({"dgate": p, "ptr": None, "gate": None}, b"not there"), ({"dw2": p}, b"next norm")):
+        assert bwd(**kw) == -1 and word in L.agb_last_error(), kw
