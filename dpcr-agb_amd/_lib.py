@@ -64,6 +64,11 @@ _SIGNATURES = {
     "agb_adabelief_chunk": [],
     "agb_adabelief_step": [c_void_p, c_void_p, c_void_p, c_int, c_float, c_float, c_float, c_float, c_float, c_float,
                            c_float, c_float, c_int, c_float, c_void_p],
+    "agb_ns_fields": [],
+    "agb_ns_workspace_bytes": [c_void_p, c_int],
+    "agb_orthogonalize": [c_void_p, c_int, c_int, c_void_p, ctypes.c_double, c_void_p, ctypes.c_size_t, c_void_p],
+    "agb_muon_update": [c_void_p, c_int, c_int, c_void_p, ctypes.c_double, c_void_p, ctypes.c_double, ctypes.c_double, c_int,
+                        c_float, c_void_p, ctypes.c_size_t, c_void_p],
 }
 
 # entry points over activation / gradient ROW MATRICES exist twice: fp32 rows (agb_xxx) and bf16 rows (agb_xxx_h), same

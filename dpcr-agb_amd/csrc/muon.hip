@@ -1,0 +1,653 @@
+// muon.hip — orthogonalised updates (muon_ops.orthogonalize / muon_update, optim.Muon): Newton-Schulz iterations on a list of
+// matrix stacks at once.  A matrix M [rows, cols] is taken by its shorter side k and its longer side n, as X [n, k]:
+//     X = M / (|M|_F + eps);   repeat:  G = X^T X,   P = b G + c G G,   X <- a X + X P
+// (an odd polynomial of every singular value), and the result is written out or, in an update, stepped along:
+//     m <- mu m + (1 - mu) g,  M = m  or  (1 - mu) g + mu m,  p <- decay p - step X.
+//
+// Bound: matrix instructions.  Operands are PAIRS of fp16, x 2^13 = hi + lo (22 to 23 bits), a product is three MFMAs — lo hi +
+// hi lo + hi hi, the dropped lo lo is 2^-24 of it — accumulated in fp32: the error of the result against 64 bits is that of
+// fp32 products (1e-6; plain bf16 or fp16 operands: 1e-3 and more, since the polynomial lifts the small singular values'
+// rounding noise up to 485-fold) at a ceiling of 2500 / 3 TFLOP/s instead of the 157 of fp32 MFMA.  2^13: entries are bounded
+// by the singular values' bound (checked from the coefficients to stay below 7), so hi stays below 65504, and an entry of 2^-13
+// still keeps its 22 bits.  a X is added in fp32 behind the products: folded into P's diagonal it would cost the small
+// directions two more bits.
+//
+// Layout: X is held twice, XT [n][k] and XL [k][n], so that every product reads both operands along their rows (G: XL XL^T,
+// P: G G^T with G symmetric, X P: XT P^T with P symmetric); both are written by the product that makes them, through an LDS
+// tile.  A row is cut into blocks of 32: 32 hi, then 32 lo — 128 contiguous bytes, what one step of a product takes of it.
+// Rows and blocks are padded to multiples of 64 with zeros, which the iteration keeps zero.  G and P are symmetric: only tiles
+// on and above the diagonal are computed.  G has few tiles and a long sum: it is split over n into chunks, folded in order.
+#include "agb_common.h"
+
+typedef _Float16 half_t;
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+#define NS_THREADS 256
+#define NS_SCALE 8192.f
+#define NS_UNSCALE (1.f / 8192.f)
+#define NS_CHUNK 16384      // elements of one partial sum of squares
+#define NS_MAX_STEPS 64
+
+struct NsMat {
+    const void* in;
+    void* out;
+    float* mom;
+    long long in_ld, in_bs, out_ld, out_bs;
+    int rows, cols, batch, type;      // type of `in` (and of `out` where nothing is updated): 0 fp32, 1 bf16, 2 fp16
+    int k, n, kp, np, tall;
+    int tile, kt, nt, tri, splits, chunk;      // product tile; tiles along k and n; tiles on and above the diagonal
+    int sums;                                  // partial sums of squares per matrix
+    float step;
+    half_t *xt[2], *xl, *g, *p;                // planes of matrix 0 of the stack
+    float* part;
+    double* sq;
+    int at[4];      // first workgroup in the launches over: chunks of 16384 elements, 64x64 blocks, G tiles x splits, X tiles
+    int at_p, at_f; // ... over: G / P tiles, 64x64 blocks of G tiles (fold)
+};
+
+// ---- pairs of fp16
+__device__ __forceinline__ void ns_split(float v, half_t& hi, half_t& lo) {
+    const float s = v * NS_SCALE;
+    hi = (half_t)s;
+    lo = (half_t)(s - (float)hi);
+}
+__device__ __forceinline__ void ns_split8(const float* v, half8& hi, half8& lo) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        half_t h, l;
+        ns_split(v[e], h, l);
+        hi[e] = h;
+        lo[e] = l;
+    }
+}
+// element offset of (row, first column of a group of 8) of a plane pair with `cols` padded columns; lo: 32 further
+__device__ __forceinline__ size_t ns_at(size_t row, int col, int cols) {
+    return row * 2 * (size_t)cols + (size_t)(col >> 5) * 64 + (col & 31);
+}
+
+// which matrix a workgroup belongs to: the last whose first workgroup is not behind it (64 candidates a look)
+template <int WHICH>
+__device__ __forceinline__ int ns_first(const NsMat& m) {
+    return WHICH < 4 ? m.at[WHICH & 3] : WHICH == 4 ? m.at_p : m.at_f;
+}
+template <int WHICH>
+__device__ __forceinline__ int ns_find(const NsMat* tab, int count, int wg) {
+    int found = -1;
+    for (int base = 0; base < count; base += 64) {
+        const int i = base + (threadIdx.x & 63);
+        const bool in = i < count && ns_first<WHICH>(tab[i]) <= wg;
+        found += __popcll(__ballot(in));
+    }
+    return __builtin_amdgcn_readfirstlane(found);
+}
+
+__global__ void k_ns_table(NsMat* tab, int base, int count, const NsMat a, const NsMat b, const NsMat c, const NsMat d, const NsMat e,
+                           const NsMat f, const NsMat g, const NsMat h) {
+    const NsMat* all[8] = {&a, &b, &c, &d, &e, &f, &g, &h};
+    for (int i = 0; i < 8; ++i)
+        if ((int)threadIdx.x == i && i < count) tab[base + i] = *all[i];
+}
+
+// ---- the matrix that is orthogonalised
+struct NsUpdate {
+    int on, nesterov;
+    float mu, omu, clip, decay;
+};
+__device__ __forceinline__ float ns_in(const NsMat& m, size_t off) {
+    if (m.type == 0) return ((const float*)m.in)[off];
+    if (m.type == 1) return ld1((const bf16_t*)m.in + off);
+    return (float)((const half_t*)m.in)[off];
+}
+__device__ __forceinline__ float ns_clip(float g, float clip) {      // (NaN stays)
+    if (clip > 0.f) g = g > clip ? clip : g < -clip ? -clip : g;
+    return g;
+}
+
+// sums of squares in 64 bits (neither huge nor tiny entries leave the range), and the momentum's update
+__global__ __launch_bounds__(NS_THREADS) void k_ns_squares(const NsMat* tab, int count, const NsUpdate up) {
+    const NsMat& m = tab[ns_find<0>(tab, count, blockIdx.x)];
+    const int at = blockIdx.x - m.at[0], b = at / m.sums, part = at % m.sums;
+    const size_t total = (size_t)m.rows * m.cols, first = (size_t)part * NS_CHUNK;
+    const size_t last = first + NS_CHUNK < total ? first + NS_CHUNK : total;
+    double s = 0;
+    for (size_t i = first + threadIdx.x; i < last; i += NS_THREADS) {
+        const size_t r = i / m.cols, c = i % m.cols;
+        const size_t off = b * m.in_bs + r * m.in_ld + c;
+        float v = ns_in(m, off);
+        if (up.on) {
+            v = ns_clip(v, up.clip);
+            const float mom = m.mom[i] * up.mu + v * up.omu;
+            m.mom[i] = mom;
+            v = up.nesterov ? v * up.omu + mom * up.mu : mom;
+        }
+        s += (double)v * v;
+    }
+    __shared__ double red[NS_THREADS];
+    red[threadIdx.x] = s;
+    __syncthreads();
+    for (int o = NS_THREADS / 2; o > 0; o >>= 1) {
+        if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) m.sq[(size_t)b * m.sums + part] = red[0];
+}
+
+// X = M / (|M| + eps) as plane pairs in both orders, 64 x 64 of XT's [n][k] at a time
+__global__ __launch_bounds__(NS_THREADS) void k_ns_planes(const NsMat* tab, int count, const NsUpdate up, double eps) {
+    const NsMat& m = tab[ns_find<1>(tab, count, blockIdx.x)];
+    const int kb = m.kp / 64, nb = m.np / 64;
+    int at = blockIdx.x - m.at[1];
+    const int b = at / (kb * nb);
+    at %= kb * nb;
+    const int n0 = at / kb * 64, k0 = at % kb * 64;
+    __shared__ double red[NS_THREADS];
+    __shared__ float tile[64][65];
+    double s = 0;
+    for (int i = threadIdx.x; i < m.sums; i += NS_THREADS) s += m.sq[(size_t)b * m.sums + i];
+    red[threadIdx.x] = s;
+    __syncthreads();
+    for (int o = NS_THREADS / 2; o > 0; o >>= 1) {
+        if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
+        __syncthreads();
+    }
+    const double norm = sqrt(red[0]) + eps;
+    // rows of M along threadIdx / 64, columns along the lanes; tile[n][k]
+    for (int i = threadIdx.x >> 6; i < 64; i += NS_THREADS / 64) {
+        const int j = threadIdx.x & 63;
+        const int r = (m.tall ? n0 : k0) + i, c = (m.tall ? k0 : n0) + j;
+        float v = 0.f;
+        if (r < m.rows && c < m.cols) {
+            v = ns_in(m, b * m.in_bs + r * m.in_ld + c);
+            if (up.on) {
+                v = ns_clip(v, up.clip);
+                const float mom = m.mom[(size_t)r * m.cols + c];
+                v = up.nesterov ? v * up.omu + mom * up.mu : mom;
+            }
+            v = (float)(v / norm);
+        }
+        if (m.tall) tile[i][j] = v;
+        else tile[j][i] = v;
+    }
+    __syncthreads();
+    half_t* xt = m.xt[0] + (size_t)b * m.np * m.kp * 2;
+    half_t* xl = m.xl + (size_t)b * m.np * m.kp * 2;
+    for (int q = threadIdx.x; q < 512; q += NS_THREADS) {
+        const int row = q >> 3, col = (q & 7) * 8;
+        float v[8];
+        half8 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = tile[row][col + e];
+        ns_split8(v, hi, lo);
+        size_t o = ns_at(n0 + row, k0 + col, m.kp);
+        *(half8*)(xt + o) = hi;
+        *(half8*)(xt + o + 32) = lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = tile[col + e][row];
+        ns_split8(v, hi, lo);
+        o = ns_at(k0 + row, n0 + col, m.np);
+        *(half8*)(xl + o) = hi;
+        *(half8*)(xl + o + 32) = lo;
+    }
+}
+
+// ---- T x T tile of A B^T, both plane pairs, columns [c0, c1) (multiples of 32); four waves, a quarter of the tile each.
+// Rows behind a matrix's last are read as its last row and never stored.  LDS: a row's 128 bytes are eight pieces of 16, piece
+// q of row r at place q ^ (r / 2 % 8): the 16 lanes that read one piece of 16 rows together meet each bank once.
+template <int T>
+struct NsTile {
+    static constexpr int S = T / 64;           // 32 x 32 blocks of a wave along each side
+    static constexpr int LOADS = T / 32;       // 16-byte pieces of a thread, per operand and step
+    f32x16 acc[S][S];
+
+    __device__ __forceinline__ void run(const half_t* A, int a0, int a_rows, int a_cols, const half_t* B, int b0, int b_rows,
+                                        int b_cols, int c0, int c1, char* lds) {
+        const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+        const int wr = (wave >> 1) * (T / 2), wc = (wave & 1) * (T / 2);
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+        const uint4 *pa[LOADS], *pb[LOADS];
+        int put[LOADS];
+#pragma unroll
+        for (int l = 0; l < LOADS; ++l) {
+            const int row = l * 32 + (t >> 3), piece = t & 7;
+            pa[l] = (const uint4*)(A + ((size_t)min(a0 + row, a_rows - 1) * a_cols + c0) * 2) + piece;
+            pb[l] = (const uint4*)(B + ((size_t)min(b0 + row, b_rows - 1) * b_cols + c0) * 2) + piece;
+            put[l] = row * 128 + ((piece ^ ((row >> 1) & 7)) << 4);
+        }
+        uint4 ra[LOADS], rb[LOADS];
+#pragma unroll
+        for (int l = 0; l < LOADS; ++l) { ra[l] = *pa[l]; rb[l] = *pb[l]; }
+        int buf = 0;
+        for (int c = c0; c < c1; c += 32) {
+            char* la = lds + buf * (T * 256);
+            char* lb = la + T * 128;
+            buf ^= 1;
+#pragma unroll
+            for (int l = 0; l < LOADS; ++l) {
+                *(uint4*)(la + put[l]) = ra[l];
+                *(uint4*)(lb + put[l]) = rb[l];
+            }
+            __syncthreads();
+            if (c + 32 < c1) {
+#pragma unroll
+                for (int l = 0; l < LOADS; ++l) {
+                    pa[l] += 8;
+                    pb[l] += 8;
+                    ra[l] = *pa[l];
+                    rb[l] = *pb[l];
+                }
+            }
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                half8 ah[S], al[S], bh[S], bl[S];
+#pragma unroll
+                for (int i = 0; i < S; ++i) {
+                    const int r = wr + i * 32 + (lane & 31), q = kk * 2 + (lane >> 5), x = (r >> 1) & 7;
+                    ah[i] = *(half8*)(la + r * 128 + ((q ^ x) << 4));
+                    al[i] = *(half8*)(la + r * 128 + (((q + 4) ^ x) << 4));
+                    const int s = wc + i * 32 + (lane & 31), y = (s >> 1) & 7;
+                    bh[i] = *(half8*)(lb + s * 128 + ((q ^ y) << 4));
+                    bl[i] = *(half8*)(lb + s * 128 + (((q + 4) ^ y) << 4));
+                }
+#pragma unroll
+                for (int i = 0; i < S; ++i)
+#pragma unroll
+                    for (int j = 0; j < S; ++j) {
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], acc[i][j], 0, 0, 0);
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], acc[i][j], 0, 0, 0);
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
+                    }
+            }
+        }
+        __syncthreads();
+    }
+    // the tile's sums into LDS, tile[row][col] with rows T + 1 apart
+    __device__ __forceinline__ void stage(float* tile) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int wr = (wave >> 1) * (T / 2), wc = (wave & 1) * (T / 2);
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int row = wr + i * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5);
+                    tile[row * (T + 1) + wc + j * 32 + (lane & 31)] = acc[i][j][e] * (NS_UNSCALE * NS_UNSCALE);
+                }
+        __syncthreads();
+    }
+};
+
+#define NS_LDS (128 * 129 * 4)      // the larger of two steps' operands (64 KB) and the staged tile
+
+// tile number -> (i, j), i <= j, of a triangle of `t` rows
+__device__ __forceinline__ void ns_pair(int l, int t, int& i, int& j) {
+    i = 0;
+    while (l >= t - i) { l -= t - i; ++i; }
+    j = i + l;
+}
+
+// rows [r0, r0 + T) and columns [c0, c0 + T) of a symmetric plane pair [kp][kp] from the staged tile, and its mirror image
+template <int T>
+__device__ __forceinline__ void ns_symmetric(half_t* out, int kp, int r0, int c0, const float* tile) {
+    for (int q = threadIdx.x; q < T * T / 8; q += NS_THREADS) {
+        const int row = q / (T / 8), col = q % (T / 8) * 8;
+        float v[8];
+        half8 hi, lo;
+        if (r0 + row < kp && c0 + col < kp) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = tile[row * (T + 1) + col + e];
+            ns_split8(v, hi, lo);
+            const size_t o = ns_at(r0 + row, c0 + col, kp);
+            *(half8*)(out + o) = hi;
+            *(half8*)(out + o + 32) = lo;
+        }
+        if (r0 != c0 && c0 + row < kp && r0 + col < kp) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = tile[(col + e) * (T + 1) + row];
+            ns_split8(v, hi, lo);
+            const size_t o = ns_at(c0 + row, r0 + col, kp);
+            *(half8*)(out + o) = hi;
+            *(half8*)(out + o + 32) = lo;
+        }
+    }
+}
+
+// G = XL XL^T, a chunk of n at a time
+template <int T>
+__device__ __forceinline__ void ns_gram(const NsMat& m, int at, char* lds) {
+    const int b = at / (m.tri * m.splits);
+    at %= m.tri * m.splits;
+    const int split = at / m.tri, l = at % m.tri;
+    int i, j;
+    ns_pair(l, m.kt, i, j);
+    const half_t* xl = m.xl + (size_t)b * m.np * m.kp * 2;
+    const int c0 = split * m.chunk, c1 = min(m.np, c0 + m.chunk);
+    NsTile<T> t;
+    t.run(xl, i * T, m.kp, m.np, xl, j * T, m.kp, m.np, c0, c1, lds);
+    float* tile = (float*)lds;
+    t.stage(tile);
+    if (m.splits == 1) {
+        ns_symmetric<T>(m.g + (size_t)b * m.kp * m.kp * 2, m.kp, i * T, j * T, tile);
+    } else {
+        float* out = m.part + (((size_t)b * m.splits + split) * m.tri + l) * (T * T);
+        for (int q = threadIdx.x; q < T * T; q += NS_THREADS) out[q] = tile[q / T * (T + 1) + q % T];
+    }
+}
+__global__ __launch_bounds__(NS_THREADS) void k_ns_gram(const NsMat* tab, int count) {
+    extern __shared__ __align__(16) char lds[];
+    const NsMat& m = tab[ns_find<2>(tab, count, blockIdx.x)];
+    if (m.tile == 128) ns_gram<128>(m, blockIdx.x - m.at[2], lds);
+    else ns_gram<64>(m, blockIdx.x - m.at[2], lds);
+}
+
+// the chunks' sums in order, a 64 x 64 block of a tile
+__global__ __launch_bounds__(NS_THREADS) void k_ns_fold(const NsMat* tab, int count) {
+    const NsMat& m = tab[ns_find<5>(tab, count, blockIdx.x)];
+    __shared__ float tile[64 * 65];
+    const int T = m.tile, sub = T / 64;
+    int at = blockIdx.x - m.at_f;
+    const int b = at / (m.tri * sub * sub);
+    at %= m.tri * sub * sub;
+    const int l = at / (sub * sub), r = at % (sub * sub) / sub * 64, c = at % sub * 64;
+    int i, j;
+    ns_pair(l, m.kt, i, j);
+    if (i == j && c < r) return;      // (its mirror image writes it)
+    const float* in = m.part + ((size_t)b * m.splits * m.tri + l) * (T * T);
+    for (int q = threadIdx.x; q < 1024; q += NS_THREADS) {
+        const int row = q >> 4, col = (q & 15) * 4;
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int p = 0; p < m.splits; ++p) {
+            const float4 v = *(const float4*)(in + (size_t)p * m.tri * (T * T) + (r + row) * T + c + col);
+            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        }
+        float* o = tile + row * 65 + col;
+        o[0] = s.x; o[1] = s.y; o[2] = s.z; o[3] = s.w;
+    }
+    __syncthreads();
+    ns_symmetric<64>(m.g + (size_t)b * m.kp * m.kp * 2, m.kp, i * T + r, j * T + c, tile);
+}
+
+// P = b G + c G G
+template <int T>
+__device__ __forceinline__ void ns_poly(const NsMat& m, int at, float cb, float cc, char* lds) {
+    const int b = at / m.tri;
+    int i, j;
+    ns_pair(at % m.tri, m.kt, i, j);
+    const half_t* g = m.g + (size_t)b * m.kp * m.kp * 2;
+    NsTile<T> t;
+    t.run(g, i * T, m.kp, m.kp, g, j * T, m.kp, m.kp, 0, m.kp, lds);
+    float* tile = (float*)lds;
+    t.stage(tile);
+    for (int q = threadIdx.x; q < T * T / 8; q += NS_THREADS) {
+        const int row = q / (T / 8), col = q % (T / 8) * 8;
+        if (i * T + row >= m.kp || j * T + col >= m.kp) continue;
+        const size_t o = ns_at(i * T + row, j * T + col, m.kp);
+        const half8 hi = *(const half8*)(g + o), lo = *(const half8*)(g + o + 32);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float* v = tile + row * (T + 1) + col + e;
+            *v = cc * *v + cb * (((float)hi[e] + (float)lo[e]) * NS_UNSCALE);
+        }
+    }
+    __syncthreads();
+    ns_symmetric<T>(m.p + (size_t)b * m.kp * m.kp * 2, m.kp, i * T, j * T, tile);
+}
+__global__ __launch_bounds__(NS_THREADS) void k_ns_poly(const NsMat* tab, int count, float cb, float cc) {
+    extern __shared__ __align__(16) char lds[];
+    const NsMat& m = tab[ns_find<4>(tab, count, blockIdx.x)];
+    if (m.tile == 128) ns_poly<128>(m, blockIdx.x - m.at_p, cb, cc, lds);
+    else ns_poly<64>(m, blockIdx.x - m.at_p, cb, cc, lds);
+}
+
+__device__ __forceinline__ void ns_out(const NsMat& m, const NsUpdate& up, int b, int r, int c, float v) {
+    const size_t o = b * m.out_bs + (size_t)r * m.out_ld + c;
+    if (up.on) {
+        float* p = (float*)m.out + o;
+        *p = *p * up.decay - m.step * v;
+    } else if (m.type == 0) {
+        ((float*)m.out)[o] = v;
+    } else if (m.type == 1) {
+        st1((bf16_t*)m.out + o, v);
+    } else {
+        ((half_t*)m.out)[o] = (half_t)v;
+    }
+}
+
+// X <- a X + X P
+template <int T>
+__device__ __forceinline__ void ns_apply(const NsMat& m, int at, int from, float ca, bool last, const NsUpdate& up, char* lds) {
+    const int b = at / (m.nt * m.kt);
+    at %= m.nt * m.kt;
+    const int n0 = at / m.kt * T, k0 = at % m.kt * T;
+    const size_t plane = (size_t)b * m.np * m.kp * 2;
+    const half_t* x = m.xt[from] + plane;
+    NsTile<T> t;
+    t.run(x, n0, m.np, m.kp, m.p + (size_t)b * m.kp * m.kp * 2, k0, m.kp, m.kp, 0, m.kp, lds);
+    float* tile = (float*)lds;
+    t.stage(tile);
+    for (int q = threadIdx.x; q < T * T / 8; q += NS_THREADS) {
+        const int row = q / (T / 8), col = q % (T / 8) * 8;
+        if (n0 + row >= m.np || k0 + col >= m.kp) continue;
+        const size_t o = ns_at(n0 + row, k0 + col, m.kp);
+        const half8 xh = *(const half8*)(x + o), xlo = *(const half8*)(x + o + 32);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float* p = tile + row * (T + 1) + col + e;
+            v[e] = *p + ca * (((float)xh[e] + (float)xlo[e]) * NS_UNSCALE);
+            *p = v[e];
+        }
+        if (!last) {
+            half8 hi, lo;
+            ns_split8(v, hi, lo);
+            half_t* out = m.xt[from ^ 1] + plane + o;
+            *(half8*)out = hi;
+            *(half8*)(out + 32) = lo;
+        }
+    }
+    __syncthreads();
+    if (!last) {
+        half_t* xl = m.xl + plane;
+        for (int q = threadIdx.x; q < T * T / 8; q += NS_THREADS) {
+            const int row = q / (T / 8), col = q % (T / 8) * 8;
+            if (k0 + row >= m.kp || n0 + col >= m.np) continue;
+            float v[8];
+            half8 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = tile[(col + e) * (T + 1) + row];
+            ns_split8(v, hi, lo);
+            const size_t o = ns_at(k0 + row, n0 + col, m.np);
+            *(half8*)(xl + o) = hi;
+            *(half8*)(xl + o + 32) = lo;
+        }
+    } else {
+        for (int q = threadIdx.x; q < T * T; q += NS_THREADS) {      // (lanes along the output's rows)
+            const int i = q / T, j = q % T;
+            const int r = (m.tall ? n0 : k0) + i, c = (m.tall ? k0 : n0) + j;
+            if (r < m.rows && c < m.cols) ns_out(m, up, b, r, c, m.tall ? tile[i * (T + 1) + j] : tile[j * (T + 1) + i]);
+        }
+    }
+}
+__global__ __launch_bounds__(NS_THREADS) void k_ns_apply(const NsMat* tab, int count, int from, float ca, int last,
+                                                         const NsUpdate up) {
+    extern __shared__ __align__(16) char lds[];
+    const NsMat& m = tab[ns_find<3>(tab, count, blockIdx.x)];
+    if (m.tile == 128) ns_apply<128>(m, blockIdx.x - m.at[3], from, ca, last, up, lds);
+    else ns_apply<64>(m, blockIdx.x - m.at[3], from, ca, last, up, lds);
+}
+
+// ---- host side
+// fields of a matrix stack in the callers' table (int64 each)
+enum { NS_IN, NS_OUT, NS_MOM, NS_ROWS, NS_COLS, NS_BATCH, NS_IN_LD, NS_IN_BS, NS_OUT_LD, NS_OUT_BS, NS_TYPE, NS_FIELDS };
+#define NS_MAX_SIDE (1 << 24)
+
+struct NsPlan {
+    size_t bytes;
+    int grid[6];      // chunks, blocks, gram, apply, poly, fold
+};
+
+// One matrix stack's part of the workspace and of the launches.  false: a size that is not taken.
+static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
+    const long long rows = f[NS_ROWS], cols = f[NS_COLS], batch = f[NS_BATCH];
+    if (rows < 1 || cols < 1 || batch < 1 || rows > NS_MAX_SIDE || cols > NS_MAX_SIDE || batch > (1 << 20)) return false;
+    m.in = (const void*)f[NS_IN]; m.out = (void*)f[NS_OUT]; m.mom = (float*)f[NS_MOM];
+    m.in_ld = f[NS_IN_LD]; m.in_bs = f[NS_IN_BS]; m.out_ld = f[NS_OUT_LD]; m.out_bs = f[NS_OUT_BS];
+    m.rows = (int)rows; m.cols = (int)cols; m.batch = (int)batch; m.type = (int)f[NS_TYPE];
+    m.tall = rows >= cols;
+    m.k = m.tall ? m.cols : m.rows;
+    m.n = m.tall ? m.rows : m.cols;
+    if (m.k > 16384) return false;
+    m.kp = agb_cdiv(m.k, 64) * 64;
+    m.np = agb_cdiv(m.n, 64) * 64;
+    m.tile = m.kp >= 256 ? 128 : 64;
+    m.kt = agb_cdiv(m.kp, m.tile);
+    m.nt = agb_cdiv(m.np, m.tile);
+    m.tri = m.kt * (m.kt + 1) / 2;
+    const long long tiles = (long long)m.tri * m.batch;
+    int splits = tiles >= 256 ? 1 : agb_cdiv(256, tiles);
+    if (splits > m.np / 256) splits = m.np / 256;
+    if (splits < 1) splits = 1;
+    m.chunk = agb_cdiv(agb_cdiv(m.np, splits), 32) * 32;
+    m.splits = agb_cdiv(m.np, m.chunk);
+    m.sums = agb_cdiv((long long)rows * cols, NS_CHUNK);
+    const size_t x = (size_t)m.np * m.kp * 4 * batch, g = (size_t)m.kp * m.kp * 4 * batch;
+    auto take = [&](size_t n) {
+        char* p = ws ? ws + plan.bytes : nullptr;
+        plan.bytes += (n + 255) / 256 * 256;
+        return p;
+    };
+    m.xt[0] = (half_t*)take(x);
+    m.xt[1] = (half_t*)take(x);
+    m.xl = (half_t*)take(x);
+    m.g = (half_t*)take(g);
+    m.p = (half_t*)take(g);
+    m.part = (float*)take(m.splits > 1 ? (size_t)m.splits * tiles * m.tile * m.tile * 4 : 0);
+    m.sq = (double*)take((size_t)m.sums * batch * 8);
+    const long long wgs[6] = {(long long)m.sums * batch, (long long)(m.kp / 64) * (m.np / 64) * batch, tiles * m.splits,
+                              (long long)m.kt * m.nt * batch, tiles,
+                              m.splits > 1 ? tiles * (m.tile / 64) * (m.tile / 64) : 0};
+    int* at[6] = {&m.at[0], &m.at[1], &m.at[2], &m.at[3], &m.at_p, &m.at_f};
+    for (int i = 0; i < 6; ++i) {
+        *at[i] = plan.grid[i];
+        if (plan.grid[i] + wgs[i] > 0x7fffffff) return false;
+        plan.grid[i] += (int)wgs[i];
+    }
+    return true;
+}
+
+// Largest |sigma| along the iterations from [0, 1], and largest |b s^2 + c s^4|: both are entries' bounds of what is held as
+// fp16 pairs.
+static bool ns_bounded(const float* coef, int steps) {
+    double hi = 1.0;
+    for (int i = 0; i < steps; ++i) {
+        const double a = coef[3 * i], b = coef[3 * i + 1], c = coef[3 * i + 2];
+        double next = 0;
+        if (!(hi * hi < 7)) return false;
+        for (int s = 0; s <= 256; ++s) {
+            const double x = hi * s / 256, q = b * x * x + c * x * x * x * x, v = x * (a + q);
+            if (!(q < 7 && q > -7)) return false;
+            const double w = v < 0 ? -v : v;
+            if (!(w <= 7)) return false;
+            next = w > next ? w : next;
+        }
+        hi = next * 1.001 + 1e-3;
+    }
+    return true;
+}
+
+static int ns_run(const char* name, const long long* fields, int count, int steps, const float* coef, double eps, const float* step,
+                  const NsUpdate& up, void* workspace, size_t workspace_bytes, hipStream_t st) {
+    AGB_CHECK_ARG(count >= 0 && (count == 0 || fields), "%s: %d matrices", name, count);
+    AGB_CHECK_ARG(steps >= 1 && steps <= NS_MAX_STEPS && coef, "%s: %d steps (1 to %d)", name, steps, NS_MAX_STEPS);
+    AGB_CHECK_ARG(ns_bounded(coef, steps), "%s: the coefficients let singular values grow past 7 (or hi^2 past 7)", name);
+    AGB_CHECK_ARG(eps >= 0, "%s: eps", name);
+    if (count == 0) return AGB_OK;
+    NsPlan plan = {};
+    const size_t table = ((size_t)count * sizeof(NsMat) + 255) / 256 * 256;
+    plan.bytes = table;
+    NsMat m[8];
+    // sizes first: nothing is enqueued before everything has been looked at
+    for (int i = 0; i < count; ++i) {
+        const long long* f = fields + (size_t)i * NS_FIELDS;
+        AGB_CHECK_ARG(ns_plan(f, m[0], nullptr, plan), "%s: matrix %d: [%lld, %lld, %lld] is not taken", name, i, f[NS_BATCH],
+                      f[NS_ROWS], f[NS_COLS]);
+        AGB_CHECK_ARG(m[0].in && m[0].out && (!up.on || m[0].mom), "%s: matrix %d: null pointer", name, i);
+        AGB_CHECK_ARG(m[0].type >= 0 && m[0].type <= 2, "%s: matrix %d: type %d", name, i, m[0].type);
+        AGB_CHECK_ARG(m[0].in_ld >= m[0].cols && m[0].out_ld >= m[0].cols, "%s: matrix %d: row stride", name, i);
+        AGB_CHECK_ARG(!up.on || m[0].batch == 1, "%s: matrix %d: updates take one matrix each", name, i);
+    }
+    AGB_CHECK_ARG(workspace && workspace_bytes >= plan.bytes, "%s: workspace of %zu bytes, %zu needed", name, workspace_bytes,
+                  plan.bytes);
+    NsMat* tab = (NsMat*)workspace;
+    plan = {};
+    plan.bytes = table;
+    for (int base = 0; base < count; base += 8) {
+        const int some = count - base < 8 ? count - base : 8;
+        for (int i = 0; i < 8; ++i) m[i] = {};
+        for (int i = 0; i < some; ++i) {
+            ns_plan(fields + (size_t)(base + i) * NS_FIELDS, m[i], (char*)workspace, plan);
+            m[i].step = step ? step[base + i] : 0.f;
+        }
+        hipLaunchKernelGGL(k_ns_table, dim3(1), dim3(64), 0, st, tab, base, some, m[0], m[1], m[2], m[3], m[4], m[5], m[6], m[7]);
+        AGB_CHECK_LAUNCH(name);
+    }
+    for (const void* k : {(const void*)k_ns_gram, (const void*)k_ns_poly, (const void*)k_ns_apply}) {
+        const hipError_t e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, NS_LDS);
+        if (e != hipSuccess) { agb_set_error("%s: %s", name, hipGetErrorString(e)); return AGB_ELAUNCH; }
+    }
+    hipLaunchKernelGGL(k_ns_squares, dim3(plan.grid[0]), dim3(NS_THREADS), 0, st, tab, count, up);
+    hipLaunchKernelGGL(k_ns_planes, dim3(plan.grid[1]), dim3(NS_THREADS), 0, st, tab, count, up, eps);
+    for (int i = 0; i < steps; ++i) {
+        hipLaunchKernelGGL(k_ns_gram, dim3(plan.grid[2]), dim3(NS_THREADS), NS_LDS, st, tab, count);
+        if (plan.grid[5]) hipLaunchKernelGGL(k_ns_fold, dim3(plan.grid[5]), dim3(NS_THREADS), 0, st, tab, count);
+        hipLaunchKernelGGL(k_ns_poly, dim3(plan.grid[4]), dim3(NS_THREADS), NS_LDS, st, tab, count, coef[3 * i + 1],
+                           coef[3 * i + 2]);
+        hipLaunchKernelGGL(k_ns_apply, dim3(plan.grid[3]), dim3(NS_THREADS), NS_LDS, st, tab, count, i & 1, coef[3 * i],
+                           i == steps - 1, up);
+    }
+    AGB_CHECK_LAUNCH(name);
+    return AGB_OK;
+}
+
+extern "C" {
+
+int agb_ns_fields(void) { return NS_FIELDS; }
+
+size_t agb_ns_workspace_bytes(const long long* fields, int count) {
+    if (count < 1 || !fields) return 0;
+    NsPlan plan = {};
+    plan.bytes = ((size_t)count * sizeof(NsMat) + 255) / 256 * 256;
+    NsMat m;
+    for (int i = 0; i < count; ++i)
+        if (!ns_plan(fields + (size_t)i * NS_FIELDS, m, nullptr, plan)) return 0;
+    return plan.bytes;
+}
+
+int agb_orthogonalize(const long long* fields, int count, int steps, const float* coef, double eps, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+    const NsUpdate up = {};
+    return ns_run("agb_orthogonalize", fields, count, steps, coef, eps, nullptr, up, workspace, workspace_bytes,
+                  (hipStream_t)stream);
+}
+
+int agb_muon_update(const long long* fields, int count, int steps, const float* coef, double eps, const float* step, double decay,
+                    double momentum, int nesterov, float clip, void* workspace, size_t workspace_bytes, void* stream) {
+    AGB_CHECK_ARG(count == 0 || step, "agb_muon_update: null pointer");
+    AGB_CHECK_ARG(momentum >= 0 && momentum < 1, "agb_muon_update: momentum %g", momentum);
+    NsUpdate up;
+    up.on = 1;
+    up.nesterov = nesterov != 0;
+    up.mu = (float)momentum;
+    up.omu = (float)(1 - momentum);      // (1 - momentum in double: 1 - 0.95f is not 0.05f)
+    up.clip = clip;
+    up.decay = (float)decay;
+    return ns_run("agb_muon_update", fields, count, steps, coef, eps, step, up, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -16,7 +16,7 @@ import numpy as np
 import torch
 import torch.nn.functional as F
 
-from ..optim import AdaBelief
+from ..optim import AdaBelief, Muon
 
 REG_LOSSES = {"smoothl1": F.smooth_l1_loss, "l2": F.mse_loss, "l1": F.l1_loss}
 OUT_ACT = {"linear": lambda x: x, "elu": F.elu, "relu": F.relu}
@@ -159,9 +159,9 @@ class InstanceBase(torch.nn.Module):
         opt = training.optim.optimizer
         name = opt.get("name", opt.get("class", "AdaBelief"))
         params = dict(opt.get("params", {}))
-        cls = AdaBelief if name == "AdaBelief" else getattr(torch.optim, name)
+        cls = {"AdaBelief": AdaBelief, "Muon": Muon}.get(name) or getattr(torch.optim, name)
         self._grad_clip = training.get("grad_clip", -1)
-        if cls is AdaBelief and torch.cuda.is_available() and next(self.parameters()).is_cuda:
+        if cls in (AdaBelief, Muon) and torch.cuda.is_available() and next(self.parameters()).is_cuda:
             # one fused HIP launch per parameter group, gradient clip folded in
             params.update(fused=True, clip_value=self._grad_clip if self._grad_clip > 0 else None)
         self._optimizer = cls(self.get_parameter_list(), **params)

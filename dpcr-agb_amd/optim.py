@@ -47,6 +47,10 @@ class AdaBelief(Optimizer):
             step_size = -1
         return num_sma, step_size
 
+    def _element_wise(self, group):
+        """The parameters of a group that take this class's update."""
+        return group["params"]
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -55,7 +59,7 @@ class AdaBelief(Optimizer):
                 loss = closure()
         for group in self.param_groups:
             params, grads, m, v = [], [], [], []
-            for p in group["params"]:
+            for p in self._element_wise(group):
                 if p.grad is None:
                     continue
                 if p.grad.is_sparse:
@@ -181,3 +185,62 @@ class AdaBelief(Optimizer):
         # (the parameters were rewritten through raw pointers: torch's version counters did not move)
         from .sparse_ops import bump_weight_epoch
         bump_weight_epoch()
+
+
+class Muon(AdaBelief):
+    """Weight matrices along their orthogonalised momentum (muon_ops.muon_update, csrc/muon.hip), everything else — biases, norm
+    weights, single rows — by AdaBelief with this class's AdaBelief arguments.
+
+    A parameter is a matrix with its leading axes merged: a convolution kernel [offsets, Cin, Cout] is [offsets * Cin, Cout].
+    A group with ``muon=False`` (a head, an embedding) is left to AdaBelief altogether.  ``adjust``: muon_ops.adjust_factor; with
+    "rms" the learning rate and weight decay of an Adam-like optimiser carry over.  ``clip_value`` limits gradient elements, in both
+    updates.  State: ``momentum_buffer`` of matrices, AdaBelief's of the others.  All matrices of a group go through the same
+    launches (20 to 30 in all, whatever their number)."""
+
+    def __init__(self, params, lr=1e-3, momentum=0.95, nesterov=True, ns_steps=5, ns_coefficients=None, ns_eps=1e-7, adjust="rms",
+                 **adabelief):
+        from .muon_ops import COEFFICIENTS, MAX_STEPS, adjust_factor
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError(f"Invalid momentum: {momentum}")
+        if not 1 <= ns_steps <= MAX_STEPS:
+            raise ValueError(f"Invalid number of Newton-Schulz steps: {ns_steps}")
+        adjust_factor(adjust, 2, 2)
+        super().__init__(params, lr=lr, **adabelief)
+        mine = dict(momentum=momentum, nesterov=nesterov, ns_steps=ns_steps, ns_eps=ns_eps, adjust=adjust, muon=True,
+                    ns_coefficients=tuple(ns_coefficients) if ns_coefficients is not None else COEFFICIENTS)
+        self.defaults.update(mine)
+        for group in self.param_groups:
+            for k, v in mine.items():
+                group.setdefault(k, v)
+
+    @staticmethod
+    def _is_matrix(p):
+        from .muon_ops import matrix_shape
+        return matrix_shape(p) is not None
+
+    def _element_wise(self, group):
+        return [p for p in group["params"] if not (group["muon"] and self._is_matrix(p))]
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        from .muon_ops import _update
+        loss = super().step(closure)
+        for group in self.param_groups:
+            if not group["muon"]:
+                continue
+            params = [p for p in group["params"] if p.grad is not None and self._is_matrix(p)]
+            if any(p.grad.is_sparse for p in params):
+                raise RuntimeError("Muon does not support sparse gradients")
+            if not params:
+                continue
+            momenta = []
+            for p in params:
+                st = self.state[p]
+                if "momentum_buffer" not in st:
+                    st["momentum_buffer"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+                momenta.append(st["momentum_buffer"])
+            lr, wd = group["lr"], group["weight_decay"]
+            decay = 1.0 - (wd if group["fixed_decay"] else lr * wd)
+            _update(params, [p.grad for p in params], momenta, lr, decay, group["momentum"], group["nesterov"], group["ns_steps"],
+                    group["ns_coefficients"], group["ns_eps"], group["adjust"], self.clip_value)
+        return loss

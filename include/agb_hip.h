@@ -573,6 +573,23 @@ int agb_adabelief_step(const void* descs, const int32_t* chunk_tensor, const int
                        float decay, float beta1, float beta2, float one_minus_beta1, float one_minus_beta2, float eps,
                        float step, float inv_sqrt_bc2, int mode, float clip, void* stream);
 
+/* Orthogonalised updates.  X = M / (|M|_F + eps), then `steps` times X <- a X + (b G + c G G) X with G = X X^T; coef (host)
+ * float[steps][3] = (a, b, c), such that singular values from [0, 1] keep sigma^2 and |b sigma^2 + c sigma^4| below 7.
+ * fields (host): int64[count][agb_ns_fields()] of matrix stacks: input, output, momentum (device addresses), rows, cols, number of
+ * matrices, row stride and matrix stride of the input and of the output (elements), type of input and output (0 fp32, 1 bf16,
+ * 2 fp16).  Columns are adjacent; rows, cols <= 2^24, the shorter <= 16384.  All stacks share the launches; the table travels in
+ * kernel arguments (nothing on the host is read after the call returns).  workspace: agb_ns_workspace_bytes (0: a size that is
+ * not taken).  agb_orthogonalize: input may be output.
+ * agb_muon_update: one matrix per entry; input = gradient g (clipped to +-clip where clip > 0), output = fp32 parameter p,
+ * momentum fp32 contiguous m:  m <- momentum m + (1 - momentum) g;  M = nesterov ? (1 - momentum) g + momentum m : m;
+ * p <- decay p - step[i] X (step: host float[count]).  No tensor may appear twice. */
+int agb_ns_fields(void);                                                    /* host helper */
+size_t agb_ns_workspace_bytes(const long long* fields, int count);          /* host helper */
+int agb_orthogonalize(const long long* fields, int count, int steps, const float* coef, double eps, void* workspace,
+                      size_t workspace_bytes, void* stream);
+int agb_muon_update(const long long* fields, int count, int steps, const float* coef, double eps, const float* step, double decay,
+                    double momentum, int nesterov, float clip, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- NFI transform chain on the device (dpcr-agb_amd/csrc/transform.hip) -------------------------------------------
  * Replaces, for a whole batch, the per-sample CPU transforms of conf/data/instance/NFI/transforms/sparse-xy.yaml:
  * ScalePos, MoveCenterPosPerSample, StartZFromZero (core/data_transform/transforms.py:590-598,722-739,766-769),
