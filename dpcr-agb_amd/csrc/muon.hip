@@ -26,23 +26,24 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 #define NS_THREADS 256
 #define NS_SCALE 8192.f
 #define NS_UNSCALE (1.f / 8192.f)
-#define NS_CHUNK 16384      // elements of one partial sum of squares
+#define NS_CHUNK 4096       // elements of one partial sum of squares
 #define NS_MAX_STEPS 64
 
-struct NsMat {
+struct __attribute__((aligned(16))) NsMat {
     const void* in;
     void* out;
     float* mom;
     long long in_ld, in_bs, out_ld, out_bs;
     int rows, cols, batch, type;      // type of `in` (and of `out` where nothing is updated): 0 fp32, 1 bf16, 2 fp16
     int k, n, kp, np, tall;
+    int vec;                          // contiguous and aligned: four elements at a time
     int tile, kt, nt, tri, splits, chunk;      // product tile; tiles along k and n; tiles on and above the diagonal
     int sums;                                  // partial sums of squares per matrix
     float step;
     half_t *xt[2], *xl, *g, *p;                // planes of matrix 0 of the stack
     float* part;
     double* sq;
-    int at[4];      // first workgroup in the launches over: chunks of 16384 elements, 64x64 blocks, G tiles x splits, X tiles
+    int at[4];      // first workgroup in the launches over: chunks of 4096 elements, 64x64 blocks, G tiles x splits, X tiles
     int at_p, at_f; // ... over: G / P tiles, 64x64 blocks of G tiles (fold)
 };
 
@@ -82,11 +83,16 @@ __device__ __forceinline__ int ns_find(const NsMat* tab, int count, int wg) {
     return __builtin_amdgcn_readfirstlane(found);
 }
 
-__global__ void k_ns_table(NsMat* tab, int base, int count, const NsMat a, const NsMat b, const NsMat c, const NsMat d, const NsMat e,
-                           const NsMat f, const NsMat g, const NsMat h) {
-    const NsMat* all[8] = {&a, &b, &c, &d, &e, &f, &g, &h};
-    for (int i = 0; i < 8; ++i)
-        if ((int)threadIdx.x == i && i < count) tab[base + i] = *all[i];
+// The table's way to the device: by value, in kernel arguments (a captured call keeps its own), copied by all lanes at once.
+#define NS_TABLE 16
+struct NsTable {
+    NsMat m[NS_TABLE];
+};
+static_assert(sizeof(NsTable) < 3900 && sizeof(NsMat) % 16 == 0, "kernel arguments hold 4 KB");
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+__global__ __launch_bounds__(256) void k_ns_table(const NsTable t, u32x4* tab, int pieces) {
+    const auto* from = (const __attribute__((address_space(4))) u32x4*)__builtin_amdgcn_kernarg_segment_ptr();      // (t: the first)
+    if ((int)threadIdx.x < pieces) tab[threadIdx.x] = from[threadIdx.x];
 }
 
 // ---- the matrix that is orthogonalised
@@ -99,6 +105,17 @@ __device__ __forceinline__ float ns_in(const NsMat& m, size_t off) {
     if (m.type == 1) return ld1((const bf16_t*)m.in + off);
     return (float)((const half_t*)m.in)[off];
 }
+__device__ __forceinline__ void ns_in4(const NsMat& m, size_t off, float* v) {      // (aligned)
+    float4 q;
+    if (m.type == 0) q = ld4((const float*)m.in + off);
+    else if (m.type == 1) q = ld4((const bf16_t*)m.in + off);
+    else {
+        typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+        const half4 h = *(const half4*)((const half_t*)m.in + off);
+        q = make_float4((float)h[0], (float)h[1], (float)h[2], (float)h[3]);
+    }
+    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+}
 __device__ __forceinline__ float ns_clip(float g, float clip) {      // (NaN stays)
     if (clip > 0.f) g = g > clip ? clip : g < -clip ? -clip : g;
     return g;
@@ -108,20 +125,47 @@ __device__ __forceinline__ float ns_clip(float g, float clip) {      // (NaN sta
 __global__ __launch_bounds__(NS_THREADS) void k_ns_squares(const NsMat* tab, int count, const NsUpdate up) {
     const NsMat& m = tab[ns_find<0>(tab, count, blockIdx.x)];
     const int at = blockIdx.x - m.at[0], b = at / m.sums, part = at % m.sums;
-    const size_t total = (size_t)m.rows * m.cols, first = (size_t)part * NS_CHUNK;
-    const size_t last = first + NS_CHUNK < total ? first + NS_CHUNK : total;
+    const long long total = (long long)m.rows * m.cols, first = (long long)part * NS_CHUNK;
+    const long long last = first + NS_CHUNK < total ? first + NS_CHUNK : total;
+    const bool linear = m.in_ld == m.cols;
+    const long long base = b * m.in_bs;
     double s = 0;
-    for (size_t i = first + threadIdx.x; i < last; i += NS_THREADS) {
-        const size_t r = i / m.cols, c = i % m.cols;
-        const size_t off = b * m.in_bs + r * m.in_ld + c;
-        float v = ns_in(m, off);
-        if (up.on) {
-            v = ns_clip(v, up.clip);
-            const float mom = m.mom[i] * up.mu + v * up.omu;
-            m.mom[i] = mom;
-            v = up.nesterov ? v * up.omu + mom * up.mu : mom;
+    for (long long i0 = first + threadIdx.x * 4; i0 < last; i0 += NS_THREADS * 4) {
+        float v[4], mom[4];
+        const bool whole = m.vec && i0 + 4 <= last;
+        if (whole) {
+            ns_in4(m, base + i0, v);
+            if (up.on) {
+                const float4 q = *(const float4*)(m.mom + i0);
+                mom[0] = q.x; mom[1] = q.y; mom[2] = q.z; mom[3] = q.w;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const long long i = i0 + e;
+                v[e] = mom[e] = 0.f;
+                if (i >= last) continue;
+                v[e] = ns_in(m, linear ? base + i : base + i / m.cols * m.in_ld + i % m.cols);
+                if (up.on) mom[e] = m.mom[i];
+            }
         }
-        s += (double)v * v;
+        if (up.on) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = ns_clip(v[e], up.clip);
+                mom[e] = mom[e] * up.mu + v[e] * up.omu;
+                v[e] = up.nesterov ? v[e] * up.omu + mom[e] * up.mu : mom[e];
+            }
+            if (whole) {
+                *(float4*)(m.mom + i0) = make_float4(mom[0], mom[1], mom[2], mom[3]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (i0 + e < last) m.mom[i0 + e] = mom[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s += (double)v[e] * v[e];
     }
     __shared__ double red[NS_THREADS];
     red[threadIdx.x] = s;
@@ -191,18 +235,26 @@ __global__ __launch_bounds__(NS_THREADS) void k_ns_planes(const NsMat* tab, int 
     }
 }
 
-// ---- T x T tile of A B^T, both plane pairs, columns [c0, c1) (multiples of 32); four waves, a quarter of the tile each.
-// Rows behind a matrix's last are read as its last row and never stored.  LDS: a row's 128 bytes are eight pieces of 16, piece
-// q of row r at place q ^ (r / 2 % 8): the 16 lanes that read one piece of 16 rows together meet each bank once.
+// ---- T x T tile of A B^T, both plane pairs, columns [c0, c1) (multiples of 64); four waves, a quarter of the tile each.
+// A step takes 32 columns (T = 128) or 64 (T = 64: as many bytes) straight from global memory to LDS, 16 bytes a lane, one step
+// ahead of the products; the fragments of a step are read before the next step's transfers are issued, so that the wait for
+// those stands at the next step's start.  Rows behind a matrix's last are read as its last row and never stored.  LDS: a row's
+// 128 bytes of 32 columns are eight pieces of 16, piece q of row r at place q ^ (r / 2 % 8): the 16 lanes that read one piece
+// of 16 rows together meet each bank once.
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef const __attribute__((address_space(1))) void* glb_ptr;
+
 template <int T>
 struct NsTile {
     static constexpr int S = T / 64;           // 32 x 32 blocks of a wave along each side
-    static constexpr int LOADS = T / 32;       // 16-byte pieces of a thread, per operand and step
+    static constexpr int KS = 128 / T;         // blocks of 32 columns of a step
+    static constexpr int LOADS = T / 32;       // 16-byte transfers of a lane, per operand and block
+    static constexpr int HALF = T * 128 * KS;  // bytes of an operand's step
     f32x16 acc[S][S];
 
     __device__ __forceinline__ void run(const half_t* A, int a0, int a_rows, int a_cols, const half_t* B, int b0, int b_rows,
                                         int b_cols, int c0, int c1, char* lds) {
-        const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+        const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
         const int wr = (wave >> 1) * (T / 2), wc = (wave & 1) * (T / 2);
 #pragma unroll
         for (int i = 0; i < S; ++i)
@@ -210,58 +262,70 @@ struct NsTile {
             for (int j = 0; j < S; ++j)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-        const uint4 *pa[LOADS], *pb[LOADS];
-        int put[LOADS];
+        const char* base_a = (const char*)(A + (size_t)c0 * 2);
+        const char* base_b = (const char*)(B + (size_t)c0 * 2);
+        size_t off_a[LOADS], off_b[LOADS];
 #pragma unroll
         for (int l = 0; l < LOADS; ++l) {
-            const int row = l * 32 + (t >> 3), piece = t & 7;
-            pa[l] = (const uint4*)(A + ((size_t)min(a0 + row, a_rows - 1) * a_cols + c0) * 2) + piece;
-            pb[l] = (const uint4*)(B + ((size_t)min(b0 + row, b_rows - 1) * b_cols + c0) * 2) + piece;
-            put[l] = row * 128 + ((piece ^ ((row >> 1) & 7)) << 4);
+            const int row = (wave * LOADS + l) * 8 + (lane >> 3), piece = (lane & 7) ^ ((row >> 1) & 7);
+            off_a[l] = (size_t)min(a0 + row, a_rows - 1) * a_cols * 4 + piece * 16;
+            off_b[l] = (size_t)min(b0 + row, b_rows - 1) * b_cols * 4 + piece * 16;
         }
-        uint4 ra[LOADS], rb[LOADS];
+        auto fetch = [&](char* to, int step) {
 #pragma unroll
-        for (int l = 0; l < LOADS; ++l) { ra[l] = *pa[l]; rb[l] = *pb[l]; }
-        int buf = 0;
-        for (int c = c0; c < c1; c += 32) {
-            char* la = lds + buf * (T * 256);
-            char* lb = la + T * 128;
-            buf ^= 1;
-#pragma unroll
-            for (int l = 0; l < LOADS; ++l) {
-                *(uint4*)(la + put[l]) = ra[l];
-                *(uint4*)(lb + put[l]) = rb[l];
-            }
-            __syncthreads();
-            if (c + 32 < c1) {
+            for (int s = 0; s < KS; ++s)
 #pragma unroll
                 for (int l = 0; l < LOADS; ++l) {
-                    pa[l] += 8;
-                    pb[l] += 8;
-                    ra[l] = *pa[l];
-                    rb[l] = *pb[l];
+                    char* dst = to + s * (T * 128) + (wave * LOADS + l) * 1024;
+                    const size_t c = (size_t)(step * KS + s) * 128;
+                    __builtin_amdgcn_global_load_lds((glb_ptr)(base_a + c + off_a[l]), (lds_ptr)dst, 16, 0, 0);
+                    __builtin_amdgcn_global_load_lds((glb_ptr)(base_b + c + off_b[l]), (lds_ptr)(dst + HALF), 16, 0, 0);
                 }
-            }
+        };
+        int at_a[S][2], at_b[S][2];
+#pragma unroll
+        for (int i = 0; i < S; ++i)
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
-                half8 ah[S], al[S], bh[S], bl[S];
+                const int q = kk * 2 + (lane >> 5), r = wr + i * 32 + (lane & 31), c = wc + i * 32 + (lane & 31);
+                at_a[i][kk] = r * 128 + ((q ^ ((r >> 1) & 7)) << 4);          // (lo: the place with bit 2 of the piece flipped)
+                at_b[i][kk] = HALF + c * 128 + ((q ^ ((c >> 1) & 7)) << 4);
+            }
+        const int steps = (c1 - c0) / (32 * KS);
+        fetch(lds, 0);
+        for (int step = 0; step < steps; ++step) {
+            const char* now = lds + (step & 1) * (2 * HALF);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            half8 ah[KS * 2][S], al[KS * 2][S], bh[KS * 2][S], bl[KS * 2][S];
+#pragma unroll
+            for (int k = 0; k < KS * 2; ++k)
 #pragma unroll
                 for (int i = 0; i < S; ++i) {
-                    const int r = wr + i * 32 + (lane & 31), q = kk * 2 + (lane >> 5), x = (r >> 1) & 7;
-                    ah[i] = *(half8*)(la + r * 128 + ((q ^ x) << 4));
-                    al[i] = *(half8*)(la + r * 128 + (((q + 4) ^ x) << 4));
-                    const int s = wc + i * 32 + (lane & 31), y = (s >> 1) & 7;
-                    bh[i] = *(half8*)(lb + s * 128 + ((q ^ y) << 4));
-                    bl[i] = *(half8*)(lb + s * 128 + (((q + 4) ^ y) << 4));
+                    const char* blk = now + (k >> 1) * (T * 128);
+                    ah[k][i] = *(const half8*)(blk + at_a[i][k & 1]);
+                    al[k][i] = *(const half8*)(blk + (at_a[i][k & 1] ^ 64));
+                    bh[k][i] = *(const half8*)(blk + at_b[i][k & 1]);
+                    bl[k][i] = *(const half8*)(blk + (at_b[i][k & 1] ^ 64));
                 }
+            if (step + 1 < steps) fetch(lds + ((step + 1) & 1) * (2 * HALF), step + 1);
+#pragma unroll
+            for (int k = 0; k < KS * 2; ++k) {
 #pragma unroll
                 for (int i = 0; i < S; ++i)
 #pragma unroll
-                    for (int j = 0; j < S; ++j) {
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], acc[i][j], 0, 0, 0);
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], acc[i][j], 0, 0, 0);
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
-                    }
+                    for (int j = 0; j < S; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[k][i], bh[k][j], acc[i][j], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < S; ++i)
+#pragma unroll
+                    for (int j = 0; j < S; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[k][i], bl[k][j], acc[i][j], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < S; ++i)
+#pragma unroll
+                    for (int j = 0; j < S; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[k][i], bh[k][j], acc[i][j], 0, 0, 0);
             }
         }
         __syncthreads();
@@ -500,6 +564,7 @@ static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
     m.in_ld = f[NS_IN_LD]; m.in_bs = f[NS_IN_BS]; m.out_ld = f[NS_OUT_LD]; m.out_bs = f[NS_OUT_BS];
     m.rows = (int)rows; m.cols = (int)cols; m.batch = (int)batch; m.type = (int)f[NS_TYPE];
     m.tall = rows >= cols;
+    m.vec = m.in_ld == cols && m.in_bs % 4 == 0 && f[NS_IN] % 16 == 0 && f[NS_MOM] % 16 == 0;
     m.k = m.tall ? m.cols : m.rows;
     m.n = m.tall ? m.rows : m.cols;
     if (m.k > 16384) return false;
@@ -513,7 +578,7 @@ static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
     int splits = tiles >= 256 ? 1 : agb_cdiv(256, tiles);
     if (splits > m.np / 256) splits = m.np / 256;
     if (splits < 1) splits = 1;
-    m.chunk = agb_cdiv(agb_cdiv(m.np, splits), 32) * 32;
+    m.chunk = agb_cdiv(agb_cdiv(m.np, splits), 64) * 64;
     m.splits = agb_cdiv(m.np, m.chunk);
     m.sums = agb_cdiv((long long)rows * cols, NS_CHUNK);
     const size_t x = (size_t)m.np * m.kp * 4 * batch, g = (size_t)m.kp * m.kp * 4 * batch;
@@ -571,7 +636,8 @@ static int ns_run(const char* name, const long long* fields, int count, int step
     NsPlan plan = {};
     const size_t table = ((size_t)count * sizeof(NsMat) + 255) / 256 * 256;
     plan.bytes = table;
-    NsMat m[8];
+    NsTable t;
+    NsMat* m = t.m;
     // sizes first: nothing is enqueued before everything has been looked at
     for (int i = 0; i < count; ++i) {
         const long long* f = fields + (size_t)i * NS_FIELDS;
@@ -587,14 +653,14 @@ static int ns_run(const char* name, const long long* fields, int count, int step
     NsMat* tab = (NsMat*)workspace;
     plan = {};
     plan.bytes = table;
-    for (int base = 0; base < count; base += 8) {
-        const int some = count - base < 8 ? count - base : 8;
-        for (int i = 0; i < 8; ++i) m[i] = {};
+    for (int base = 0; base < count; base += NS_TABLE) {
+        const int some = count - base < NS_TABLE ? count - base : NS_TABLE;
+        t = {};
         for (int i = 0; i < some; ++i) {
             ns_plan(fields + (size_t)(base + i) * NS_FIELDS, m[i], (char*)workspace, plan);
             m[i].step = step ? step[base + i] : 0.f;
         }
-        hipLaunchKernelGGL(k_ns_table, dim3(1), dim3(64), 0, st, tab, base, some, m[0], m[1], m[2], m[3], m[4], m[5], m[6], m[7]);
+        hipLaunchKernelGGL(k_ns_table, dim3(1), dim3(256), 0, st, t, (u32x4*)(tab + base), (int)(some * sizeof(NsMat) / 16));
         AGB_CHECK_LAUNCH(name);
     }
     for (const void* k : {(const void*)k_ns_gram, (const void*)k_ns_poly, (const void*)k_ns_apply}) {
