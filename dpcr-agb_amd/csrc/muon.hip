@@ -12,11 +12,11 @@
 // still keeps its 22 bits.  a X is added in fp32 behind the products: folded into P's diagonal it would cost the small
 // directions two more bits.
 //
-// Layout: X is held twice, XT [n][k] and XL [k][n], so that every product reads both operands along their rows (G: XL XL^T,
-// P: G G^T with G symmetric, X P: XT P^T with P symmetric); both are written by the product that makes them, through an LDS
-// tile.  A row is cut into blocks of 32: 32 hi, then 32 lo — 128 contiguous bytes, what one step of a product takes of it.
-// Rows and blocks are padded to multiples of 64 with zeros, which the iteration keeps zero.  G and P are symmetric: only tiles
-// on and above the diagonal are computed.  G has few tiles and a long sum: it is split over n into chunks, folded in order.
+// Layout: X is held as [n][k] (the longer side down), so X P reads both operands along their rows (P is symmetric), and G = X^T X
+// reads X down its columns: those fragments are transposed by the LDS reads.  A row is cut into blocks of 32: 32 hi, then 32 lo —
+// 128 contiguous bytes.  Rows and blocks are padded to multiples of 64 with zeros, which the iteration keeps zero.  G and P are
+// symmetric: only tiles on and above the diagonal are computed.  G has few tiles and a long sum: it is split over n into chunks,
+// folded in order.
 #include "agb_common.h"
 
 typedef _Float16 half_t;
@@ -24,6 +24,7 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 #define NS_THREADS 256
+#define NS_WIDE 512           // threads of a product's workgroup
 #define NS_SCALE 8192.f
 #define NS_UNSCALE (1.f / 8192.f)
 #define NS_CHUNK 4096       // elements of one partial sum of squares
@@ -37,14 +38,15 @@ struct __attribute__((aligned(16))) NsMat {
     int rows, cols, batch, type;      // type of `in` (and of `out` where nothing is updated): 0 fp32, 1 bf16, 2 fp16
     int k, n, kp, np, tall;
     int vec;                          // contiguous and aligned: four elements at a time
-    int tile, kt, nt, tri, splits, chunk;      // product tile; tiles along k and n; tiles on and above the diagonal
+    int tile, kt, nt, tri, splits, chunk;      // tile of G and X; tiles along k and n; tiles on and above the diagonal
+    int tile_p, kt_p, tri_p;                   // tile of P
     int sums;                                  // partial sums of squares per matrix
     float step;
-    half_t *xt[2], *xl, *g, *p;                // planes of matrix 0 of the stack
+    half_t *xt[2], *g, *p;                     // planes of matrix 0 of the stack
     float* part;
     double* sq;
-    int at[4];      // first workgroup in the launches over: chunks of 4096 elements, 64x64 blocks, G tiles x splits, X tiles
-    int at_p, at_f; // ... over: G / P tiles, 64x64 blocks of G tiles (fold)
+    int at[6];      // first workgroup in the launches over: NS_CHUNKs, 64 x 64 blocks of X, G tiles x splits, X tiles, P tiles,
+                    // 32 x 32 blocks of G tiles (fold)
 };
 
 // ---- pairs of fp16
@@ -68,19 +70,15 @@ __device__ __forceinline__ size_t ns_at(size_t row, int col, int cols) {
 }
 
 // which matrix a workgroup belongs to: the last whose first workgroup is not behind it (64 candidates a look)
+enum { NS_SQUARES, NS_PLANES, NS_GRAM, NS_APPLY, NS_POLY, NS_FOLD, NS_LAUNCHES };
 template <int WHICH>
-__device__ __forceinline__ int ns_first(const NsMat& m) {
-    return WHICH < 4 ? m.at[WHICH & 3] : WHICH == 4 ? m.at_p : m.at_f;
-}
-template <int WHICH>
-__device__ __forceinline__ int ns_find(const NsMat* tab, int count, int wg) {
+__device__ __forceinline__ const NsMat& ns_find(const NsMat* tab, int count) {
     int found = -1;
     for (int base = 0; base < count; base += 64) {
         const int i = base + (threadIdx.x & 63);
-        const bool in = i < count && ns_first<WHICH>(tab[i]) <= wg;
-        found += __popcll(__ballot(in));
+        found += __popcll(__ballot(i < count && tab[i].at[WHICH] <= (int)blockIdx.x));
     }
-    return __builtin_amdgcn_readfirstlane(found);
+    return tab[__builtin_amdgcn_readfirstlane(found)];
 }
 
 // The table's way to the device: by value, in kernel arguments (a captured call keeps its own), copied by all lanes at once.
@@ -123,8 +121,8 @@ __device__ __forceinline__ float ns_clip(float g, float clip) {      // (NaN sta
 
 // sums of squares in 64 bits (neither huge nor tiny entries leave the range), and the momentum's update
 __global__ __launch_bounds__(NS_THREADS) void k_ns_squares(const NsMat* tab, int count, const NsUpdate up) {
-    const NsMat& m = tab[ns_find<0>(tab, count, blockIdx.x)];
-    const int at = blockIdx.x - m.at[0], b = at / m.sums, part = at % m.sums;
+    const NsMat& m = ns_find<NS_SQUARES>(tab, count);
+    const int at = blockIdx.x - m.at[NS_SQUARES], b = at / m.sums, part = at % m.sums;
     const long long total = (long long)m.rows * m.cols, first = (long long)part * NS_CHUNK;
     const long long last = first + NS_CHUNK < total ? first + NS_CHUNK : total;
     const bool linear = m.in_ld == m.cols;
@@ -177,11 +175,11 @@ __global__ __launch_bounds__(NS_THREADS) void k_ns_squares(const NsMat* tab, int
     if (threadIdx.x == 0) m.sq[(size_t)b * m.sums + part] = red[0];
 }
 
-// X = M / (|M| + eps) as plane pairs in both orders, 64 x 64 of XT's [n][k] at a time
+// X = M / (|M| + eps) as plane pairs, 64 x 64 of [n][k] at a time
 __global__ __launch_bounds__(NS_THREADS) void k_ns_planes(const NsMat* tab, int count, const NsUpdate up, double eps) {
-    const NsMat& m = tab[ns_find<1>(tab, count, blockIdx.x)];
+    const NsMat& m = ns_find<NS_PLANES>(tab, count);
     const int kb = m.kp / 64, nb = m.np / 64;
-    int at = blockIdx.x - m.at[1];
+    int at = blockIdx.x - m.at[NS_PLANES];
     const int b = at / (kb * nb);
     at %= kb * nb;
     const int n0 = at / kb * 64, k0 = at % kb * 64;
@@ -215,7 +213,6 @@ __global__ __launch_bounds__(NS_THREADS) void k_ns_planes(const NsMat* tab, int 
     }
     __syncthreads();
     half_t* xt = m.xt[0] + (size_t)b * m.np * m.kp * 2;
-    half_t* xl = m.xl + (size_t)b * m.np * m.kp * 2;
     for (int q = threadIdx.x; q < 512; q += NS_THREADS) {
         const int row = q >> 3, col = (q & 7) * 8;
         float v[8];
@@ -223,38 +220,45 @@ __global__ __launch_bounds__(NS_THREADS) void k_ns_planes(const NsMat* tab, int 
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = tile[row][col + e];
         ns_split8(v, hi, lo);
-        size_t o = ns_at(n0 + row, k0 + col, m.kp);
+        const size_t o = ns_at(n0 + row, k0 + col, m.kp);
         *(half8*)(xt + o) = hi;
         *(half8*)(xt + o + 32) = lo;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = tile[col + e][row];
-        ns_split8(v, hi, lo);
-        o = ns_at(k0 + row, n0 + col, m.np);
-        *(half8*)(xl + o) = hi;
-        *(half8*)(xl + o + 32) = lo;
     }
 }
 
-// ---- T x T tile of A B^T, both plane pairs, columns [c0, c1) (multiples of 64); four waves, a quarter of the tile each.
-// A step takes 32 columns (T = 128) or 64 (T = 64: as many bytes) straight from global memory to LDS, 16 bytes a lane, one step
-// ahead of the products; the fragments of a step are read before the next step's transfers are issued, so that the wait for
-// those stands at the next step's start.  Rows behind a matrix's last are read as its last row and never stored.  LDS: a row's
-// 128 bytes of 32 columns are eight pieces of 16, piece q of row r at place q ^ (r / 2 % 8): the 16 lanes that read one piece
-// of 16 rows together meet each bank once.
+// ---- a T x T tile of a product of plane pairs, by eight waves: two groups of four, a quarter of the tile each; a step takes 64
+// of the summed index, 32 a group, so that every SIMD has two waves whatever the number of tiles (one wave alone left the matrix
+// pipe idle two thirds of a step).  Operands go straight from global memory to LDS, 16 bytes a lane, one step ahead; a step's
+// fragments are read before the next transfers are issued, so that the wait for those stands at the next step's start.
+//   rows (TR = false): sum over columns [c0, c1) of A[a0 + i][.] B[b0 + j][.]; a block of 32 columns is T rows of 128 bytes, eight
+//     pieces of 16, piece q of row r at place q ^ (r / 2 % 8): the 16 lanes that read one piece of 16 rows meet each bank once.
+//     Rows behind the last are read as the last and never stored.
+//   columns (TR = true): sum over rows [c0, c1) of A[.][a0 + i] B[.][b0 + j]; 32 rows of T columns, piece q of row r at place
+//     q ^ 4 (r % 4); ds_read_b64_tr_b16 hands a lane four rows of its column: the four rows that 16 lanes read lie in different
+//     quarters of the banks.  Column blocks behind the last are read as the last and never stored.
 typedef __attribute__((address_space(3))) void* lds_ptr;
 typedef const __attribute__((address_space(1))) void* glb_ptr;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
 
-template <int T>
+__device__ __forceinline__ half8 ns_read_tr(const char* p, int second) {
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + second));
+    return __builtin_bit_cast(half8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+template <int T, bool TR>
 struct NsTile {
     static constexpr int S = T / 64;           // 32 x 32 blocks of a wave along each side
-    static constexpr int KS = 128 / T;         // blocks of 32 columns of a step
-    static constexpr int LOADS = T / 32;       // 16-byte transfers of a lane, per operand and block
-    static constexpr int HALF = T * 128 * KS;  // bytes of an operand's step
+    static constexpr int LOADS = T / 32;       // 16-byte transfers of a lane, per operand and step
+    static constexpr int PART = T * 128;       // bytes of an operand's step of one group
+    static constexpr int P = T + 2;            // floats between rows of the staged tile: mirrored reads meet each bank once
     f32x16 acc[S][S];
 
-    __device__ __forceinline__ void run(const half_t* A, int a0, int a_rows, int a_cols, const half_t* B, int b0, int b_rows,
-                                        int b_cols, int c0, int c1, char* lds) {
-        const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    __device__ __forceinline__ void run(const half_t* A, int a0, int a_rows, const half_t* B, int b0, int b_rows, int cols,
+                                        int c0, int c1, char* lds) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) & 3);
+        const int group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
         const int wr = (wave >> 1) * (T / 2), wc = (wave & 1) * (T / 2);
 #pragma unroll
         for (int i = 0; i < S; ++i)
@@ -262,55 +266,76 @@ struct NsTile {
             for (int j = 0; j < S; ++j)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-        const char* base_a = (const char*)(A + (size_t)c0 * 2);
-        const char* base_b = (const char*)(B + (size_t)c0 * 2);
-        size_t off_a[LOADS], off_b[LOADS];
+        // a step further: 64 columns or 64 rows
+        const size_t stride = TR ? (size_t)64 * cols * 4 : 256;
+        const size_t start = TR ? (size_t)(c0 + group * 32) * cols * 4 : (size_t)c0 * 4 + group * 128;
+        const char *pa[LOADS], *pb[LOADS];
 #pragma unroll
         for (int l = 0; l < LOADS; ++l) {
-            const int row = (wave * LOADS + l) * 8 + (lane >> 3), piece = (lane & 7) ^ ((row >> 1) & 7);
-            off_a[l] = (size_t)min(a0 + row, a_rows - 1) * a_cols * 4 + piece * 16;
-            off_b[l] = (size_t)min(b0 + row, b_rows - 1) * b_cols * 4 + piece * 16;
+            if constexpr (TR) {
+                const int row = (wave * LOADS + l) * (256 / T) + lane / (T / 4), piece = lane % (T / 4) ^ (4 * (row & 3));
+                const size_t at = start + (size_t)row * cols * 4 + (piece & 7) * 16;
+                pa[l] = (const char*)A + at + (size_t)min(a0 / 32 + (piece >> 3), cols / 32 - 1) * 128;
+                pb[l] = (const char*)B + at + (size_t)min(b0 / 32 + (piece >> 3), cols / 32 - 1) * 128;
+            } else {
+                const int row = (wave * LOADS + l) * 8 + (lane >> 3), piece = (lane & 7) ^ ((row >> 1) & 7);
+                pa[l] = (const char*)A + start + (size_t)min(a0 + row, a_rows - 1) * cols * 4 + piece * 16;
+                pb[l] = (const char*)B + start + (size_t)min(b0 + row, b_rows - 1) * cols * 4 + piece * 16;
+            }
         }
-        auto fetch = [&](char* to, int step) {
+        auto fetch = [&](int buffer, size_t ahead) {
+            char* to = lds + buffer * (4 * PART) + group * (2 * PART) + wave * LOADS * 1024;
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
-#pragma unroll
-                for (int l = 0; l < LOADS; ++l) {
-                    char* dst = to + s * (T * 128) + (wave * LOADS + l) * 1024;
-                    const size_t c = (size_t)(step * KS + s) * 128;
-                    __builtin_amdgcn_global_load_lds((glb_ptr)(base_a + c + off_a[l]), (lds_ptr)dst, 16, 0, 0);
-                    __builtin_amdgcn_global_load_lds((glb_ptr)(base_b + c + off_b[l]), (lds_ptr)(dst + HALF), 16, 0, 0);
-                }
+            for (int l = 0; l < LOADS; ++l) {
+                __builtin_amdgcn_global_load_lds((glb_ptr)(pa[l] + ahead), (lds_ptr)(to + l * 1024), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((glb_ptr)(pb[l] + ahead), (lds_ptr)(to + PART + l * 1024), 16, 0, 0);
+            }
         };
-        int at_a[S][2], at_b[S][2];
+        int at_a[S][2], at_b[S][2];      // hi; lo: bit 6 flipped
 #pragma unroll
         for (int i = 0; i < S; ++i)
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
-                const int q = kk * 2 + (lane >> 5), r = wr + i * 32 + (lane & 31), c = wc + i * 32 + (lane & 31);
-                at_a[i][kk] = r * 128 + ((q ^ ((r >> 1) & 7)) << 4);          // (lo: the place with bit 2 of the piece flipped)
-                at_b[i][kk] = HALF + c * 128 + ((q ^ ((c >> 1) & 7)) << 4);
+                if constexpr (TR) {
+                    const int g = lane >> 4, q = (lane & 15) >> 2, p = lane & 3, chunk = 2 * (g & 1) + (p >> 1);
+                    const int row = (kk * 16 + 8 * (g >> 1) + q) * (T * 4) + (p & 1) * 8;
+                    at_a[i][kk] = row + ((((wr / 32 + i) * 8 + chunk) ^ (4 * q)) << 4);
+                    at_b[i][kk] = PART + row + ((((wc / 32 + i) * 8 + chunk) ^ (4 * q)) << 4);
+                } else {
+                    const int q = kk * 2 + (lane >> 5), r = wr + i * 32 + (lane & 31), c = wc + i * 32 + (lane & 31);
+                    at_a[i][kk] = r * 128 + ((q ^ ((r >> 1) & 7)) << 4);
+                    at_b[i][kk] = PART + c * 128 + ((q ^ ((c >> 1) & 7)) << 4);
+                }
             }
-        const int steps = (c1 - c0) / (32 * KS);
-        fetch(lds, 0);
+        const int steps = (c1 - c0) / 64;
+        fetch(0, 0);
+        size_t ahead = 0;
         for (int step = 0; step < steps; ++step) {
-            const char* now = lds + (step & 1) * (2 * HALF);
+            const char* now = lds + (step & 1) * (4 * PART) + group * (2 * PART);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            half8 ah[KS * 2][S], al[KS * 2][S], bh[KS * 2][S], bl[KS * 2][S];
+            half8 ah[2][S], al[2][S], bh[2][S], bl[2][S];
 #pragma unroll
-            for (int k = 0; k < KS * 2; ++k)
+            for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int i = 0; i < S; ++i) {
-                    const char* blk = now + (k >> 1) * (T * 128);
-                    ah[k][i] = *(const half8*)(blk + at_a[i][k & 1]);
-                    al[k][i] = *(const half8*)(blk + (at_a[i][k & 1] ^ 64));
-                    bh[k][i] = *(const half8*)(blk + at_b[i][k & 1]);
-                    bl[k][i] = *(const half8*)(blk + (at_b[i][k & 1] ^ 64));
+                    if constexpr (TR) {
+                        ah[k][i] = ns_read_tr(now + at_a[i][k], T * 16);
+                        bh[k][i] = ns_read_tr(now + at_b[i][k], T * 16);
+                        al[k][i] = ns_read_tr(now + (at_a[i][k] ^ 64), T * 16);
+                        bl[k][i] = ns_read_tr(now + (at_b[i][k] ^ 64), T * 16);
+                    } else {
+                        ah[k][i] = *(const half8*)(now + at_a[i][k]);
+                        bh[k][i] = *(const half8*)(now + at_b[i][k]);
+                        al[k][i] = *(const half8*)(now + (at_a[i][k] ^ 64));
+                        bl[k][i] = *(const half8*)(now + (at_b[i][k] ^ 64));
+                    }
                 }
-            if (step + 1 < steps) fetch(lds + ((step + 1) & 1) * (2 * HALF), step + 1);
+            // (unconditional: behind the last step the same step again, into the buffer nobody reads any more)
+            ahead += step + 1 < steps ? stride : 0;
+            fetch((step + 1) & 1, ahead);
 #pragma unroll
-            for (int k = 0; k < KS * 2; ++k) {
+            for (int k = 0; k < 2; ++k) {
 #pragma unroll
                 for (int i = 0; i < S; ++i)
 #pragma unroll
@@ -328,26 +353,33 @@ struct NsTile {
                         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[k][i], bh[k][j], acc[i][j], 0, 0, 0);
             }
         }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
     }
-    // the tile's sums into LDS, tile[row][col] with rows T + 1 apart
+    // the sums of both groups, second first, into LDS: tile[row][col], rows P apart
     __device__ __forceinline__ void stage(float* tile) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        const int wr = (wave >> 1) * (T / 2), wc = (wave & 1) * (T / 2);
+        const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) & 3, group = threadIdx.x >> 8;
+        float* at = tile + ((wave >> 1) * (T / 2) + 4 * (lane >> 5)) * P + (wave & 1) * (T / 2) + (lane & 31);
 #pragma unroll
-        for (int i = 0; i < S; ++i)
+        for (int turn = 1; turn >= 0; --turn) {
+            if (group == turn) {
 #pragma unroll
-            for (int j = 0; j < S; ++j)
+                for (int i = 0; i < S; ++i)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int row = wr + i * 32 + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5);
-                    tile[row * (T + 1) + wc + j * 32 + (lane & 31)] = acc[i][j][e] * (NS_UNSCALE * NS_UNSCALE);
-                }
-        __syncthreads();
+                    for (int j = 0; j < S; ++j)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            float* p = at + (i * 32 + (e & 3) + 8 * (e >> 2)) * P + j * 32;
+                            const float v = acc[i][j][e] * (NS_UNSCALE * NS_UNSCALE);
+                            *p = turn ? v : *p + v;
+                        }
+            }
+            __syncthreads();
+        }
     }
 };
 
-#define NS_LDS (128 * 129 * 4)      // the larger of two steps' operands (64 KB) and the staged tile
+#define NS_LDS(T) (T * 128 * 8)      // two steps' operands of both groups; the staged tile is smaller
 
 // tile number -> (i, j), i <= j, of a triangle of `t` rows
 __device__ __forceinline__ void ns_pair(int l, int t, int& i, int& j) {
@@ -357,23 +389,26 @@ __device__ __forceinline__ void ns_pair(int l, int t, int& i, int& j) {
 }
 
 // rows [r0, r0 + T) and columns [c0, c0 + T) of a symmetric plane pair [kp][kp] from the staged tile, and its mirror image
-template <int T>
+template <int T, int P, int THREADS>
 __device__ __forceinline__ void ns_symmetric(half_t* out, int kp, int r0, int c0, const float* tile) {
-    for (int q = threadIdx.x; q < T * T / 8; q += NS_THREADS) {
-        const int row = q / (T / 8), col = q % (T / 8) * 8;
+    for (int q = threadIdx.x; q < T * T / 8; q += THREADS) {
         float v[8];
         half8 hi, lo;
+        int row = q / (T / 8), col = q % (T / 8) * 8;
         if (r0 + row < kp && c0 + col < kp) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = tile[row * (T + 1) + col + e];
+            for (int e = 0; e < 8; ++e) v[e] = tile[row * P + col + e];
             ns_split8(v, hi, lo);
             const size_t o = ns_at(r0 + row, c0 + col, kp);
             *(half8*)(out + o) = hi;
             *(half8*)(out + o + 32) = lo;
         }
+        // (sixteen lanes along the tile's columns, four down its rows: 64 contiguous bytes of a mirrored row)
+        row = (q >> 2 & 15) + (q / 64 % (T / 16)) * 16;
+        col = ((q & 3) + q / (4 * T) * 4) * 8;
         if (r0 != c0 && c0 + row < kp && r0 + col < kp) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = tile[(col + e) * (T + 1) + row];
+            for (int e = 0; e < 8; ++e) v[e] = tile[(col + e) * P + row];
             ns_split8(v, hi, lo);
             const size_t o = ns_at(c0 + row, r0 + col, kp);
             *(half8*)(out + o) = hi;
@@ -382,91 +417,92 @@ __device__ __forceinline__ void ns_symmetric(half_t* out, int kp, int r0, int c0
     }
 }
 
-// G = XL XL^T, a chunk of n at a time
+// G = X^T X, a chunk of n at a time
 template <int T>
-__device__ __forceinline__ void ns_gram(const NsMat& m, int at, char* lds) {
+__device__ __forceinline__ void ns_gram(const NsMat& m, int from, char* lds) {
+    int at = blockIdx.x - m.at[NS_GRAM];
     const int b = at / (m.tri * m.splits);
     at %= m.tri * m.splits;
     const int split = at / m.tri, l = at % m.tri;
     int i, j;
     ns_pair(l, m.kt, i, j);
-    const half_t* xl = m.xl + (size_t)b * m.np * m.kp * 2;
+    const half_t* x = m.xt[from] + (size_t)b * m.np * m.kp * 2;
     const int c0 = split * m.chunk, c1 = min(m.np, c0 + m.chunk);
-    NsTile<T> t;
-    t.run(xl, i * T, m.kp, m.np, xl, j * T, m.kp, m.np, c0, c1, lds);
+    NsTile<T, true> t;
+    t.run(x, i * T, m.np, x, j * T, m.np, m.kp, c0, c1, lds);
     float* tile = (float*)lds;
     t.stage(tile);
     if (m.splits == 1) {
-        ns_symmetric<T>(m.g + (size_t)b * m.kp * m.kp * 2, m.kp, i * T, j * T, tile);
+        ns_symmetric<T, T + 2, NS_WIDE>(m.g + (size_t)b * m.kp * m.kp * 2, m.kp, i * T, j * T, tile);
     } else {
         float* out = m.part + (((size_t)b * m.splits + split) * m.tri + l) * (T * T);
-        for (int q = threadIdx.x; q < T * T; q += NS_THREADS) out[q] = tile[q / T * (T + 1) + q % T];
+        for (int q = threadIdx.x; q < T * T; q += NS_WIDE) out[q] = tile[q / T * (T + 2) + q % T];
     }
 }
-__global__ __launch_bounds__(NS_THREADS) void k_ns_gram(const NsMat* tab, int count) {
+__global__ __launch_bounds__(NS_WIDE) void k_ns_gram(const NsMat* tab, int count, int from) {
     extern __shared__ __align__(16) char lds[];
-    const NsMat& m = tab[ns_find<2>(tab, count, blockIdx.x)];
-    if (m.tile == 128) ns_gram<128>(m, blockIdx.x - m.at[2], lds);
-    else ns_gram<64>(m, blockIdx.x - m.at[2], lds);
+    const NsMat& m = ns_find<NS_GRAM>(tab, count);
+    if (m.tile == 128) ns_gram<128>(m, from, lds);
+    else ns_gram<64>(m, from, lds);
 }
 
-// the chunks' sums in order, a 64 x 64 block of a tile
+// the chunks' sums in order, a 32 x 32 block of a tile
 __global__ __launch_bounds__(NS_THREADS) void k_ns_fold(const NsMat* tab, int count) {
-    const NsMat& m = tab[ns_find<5>(tab, count, blockIdx.x)];
-    __shared__ float tile[64 * 65];
-    const int T = m.tile, sub = T / 64;
-    int at = blockIdx.x - m.at_f;
+    const NsMat& m = ns_find<NS_FOLD>(tab, count);
+    __shared__ float tile[32 * 34];
+    const int T = m.tile, sub = T / 32;
+    int at = blockIdx.x - m.at[NS_FOLD];
     const int b = at / (m.tri * sub * sub);
     at %= m.tri * sub * sub;
-    const int l = at / (sub * sub), r = at % (sub * sub) / sub * 64, c = at % sub * 64;
+    const int l = at / (sub * sub), r = at % (sub * sub) / sub * 32, c = at % sub * 32;
     int i, j;
     ns_pair(l, m.kt, i, j);
     if (i == j && c < r) return;      // (its mirror image writes it)
-    const float* in = m.part + ((size_t)b * m.splits * m.tri + l) * (T * T);
-    for (int q = threadIdx.x; q < 1024; q += NS_THREADS) {
-        const int row = q >> 4, col = (q & 15) * 4;
-        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int p = 0; p < m.splits; ++p) {
-            const float4 v = *(const float4*)(in + (size_t)p * m.tri * (T * T) + (r + row) * T + c + col);
-            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
-        }
-        float* o = tile + row * 65 + col;
-        o[0] = s.x; o[1] = s.y; o[2] = s.z; o[3] = s.w;
+    const int row = threadIdx.x >> 3, col = (threadIdx.x & 7) * 4;
+    const float* in = m.part + ((size_t)b * m.splits * m.tri + l) * (T * T) + (r + row) * T + c + col;
+    const size_t next = (size_t)m.tri * T * T;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int p = 0; p < m.splits; ++p) {
+        const float4 v = *(const float4*)(in + p * next);
+        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
     }
+    float* o = tile + row * 34 + col;
+    o[0] = s.x; o[1] = s.y; o[2] = s.z; o[3] = s.w;
     __syncthreads();
-    ns_symmetric<64>(m.g + (size_t)b * m.kp * m.kp * 2, m.kp, i * T + r, j * T + c, tile);
+    ns_symmetric<32, 34, NS_THREADS>(m.g + (size_t)b * m.kp * m.kp * 2, m.kp, i * T + r, j * T + c, tile);
 }
 
 // P = b G + c G G
 template <int T>
-__device__ __forceinline__ void ns_poly(const NsMat& m, int at, float cb, float cc, char* lds) {
-    const int b = at / m.tri;
+__device__ __forceinline__ void ns_poly(const NsMat& m, float cb, float cc, char* lds) {
+    const int at = blockIdx.x - m.at[NS_POLY], b = at / m.tri_p;
     int i, j;
-    ns_pair(at % m.tri, m.kt, i, j);
+    ns_pair(at % m.tri_p, m.kt_p, i, j);
     const half_t* g = m.g + (size_t)b * m.kp * m.kp * 2;
-    NsTile<T> t;
-    t.run(g, i * T, m.kp, m.kp, g, j * T, m.kp, m.kp, 0, m.kp, lds);
+    NsTile<T, false> t;
+    t.run(g, i * T, m.kp, g, j * T, m.kp, m.kp, 0, m.kp, lds);
     float* tile = (float*)lds;
     t.stage(tile);
-    for (int q = threadIdx.x; q < T * T / 8; q += NS_THREADS) {
+    for (int q = threadIdx.x; q < T * T / 8; q += NS_WIDE) {
         const int row = q / (T / 8), col = q % (T / 8) * 8;
         if (i * T + row >= m.kp || j * T + col >= m.kp) continue;
         const size_t o = ns_at(i * T + row, j * T + col, m.kp);
         const half8 hi = *(const half8*)(g + o), lo = *(const half8*)(g + o + 32);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            float* v = tile + row * (T + 1) + col + e;
+            float* v = tile + row * (T + 2) + col + e;
             *v = cc * *v + cb * (((float)hi[e] + (float)lo[e]) * NS_UNSCALE);
         }
     }
     __syncthreads();
-    ns_symmetric<T>(m.p + (size_t)b * m.kp * m.kp * 2, m.kp, i * T, j * T, tile);
+    ns_symmetric<T, T + 2, NS_WIDE>(m.p + (size_t)b * m.kp * m.kp * 2, m.kp, i * T, j * T, tile);
 }
-__global__ __launch_bounds__(NS_THREADS) void k_ns_poly(const NsMat* tab, int count, float cb, float cc) {
+__global__ __launch_bounds__(NS_WIDE) void k_ns_poly(const NsMat* tab, int count, float cb, float cc) {
     extern __shared__ __align__(16) char lds[];
-    const NsMat& m = tab[ns_find<4>(tab, count, blockIdx.x)];
-    if (m.tile == 128) ns_poly<128>(m, blockIdx.x - m.at_p, cb, cc, lds);
-    else ns_poly<64>(m, blockIdx.x - m.at_p, cb, cc, lds);
+    const NsMat& m = ns_find<NS_POLY>(tab, count);
+    if (m.tile_p == 128) ns_poly<128>(m, cb, cc, lds);
+    else ns_poly<64>(m, cb, cc, lds);
 }
 
 __device__ __forceinline__ void ns_out(const NsMat& m, const NsUpdate& up, int b, int r, int c, float v) {
@@ -485,65 +521,60 @@ __device__ __forceinline__ void ns_out(const NsMat& m, const NsUpdate& up, int b
 
 // X <- a X + X P
 template <int T>
-__device__ __forceinline__ void ns_apply(const NsMat& m, int at, int from, float ca, bool last, const NsUpdate& up, char* lds) {
+__device__ __forceinline__ void ns_apply(const NsMat& m, int from, float ca, bool last, const NsUpdate& up, char* lds) {
+    constexpr int EACH = T * T / 8 / NS_WIDE, P = T + 2;
+    int at = blockIdx.x - m.at[NS_APPLY];
     const int b = at / (m.nt * m.kt);
     at %= m.nt * m.kt;
     const int n0 = at / m.kt * T, k0 = at % m.kt * T;
     const size_t plane = (size_t)b * m.np * m.kp * 2;
     const half_t* x = m.xt[from] + plane;
-    NsTile<T> t;
-    t.run(x, n0, m.np, m.kp, m.p + (size_t)b * m.kp * m.kp * 2, k0, m.kp, m.kp, 0, m.kp, lds);
+    half_t* out = m.xt[from ^ 1] + plane;
+    NsTile<T, false> t;
+    t.run(x, n0, m.np, m.p + (size_t)b * m.kp * m.kp * 2, k0, m.kp, m.kp, 0, m.kp, lds);
     float* tile = (float*)lds;
+    half8 xh[EACH], xl[EACH];
+#pragma unroll
+    for (int l = 0; l < EACH; ++l) {
+        const int q = l * NS_WIDE + threadIdx.x, row = q / (T / 8), col = q % (T / 8) * 8;
+        const size_t o = ns_at(min(n0 + row, m.np - 1), min(k0 + col, m.kp - 8), m.kp);
+        xh[l] = *(const half8*)(x + o);
+        xl[l] = *(const half8*)(x + o + 32);
+    }
     t.stage(tile);
-    for (int q = threadIdx.x; q < T * T / 8; q += NS_THREADS) {
-        const int row = q / (T / 8), col = q % (T / 8) * 8;
+#pragma unroll
+    for (int l = 0; l < EACH; ++l) {
+        const int q = l * NS_WIDE + threadIdx.x, row = q / (T / 8), col = q % (T / 8) * 8;
         if (n0 + row >= m.np || k0 + col >= m.kp) continue;
-        const size_t o = ns_at(n0 + row, k0 + col, m.kp);
-        const half8 xh = *(const half8*)(x + o), xlo = *(const half8*)(x + o + 32);
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            float* p = tile + row * (T + 1) + col + e;
-            v[e] = *p + ca * (((float)xh[e] + (float)xlo[e]) * NS_UNSCALE);
-            *p = v[e];
+            float* p = tile + row * P + col + e;
+            v[e] = *p + ca * (((float)xh[l][e] + (float)xl[l][e]) * NS_UNSCALE);
+            if (last) *p = v[e];
         }
         if (!last) {
             half8 hi, lo;
             ns_split8(v, hi, lo);
-            half_t* out = m.xt[from ^ 1] + plane + o;
-            *(half8*)out = hi;
-            *(half8*)(out + 32) = lo;
+            const size_t o = ns_at(n0 + row, k0 + col, m.kp);
+            *(half8*)(out + o) = hi;
+            *(half8*)(out + o + 32) = lo;
         }
     }
+    if (!last) return;
     __syncthreads();
-    if (!last) {
-        half_t* xl = m.xl + plane;
-        for (int q = threadIdx.x; q < T * T / 8; q += NS_THREADS) {
-            const int row = q / (T / 8), col = q % (T / 8) * 8;
-            if (k0 + row >= m.kp || n0 + col >= m.np) continue;
-            float v[8];
-            half8 hi, lo;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = tile[(col + e) * (T + 1) + row];
-            ns_split8(v, hi, lo);
-            const size_t o = ns_at(k0 + row, n0 + col, m.np);
-            *(half8*)(xl + o) = hi;
-            *(half8*)(xl + o + 32) = lo;
-        }
-    } else {
-        for (int q = threadIdx.x; q < T * T; q += NS_THREADS) {      // (lanes along the output's rows)
-            const int i = q / T, j = q % T;
-            const int r = (m.tall ? n0 : k0) + i, c = (m.tall ? k0 : n0) + j;
-            if (r < m.rows && c < m.cols) ns_out(m, up, b, r, c, m.tall ? tile[i * (T + 1) + j] : tile[j * (T + 1) + i]);
-        }
+    for (int q = threadIdx.x; q < T * T; q += NS_WIDE) {      // (lanes along the output's rows)
+        const int i = q / T, j = q % T;
+        const int r = (m.tall ? n0 : k0) + i, c = (m.tall ? k0 : n0) + j;
+        if (r < m.rows && c < m.cols) ns_out(m, up, b, r, c, m.tall ? tile[i * P + j] : tile[j * P + i]);
     }
 }
-__global__ __launch_bounds__(NS_THREADS) void k_ns_apply(const NsMat* tab, int count, int from, float ca, int last,
-                                                         const NsUpdate up) {
+__global__ __launch_bounds__(NS_WIDE) void k_ns_apply(const NsMat* tab, int count, int from, float ca, int last,
+                                                      const NsUpdate up) {
     extern __shared__ __align__(16) char lds[];
-    const NsMat& m = tab[ns_find<3>(tab, count, blockIdx.x)];
-    if (m.tile == 128) ns_apply<128>(m, blockIdx.x - m.at[3], from, ca, last, up, lds);
-    else ns_apply<64>(m, blockIdx.x - m.at[3], from, ca, last, up, lds);
+    const NsMat& m = ns_find<NS_APPLY>(tab, count);
+    if (m.tile == 128) ns_apply<128>(m, from, ca, last, up, lds);
+    else ns_apply<64>(m, from, ca, last, up, lds);
 }
 
 // ---- host side
@@ -553,7 +584,8 @@ enum { NS_IN, NS_OUT, NS_MOM, NS_ROWS, NS_COLS, NS_BATCH, NS_IN_LD, NS_IN_BS, NS
 
 struct NsPlan {
     size_t bytes;
-    int grid[6];      // chunks, blocks, gram, apply, poly, fold
+    int grid[NS_LAUNCHES];
+    bool wide, wide_p;      // a tile of 128 among those of G and X; of P
 };
 
 // One matrix stack's part of the workspace and of the launches.  false: a size that is not taken.
@@ -575,11 +607,20 @@ static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
     m.nt = agb_cdiv(m.np, m.tile);
     m.tri = m.kt * (m.kt + 1) / 2;
     const long long tiles = (long long)m.tri * m.batch;
+    // G: enough chunks of n for a workgroup per CU, none shorter than eight steps.  (By the matrix alone: what else is in the
+    // list does not change a result.)
     int splits = tiles >= 256 ? 1 : agb_cdiv(256, tiles);
-    if (splits > m.np / 256) splits = m.np / 256;
+    if (splits > m.np / 512) splits = m.np / 512;
     if (splits < 1) splits = 1;
     m.chunk = agb_cdiv(agb_cdiv(m.np, splits), 64) * 64;
     m.splits = agb_cdiv(m.np, m.chunk);
+    // P: k products a sum and few tiles: 64 x 64 as long as those fit the device twice
+    const int k64 = m.kp / 64;
+    m.tile_p = (long long)k64 * (k64 + 1) / 2 * m.batch <= 512 ? 64 : 128;
+    m.kt_p = agb_cdiv(m.kp, m.tile_p);
+    m.tri_p = m.kt_p * (m.kt_p + 1) / 2;
+    plan.wide |= m.tile == 128;
+    plan.wide_p |= m.tile_p == 128;
     m.sums = agb_cdiv((long long)rows * cols, NS_CHUNK);
     const size_t x = (size_t)m.np * m.kp * 4 * batch, g = (size_t)m.kp * m.kp * 4 * batch;
     auto take = [&](size_t n) {
@@ -589,17 +630,16 @@ static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
     };
     m.xt[0] = (half_t*)take(x);
     m.xt[1] = (half_t*)take(x);
-    m.xl = (half_t*)take(x);
     m.g = (half_t*)take(g);
     m.p = (half_t*)take(g);
     m.part = (float*)take(m.splits > 1 ? (size_t)m.splits * tiles * m.tile * m.tile * 4 : 0);
     m.sq = (double*)take((size_t)m.sums * batch * 8);
-    const long long wgs[6] = {(long long)m.sums * batch, (long long)(m.kp / 64) * (m.np / 64) * batch, tiles * m.splits,
-                              (long long)m.kt * m.nt * batch, tiles,
-                              m.splits > 1 ? tiles * (m.tile / 64) * (m.tile / 64) : 0};
-    int* at[6] = {&m.at[0], &m.at[1], &m.at[2], &m.at[3], &m.at_p, &m.at_f};
-    for (int i = 0; i < 6; ++i) {
-        *at[i] = plan.grid[i];
+    const long long sub = (m.tile / 32) * (m.tile / 32);
+    const long long wgs[NS_LAUNCHES] = {(long long)m.sums * batch, (long long)(m.kp / 64) * (m.np / 64) * batch, tiles * m.splits,
+                                        (long long)m.kt * m.nt * batch, (long long)m.tri_p * batch,
+                                        m.splits > 1 ? tiles * sub : 0};
+    for (int i = 0; i < NS_LAUNCHES; ++i) {
+        m.at[i] = plan.grid[i];
         if (plan.grid[i] + wgs[i] > 0x7fffffff) return false;
         plan.grid[i] += (int)wgs[i];
     }
@@ -664,18 +704,19 @@ static int ns_run(const char* name, const long long* fields, int count, int step
         AGB_CHECK_LAUNCH(name);
     }
     for (const void* k : {(const void*)k_ns_gram, (const void*)k_ns_poly, (const void*)k_ns_apply}) {
-        const hipError_t e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, NS_LDS);
+        const hipError_t e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, NS_LDS(128));
         if (e != hipSuccess) { agb_set_error("%s: %s", name, hipGetErrorString(e)); return AGB_ELAUNCH; }
     }
-    hipLaunchKernelGGL(k_ns_squares, dim3(plan.grid[0]), dim3(NS_THREADS), 0, st, tab, count, up);
-    hipLaunchKernelGGL(k_ns_planes, dim3(plan.grid[1]), dim3(NS_THREADS), 0, st, tab, count, up, eps);
+    const int lds = plan.wide ? NS_LDS(128) : NS_LDS(64), lds_p = plan.wide_p ? NS_LDS(128) : NS_LDS(64);
+    const int* grid = plan.grid;
+    hipLaunchKernelGGL(k_ns_squares, dim3(grid[NS_SQUARES]), dim3(NS_THREADS), 0, st, tab, count, up);
+    hipLaunchKernelGGL(k_ns_planes, dim3(grid[NS_PLANES]), dim3(NS_THREADS), 0, st, tab, count, up, eps);
     for (int i = 0; i < steps; ++i) {
-        hipLaunchKernelGGL(k_ns_gram, dim3(plan.grid[2]), dim3(NS_THREADS), NS_LDS, st, tab, count);
-        if (plan.grid[5]) hipLaunchKernelGGL(k_ns_fold, dim3(plan.grid[5]), dim3(NS_THREADS), 0, st, tab, count);
-        hipLaunchKernelGGL(k_ns_poly, dim3(plan.grid[4]), dim3(NS_THREADS), NS_LDS, st, tab, count, coef[3 * i + 1],
-                           coef[3 * i + 2]);
-        hipLaunchKernelGGL(k_ns_apply, dim3(plan.grid[3]), dim3(NS_THREADS), NS_LDS, st, tab, count, i & 1, coef[3 * i],
-                           i == steps - 1, up);
+        const float* c = coef + 3 * i;
+        hipLaunchKernelGGL(k_ns_gram, dim3(grid[NS_GRAM]), dim3(NS_WIDE), lds, st, tab, count, i & 1);
+        if (grid[NS_FOLD]) hipLaunchKernelGGL(k_ns_fold, dim3(grid[NS_FOLD]), dim3(NS_THREADS), 0, st, tab, count);
+        hipLaunchKernelGGL(k_ns_poly, dim3(grid[NS_POLY]), dim3(NS_WIDE), lds_p, st, tab, count, c[1], c[2]);
+        hipLaunchKernelGGL(k_ns_apply, dim3(grid[NS_APPLY]), dim3(NS_WIDE), lds, st, tab, count, i & 1, c[0], i == steps - 1, up);
     }
     AGB_CHECK_LAUNCH(name);
     return AGB_OK;
