@@ -13,8 +13,10 @@
 // directions two more bits.
 //
 // Layout: X is held as [n][k] (the longer side down), so X P reads both operands along their rows (P is symmetric), and G = X^T X
-// reads X down its columns: those fragments are transposed by the LDS reads.  A row is cut into blocks of 32: 32 hi, then 32 lo —
-// 128 contiguous bytes.  Rows and blocks are padded to multiples of 64 with zeros, which the iteration keeps zero.  G and P are
+// reads X down its columns: those fragments are transposed by the LDS reads.  Columns are cut into blocks of 32; a block holds
+// row after row of 128 bytes, 32 hi then 32 lo, so that what a step takes of an operand is contiguous (in rows of all columns, the
+// rows of a tile lay a power of two apart: in the same few L2 channels, and the products ran at their speed).  Rows and columns
+// are padded to multiples of 64 with zeros, which the iteration keeps zero.  G and P are
 // symmetric: only tiles on and above the diagonal are computed.  G has few tiles and a long sum: it is split over n into chunks,
 // folded in order.
 #include "agb_common.h"
@@ -64,9 +66,9 @@ __device__ __forceinline__ void ns_split8(const float* v, half8& hi, half8& lo) 
         lo[e] = l;
     }
 }
-// element offset of (row, first column of a group of 8) of a plane pair with `cols` padded columns; lo: 32 further
-__device__ __forceinline__ size_t ns_at(size_t row, int col, int cols) {
-    return row * 2 * (size_t)cols + (size_t)(col >> 5) * 64 + (col & 31);
+// element offset of (row, first column of a group of 8) of a plane pair with `rows` padded rows; lo: 32 further
+__device__ __forceinline__ size_t ns_at(int row, int col, int rows) {
+    return ((size_t)(col >> 5) * rows + row) * 64 + (col & 31);
 }
 
 // which matrix a workgroup belongs to: the last whose first workgroup is not behind it (64 candidates a look)
@@ -214,30 +216,29 @@ __global__ __launch_bounds__(NS_THREADS) void k_ns_planes(const NsMat* tab, int 
     __syncthreads();
     half_t* xt = m.xt[0] + (size_t)b * m.np * m.kp * 2;
     for (int q = threadIdx.x; q < 512; q += NS_THREADS) {
-        const int row = q >> 3, col = (q & 7) * 8;
+        const int row = q >> 2 & 63, col = (q & 3) * 8 + (q >> 8) * 32;
         float v[8];
         half8 hi, lo;
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = tile[row][col + e];
         ns_split8(v, hi, lo);
-        const size_t o = ns_at(n0 + row, k0 + col, m.kp);
+        const size_t o = ns_at(n0 + row, k0 + col, m.np);
         *(half8*)(xt + o) = hi;
         *(half8*)(xt + o + 32) = lo;
     }
 }
 
-// ---- a T x T tile of a product of plane pairs, by eight waves: two groups of four, a quarter of the tile each; a step takes 64
-// of the summed index, 32 a group, so that every SIMD has two waves whatever the number of tiles (one wave alone left the matrix
-// pipe idle two thirds of a step).  Operands go straight from global memory to LDS, 16 bytes a lane, one step ahead; a step's
-// fragments are read before the next transfers are issued, so that the wait for those stands at the next step's start.
+// ---- a T x T tile of a product of plane pairs, by eight waves: two groups of four, a quarter of the tile each; a step takes 32
+// of the summed index, 16 a group, so that every SIMD has two waves whatever the number of tiles.  Operands go straight from
+// global memory to LDS, 16 bytes a lane, into four buffers in turn: transfers are issued four steps ahead (a step of 128 x 128
+// takes about 0.3 us, a transfer from the other XCDs' side of memory more than one), fragments are read one step ahead of their
+// products.  One barrier a step: behind it everybody's transfers of the next step have landed and everybody has read this one's.
 //   rows (TR = false): sum over columns [c0, c1) of A[a0 + i][.] B[b0 + j][.]; a block of 32 columns is T rows of 128 bytes, eight
 //     pieces of 16, piece q of row r at place q ^ (r / 2 % 8): the 16 lanes that read one piece of 16 rows meet each bank once.
 //     Rows behind the last are read as the last and never stored.
 //   columns (TR = true): sum over rows [c0, c1) of A[.][a0 + i] B[.][b0 + j]; 32 rows of T columns, piece q of row r at place
 //     q ^ 4 (r % 4); ds_read_b64_tr_b16 hands a lane four rows of its column: the four rows that 16 lanes read lie in different
 //     quarters of the banks.  Column blocks behind the last are read as the last and never stored.
-typedef __attribute__((address_space(3))) void* lds_ptr;
-typedef const __attribute__((address_space(1))) void* glb_ptr;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
@@ -247,18 +248,24 @@ __device__ __forceinline__ half8 ns_read_tr(const char* p, int second) {
     return __builtin_bit_cast(half8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+// 16 bytes a lane from `from` to LDS at `to` + 16 lane.  (Written out: the compiler would wait for every transfer in flight before
+// any LDS read.  Nothing is returned in registers; the waits are NsTile::run's.)
+__device__ __forceinline__ void ns_transfer(const char* from, unsigned to) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory");
+}
+
 template <int T, bool TR>
 struct NsTile {
     static constexpr int S = T / 64;           // 32 x 32 blocks of a wave along each side
-    static constexpr int LOADS = T / 32;       // 16-byte transfers of a lane, per operand and step
-    static constexpr int PART = T * 128;       // bytes of an operand's step of one group
+    static constexpr int LOADS = T / 64;       // 16-byte transfers of a lane, per operand and step
+    static constexpr int PART = T * 128;       // bytes of an operand's step
+    static constexpr int BUFFERS = 4;
     static constexpr int P = T + 2;            // floats between rows of the staged tile: mirrored reads meet each bank once
     f32x16 acc[S][S];
 
     __device__ __forceinline__ void run(const half_t* A, int a0, int a_rows, const half_t* B, int b0, int b_rows, int cols,
                                         int c0, int c1, char* lds) {
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) & 3);
-        const int group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+        const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = all & 3, group = all >> 2;
         const int wr = (wave >> 1) * (T / 2), wc = (wave & 1) * (T / 2);
 #pragma unroll
         for (int i = 0; i < S; ++i)
@@ -266,94 +273,123 @@ struct NsTile {
             for (int j = 0; j < S; ++j)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-        // a step further: 64 columns or 64 rows
-        const size_t stride = TR ? (size_t)64 * cols * 4 : 256;
-        const size_t start = TR ? (size_t)(c0 + group * 32) * cols * 4 : (size_t)c0 * 4 + group * 128;
         const char *pa[LOADS], *pb[LOADS];
 #pragma unroll
         for (int l = 0; l < LOADS; ++l) {
             if constexpr (TR) {
-                const int row = (wave * LOADS + l) * (256 / T) + lane / (T / 4), piece = lane % (T / 4) ^ (4 * (row & 3));
-                const size_t at = start + (size_t)row * cols * 4 + (piece & 7) * 16;
-                pa[l] = (const char*)A + at + (size_t)min(a0 / 32 + (piece >> 3), cols / 32 - 1) * 128;
-                pb[l] = (const char*)B + at + (size_t)min(b0 / 32 + (piece >> 3), cols / 32 - 1) * 128;
+                const int row = (all * LOADS + l) * (256 / T) + lane / (T / 4), piece = lane % (T / 4) ^ (4 * (row & 3));
+                pa[l] = (const char*)A + ((size_t)min(a0 / 32 + (piece >> 3), cols / 32 - 1) * a_rows + c0 + row) * 128 + (piece & 7) * 16;
+                pb[l] = (const char*)B + ((size_t)min(b0 / 32 + (piece >> 3), cols / 32 - 1) * b_rows + c0 + row) * 128 + (piece & 7) * 16;
             } else {
-                const int row = (wave * LOADS + l) * 8 + (lane >> 3), piece = (lane & 7) ^ ((row >> 1) & 7);
-                pa[l] = (const char*)A + start + (size_t)min(a0 + row, a_rows - 1) * cols * 4 + piece * 16;
-                pb[l] = (const char*)B + start + (size_t)min(b0 + row, b_rows - 1) * cols * 4 + piece * 16;
+                const int row = (all * LOADS + l) * 8 + (lane >> 3), piece = (lane & 7) ^ ((row >> 1) & 7);
+                pa[l] = (const char*)A + ((size_t)(c0 / 32) * a_rows + min(a0 + row, a_rows - 1)) * 128 + piece * 16;
+                pb[l] = (const char*)B + ((size_t)(c0 / 32) * b_rows + min(b0 + row, b_rows - 1)) * 128 + piece * 16;
             }
         }
-        auto fetch = [&](int buffer, size_t ahead) {
-            char* to = lds + buffer * (4 * PART) + group * (2 * PART) + wave * LOADS * 1024;
+        // a step further: 32 rows, or the next block of 32 columns
+        const size_t stride_a = TR ? 32 * 128 : (size_t)a_rows * 128, stride_b = TR ? 32 * 128 : (size_t)b_rows * 128;
+        const unsigned to = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds + all * LOADS * 1024;
+        auto fetch = [&](int step) {
+            const unsigned dst = to + (step % BUFFERS) * (2 * PART);
 #pragma unroll
             for (int l = 0; l < LOADS; ++l) {
-                __builtin_amdgcn_global_load_lds((glb_ptr)(pa[l] + ahead), (lds_ptr)(to + l * 1024), 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((glb_ptr)(pb[l] + ahead), (lds_ptr)(to + PART + l * 1024), 16, 0, 0);
+                ns_transfer(pa[l], dst + l * 1024);
+                ns_transfer(pb[l], dst + PART + l * 1024);
+                pa[l] += stride_a;
+                pb[l] += stride_b;
             }
         };
-        int at_a[S][2], at_b[S][2];      // hi; lo: bit 6 flipped
+        int at_a[S], at_b[S];      // hi; lo: bit 6 flipped
 #pragma unroll
-        for (int i = 0; i < S; ++i)
-#pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                if constexpr (TR) {
-                    const int g = lane >> 4, q = (lane & 15) >> 2, p = lane & 3, chunk = 2 * (g & 1) + (p >> 1);
-                    const int row = (kk * 16 + 8 * (g >> 1) + q) * (T * 4) + (p & 1) * 8;
-                    at_a[i][kk] = row + ((((wr / 32 + i) * 8 + chunk) ^ (4 * q)) << 4);
-                    at_b[i][kk] = PART + row + ((((wc / 32 + i) * 8 + chunk) ^ (4 * q)) << 4);
-                } else {
-                    const int q = kk * 2 + (lane >> 5), r = wr + i * 32 + (lane & 31), c = wc + i * 32 + (lane & 31);
-                    at_a[i][kk] = r * 128 + ((q ^ ((r >> 1) & 7)) << 4);
-                    at_b[i][kk] = PART + c * 128 + ((q ^ ((c >> 1) & 7)) << 4);
-                }
-            }
-        const int steps = (c1 - c0) / 64;
-        fetch(0, 0);
-        size_t ahead = 0;
-        for (int step = 0; step < steps; ++step) {
-            const char* now = lds + (step & 1) * (4 * PART) + group * (2 * PART);
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            half8 ah[2][S], al[2][S], bh[2][S], bl[2][S];
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int i = 0; i < S; ++i) {
-                    if constexpr (TR) {
-                        ah[k][i] = ns_read_tr(now + at_a[i][k], T * 16);
-                        bh[k][i] = ns_read_tr(now + at_b[i][k], T * 16);
-                        al[k][i] = ns_read_tr(now + (at_a[i][k] ^ 64), T * 16);
-                        bl[k][i] = ns_read_tr(now + (at_b[i][k] ^ 64), T * 16);
-                    } else {
-                        ah[k][i] = *(const half8*)(now + at_a[i][k]);
-                        bh[k][i] = *(const half8*)(now + at_b[i][k]);
-                        al[k][i] = *(const half8*)(now + (at_a[i][k] ^ 64));
-                        bl[k][i] = *(const half8*)(now + (at_b[i][k] ^ 64));
-                    }
-                }
-            // (unconditional: behind the last step the same step again, into the buffer nobody reads any more)
-            ahead += step + 1 < steps ? stride : 0;
-            fetch((step + 1) & 1, ahead);
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-#pragma unroll
-                for (int i = 0; i < S; ++i)
-#pragma unroll
-                    for (int j = 0; j < S; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[k][i], bh[k][j], acc[i][j], 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < S; ++i)
-#pragma unroll
-                    for (int j = 0; j < S; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[k][i], bl[k][j], acc[i][j], 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < S; ++i)
-#pragma unroll
-                    for (int j = 0; j < S; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[k][i], bh[k][j], acc[i][j], 0, 0, 0);
+        for (int i = 0; i < S; ++i) {
+            if constexpr (TR) {
+                const int g = lane >> 4, q = (lane & 15) >> 2, p = lane & 3, chunk = 2 * (g & 1) + (p >> 1);
+                const int row = (group * 16 + 8 * (g >> 1) + q) * (T * 4) + (p & 1) * 8;
+                at_a[i] = row + ((((wr / 32 + i) * 8 + chunk) ^ (4 * q)) << 4);
+                at_b[i] = PART + row + ((((wc / 32 + i) * 8 + chunk) ^ (4 * q)) << 4);
+            } else {
+                const int q = group * 2 + (lane >> 5), r = wr + i * 32 + (lane & 31), c = wc + i * 32 + (lane & 31);
+                at_a[i] = r * 128 + ((q ^ ((r >> 1) & 7)) << 4);
+                at_b[i] = PART + c * 128 + ((q ^ ((c >> 1) & 7)) << 4);
             }
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        struct Fragments {
+            half8 ah[S], al[S], bh[S], bl[S];
+        };
+        auto read = [&](Fragments& f, int step) {
+            const char* now = lds + (step % BUFFERS) * (2 * PART);
+#pragma unroll
+            for (int i = 0; i < S; ++i) {
+                if constexpr (TR) {
+                    f.ah[i] = ns_read_tr(now + at_a[i], T * 16);
+                    f.bh[i] = ns_read_tr(now + at_b[i], T * 16);
+                    f.al[i] = ns_read_tr(now + (at_a[i] ^ 64), T * 16);
+                    f.bl[i] = ns_read_tr(now + (at_b[i] ^ 64), T * 16);
+                } else {
+                    f.ah[i] = *(const half8*)(now + at_a[i]);
+                    f.bh[i] = *(const half8*)(now + at_b[i]);
+                    f.al[i] = *(const half8*)(now + (at_a[i] ^ 64));
+                    f.bl[i] = *(const half8*)(now + (at_b[i] ^ 64));
+                }
+            }
+        };
+        // (pinned between the reads before and the meeting behind: the scheduler would carry products over the barrier, to where
+        // the next reads are waited for)
+        auto multiply = [&](const Fragments& f) {
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < S; ++i)
+#pragma unroll
+                for (int j = 0; j < S; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.al[i], f.bh[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < S; ++i)
+#pragma unroll
+                for (int j = 0; j < S; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[i], f.bl[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < S; ++i)
+#pragma unroll
+                for (int j = 0; j < S; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[i], f.bh[j], acc[i][j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        const int steps = (c1 - c0) / 32;
+        // this wave's LDS reads are done (0xC07F: lgkmcnt(0)) and its transfers but those of the last `behind` steps have landed;
+        // then everybody's
+        auto meet = [&](int behind) {
+            __builtin_amdgcn_s_waitcnt(0xC07F);
+            if (behind >= 3) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(6 * LOADS) : "memory");
+            else if (behind == 2) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(4 * LOADS) : "memory");
+            else if (behind == 1) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        };
+        auto turn = [&](const Fragments& now, Fragments& next, int step) {
+            meet(2);
+            read(next, step + 1);
+            fetch(step + BUFFERS);
+            multiply(now);
+        };
+        auto last_turn = [&](const Fragments& now, Fragments& next, int step) {
+            if (step + 1 < steps) {
+                meet(min(2, steps - 2 - step));
+                read(next, step + 1);
+            }
+            if (step + BUFFERS < steps) fetch(step + BUFFERS);
+            multiply(now);
+        };
+        Fragments f0, f1;
+        for (int step = 0; step < min(steps, BUFFERS); ++step) fetch(step);
+        meet(min(steps, BUFFERS) - 1);
+        read(f0, 0);
+        int step = 0;
+        for (; step + 3 + BUFFERS < steps; step += 4) {
+            turn(f0, f1, step);
+            turn(f1, f0, step + 1);
+            turn(f0, f1, step + 2);
+            turn(f1, f0, step + 3);
+        }
+        for (; step < steps; step += 2) {
+            last_turn(f0, f1, step);
+            if (step + 1 < steps) last_turn(f1, f0, step + 1);
+        }
         __syncthreads();
     }
     // the sums of both groups, second first, into LDS: tile[row][col], rows P apart
@@ -379,7 +415,7 @@ struct NsTile {
     }
 };
 
-#define NS_LDS(T) (T * 128 * 8)      // two steps' operands of both groups; the staged tile is smaller
+#define NS_LDS(T) (T * 128 * 8)      // four steps' operands; the staged tile is smaller
 
 // tile number -> (i, j), i <= j, of a triangle of `t` rows
 __device__ __forceinline__ void ns_pair(int l, int t, int& i, int& j) {
@@ -394,7 +430,8 @@ __device__ __forceinline__ void ns_symmetric(half_t* out, int kp, int r0, int c0
     for (int q = threadIdx.x; q < T * T / 8; q += THREADS) {
         float v[8];
         half8 hi, lo;
-        int row = q / (T / 8), col = q % (T / 8) * 8;
+        // (four lanes along a row of a block, sixteen down its rows: contiguous)
+        int row = q / 4 % T, col = (q & 3) * 8 + q / (4 * T) * 32;
         if (r0 + row < kp && c0 + col < kp) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = tile[row * P + col + e];
@@ -403,9 +440,6 @@ __device__ __forceinline__ void ns_symmetric(half_t* out, int kp, int r0, int c0
             *(half8*)(out + o) = hi;
             *(half8*)(out + o + 32) = lo;
         }
-        // (sixteen lanes along the tile's columns, four down its rows: 64 contiguous bytes of a mirrored row)
-        row = (q >> 2 & 15) + (q / 64 % (T / 16)) * 16;
-        col = ((q & 3) + q / (4 * T) * 4) * 8;
         if (r0 != c0 && c0 + row < kp && r0 + col < kp) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = tile[(col + e) * P + row];
@@ -485,7 +519,7 @@ __device__ __forceinline__ void ns_poly(const NsMat& m, float cb, float cc, char
     float* tile = (float*)lds;
     t.stage(tile);
     for (int q = threadIdx.x; q < T * T / 8; q += NS_WIDE) {
-        const int row = q / (T / 8), col = q % (T / 8) * 8;
+        const int row = q / 4 % T, col = (q & 3) * 8 + q / (4 * T) * 32;
         if (i * T + row >= m.kp || j * T + col >= m.kp) continue;
         const size_t o = ns_at(i * T + row, j * T + col, m.kp);
         const half8 hi = *(const half8*)(g + o), lo = *(const half8*)(g + o + 32);
@@ -536,15 +570,15 @@ __device__ __forceinline__ void ns_apply(const NsMat& m, int from, float ca, boo
     half8 xh[EACH], xl[EACH];
 #pragma unroll
     for (int l = 0; l < EACH; ++l) {
-        const int q = l * NS_WIDE + threadIdx.x, row = q / (T / 8), col = q % (T / 8) * 8;
-        const size_t o = ns_at(min(n0 + row, m.np - 1), min(k0 + col, m.kp - 8), m.kp);
+        const int q = l * NS_WIDE + threadIdx.x, row = q / 4 % T, col = (q & 3) * 8 + q / (4 * T) * 32;
+        const size_t o = ns_at(min(n0 + row, m.np - 1), min(k0 + col, m.kp - 8), m.np);
         xh[l] = *(const half8*)(x + o);
         xl[l] = *(const half8*)(x + o + 32);
     }
     t.stage(tile);
 #pragma unroll
     for (int l = 0; l < EACH; ++l) {
-        const int q = l * NS_WIDE + threadIdx.x, row = q / (T / 8), col = q % (T / 8) * 8;
+        const int q = l * NS_WIDE + threadIdx.x, row = q / 4 % T, col = (q & 3) * 8 + q / (4 * T) * 32;
         if (n0 + row >= m.np || k0 + col >= m.kp) continue;
         float v[8];
 #pragma unroll
@@ -556,7 +590,7 @@ __device__ __forceinline__ void ns_apply(const NsMat& m, int from, float ca, boo
         if (!last) {
             half8 hi, lo;
             ns_split8(v, hi, lo);
-            const size_t o = ns_at(n0 + row, k0 + col, m.kp);
+            const size_t o = ns_at(n0 + row, k0 + col, m.np);
             *(half8*)(out + o) = hi;
             *(half8*)(out + o + 32) = lo;
         }
