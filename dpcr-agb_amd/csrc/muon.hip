@@ -289,15 +289,20 @@ struct NsTile {
         // a step further: 32 rows, or the next block of 32 columns
         const size_t stride_a = TR ? 32 * 128 : (size_t)a_rows * 128, stride_b = TR ? 32 * 128 : (size_t)b_rows * 128;
         const unsigned to = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds + all * LOADS * 1024;
-        auto fetch = [&](int step) {
-            const unsigned dst = to + (step % BUFFERS) * (2 * PART);
-#pragma unroll
-            for (int l = 0; l < LOADS; ++l) {
-                ns_transfer(pa[l], dst + l * 1024);
-                ns_transfer(pb[l], dst + PART + l * 1024);
-                pa[l] += stride_a;
-                pb[l] += stride_b;
+        // transfer `l` of the 2 LOADS of a step; the second of a pair moves its pointers on
+        auto fetch1 = [&](int step, int l) {
+            const unsigned dst = to + (step % BUFFERS) * (2 * PART) + (l >> 1) * 1024;
+            if (l & 1) {
+                ns_transfer(pb[l >> 1], dst + PART);
+                pb[l >> 1] += stride_b;
+            } else {
+                ns_transfer(pa[l >> 1], dst);
+                pa[l >> 1] += stride_a;
             }
+        };
+        auto fetch = [&](int step) {
+#pragma unroll
+            for (int l = 0; l < 2 * LOADS; ++l) fetch1(step, l);
         };
         int at_a[S], at_b[S];      // hi; lo: bit 6 flipped
 #pragma unroll
@@ -316,40 +321,38 @@ struct NsTile {
         struct Fragments {
             half8 ah[S], al[S], bh[S], bl[S];
         };
-        auto read = [&](Fragments& f, int step) {
+        // fragment `l` of the 4 S of a step, those of the first products first
+        auto read1 = [&](Fragments& f, int step, int l) {
             const char* now = lds + (step % BUFFERS) * (2 * PART);
-#pragma unroll
-            for (int i = 0; i < S; ++i) {
-                if constexpr (TR) {
-                    f.ah[i] = ns_read_tr(now + at_a[i], T * 16);
-                    f.bh[i] = ns_read_tr(now + at_b[i], T * 16);
-                    f.al[i] = ns_read_tr(now + (at_a[i] ^ 64), T * 16);
-                    f.bl[i] = ns_read_tr(now + (at_b[i] ^ 64), T * 16);
-                } else {
-                    f.ah[i] = *(const half8*)(now + at_a[i]);
-                    f.bh[i] = *(const half8*)(now + at_b[i]);
-                    f.al[i] = *(const half8*)(now + (at_a[i] ^ 64));
-                    f.bl[i] = *(const half8*)(now + (at_b[i] ^ 64));
-                }
-            }
+            const int i = l % (2 * S) / 2, lo = (l / (2 * S)) ^ !(l & 1);       // al, bh of every block, then ah, bl
+            const char* p = now + ((l & 1 ? at_b[i] : at_a[i]) ^ (lo ? 64 : 0));
+            half8& to = l & 1 ? (lo ? f.bl[i] : f.bh[i]) : (lo ? f.al[i] : f.ah[i]);
+            to = TR ? ns_read_tr(p, T * 16) : *(const half8*)p;
         };
-        // (pinned between the reads before and the meeting behind: the scheduler would carry products over the barrier, to where
-        // the next reads are waited for)
-        auto multiply = [&](const Fragments& f) {
-            __builtin_amdgcn_sched_barrier(0);
+        auto multiply1 = [&](const Fragments& f, int l) {
+            const int i = l / S % S, j = l % S, kind = l / (S * S);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kind == 0 ? f.al[i] : f.ah[i], kind == 1 ? f.bl[j] : f.bh[j], acc[i][j],
+                                                               0, 0, 0);
+        };
+        // A step's products with the next step's reads and a later one's transfers between them, two to a product at first: what is
+        // issued while the matrix pipe is busy costs nothing.  (The scheduler is held off: it gathers the reads, and carries
+        // products over the meeting, to where those reads are waited for.)
+        auto mixed = [&](const Fragments& now, Fragments& next, int step, bool more, bool further) {
+            constexpr int READS = 4 * S, TRANSFERS = 2 * LOADS, PRODUCTS = 3 * S * S, EACH = (READS + TRANSFERS + PRODUCTS - 1) / PRODUCTS;
 #pragma unroll
-            for (int i = 0; i < S; ++i)
+            for (int l = 0; l < PRODUCTS; ++l) {
+                multiply1(now, l);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int j = 0; j < S; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.al[i], f.bh[j], acc[i][j], 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < S; ++i)
-#pragma unroll
-                for (int j = 0; j < S; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[i], f.bl[j], acc[i][j], 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < S; ++i)
-#pragma unroll
-                for (int j = 0; j < S; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[i], f.bh[j], acc[i][j], 0, 0, 0);
-            __builtin_amdgcn_sched_barrier(0);
+                for (int e = l * EACH; e < (l + 1) * EACH; ++e) {
+                    if (e < READS) {
+                        if (more) read1(next, step + 1, e);
+                    } else if (e < READS + TRANSFERS) {
+                        if (further) fetch1(step + BUFFERS, e - READS);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
         };
         const int steps = (c1 - c0) / 32;
         // this wave's LDS reads are done (0xC07F: lgkmcnt(0)) and its transfers but those of the last `behind` steps have landed;
@@ -363,22 +366,17 @@ struct NsTile {
         };
         auto turn = [&](const Fragments& now, Fragments& next, int step) {
             meet(2);
-            read(next, step + 1);
-            fetch(step + BUFFERS);
-            multiply(now);
+            mixed(now, next, step, true, true);
         };
         auto last_turn = [&](const Fragments& now, Fragments& next, int step) {
-            if (step + 1 < steps) {
-                meet(min(2, steps - 2 - step));
-                read(next, step + 1);
-            }
-            if (step + BUFFERS < steps) fetch(step + BUFFERS);
-            multiply(now);
+            if (step + 1 < steps) meet(min(2, steps - 2 - step));
+            mixed(now, next, step, step + 1 < steps, step + BUFFERS < steps);
         };
         Fragments f0, f1;
         for (int step = 0; step < min(steps, BUFFERS); ++step) fetch(step);
         meet(min(steps, BUFFERS) - 1);
-        read(f0, 0);
+#pragma unroll
+        for (int l = 0; l < 4 * S; ++l) read1(f0, 0, l);
         int step = 0;
         for (; step + 3 + BUFFERS < steps; step += 4) {
             turn(f0, f1, step);
