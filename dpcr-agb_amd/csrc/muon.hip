@@ -39,7 +39,7 @@ struct __attribute__((aligned(16))) NsMat {
     long long in_ld, in_bs, out_ld, out_bs;
     int rows, cols, batch, type;      // type of `in` (and of `out` where nothing is updated): 0 fp32, 1 bf16, 2 fp16
     int k, n, kp, np, tall;
-    int vec;                          // contiguous and aligned: four elements at a time
+    int vec, out_vec;                 // input contiguous and aligned: four elements at a time; output rows aligned: eight
     int tile, kt, nt, tri, splits, chunk;      // tile of G and X; tiles along k and n; tiles on and above the diagonal
     int tile_p, kt_p, tri_p;                   // tile of P
     int sums;                                  // partial sums of squares per matrix
@@ -48,7 +48,7 @@ struct __attribute__((aligned(16))) NsMat {
     float* part;
     double* sq;
     int at[6];      // first workgroup in the launches over: NS_CHUNKs, 64 x 64 blocks of X, G tiles x splits, X tiles, P tiles,
-                    // 32 x 32 blocks of G tiles (fold)
+                    // units of G tiles (fold)
 };
 
 // ---- pairs of fp16
@@ -260,7 +260,6 @@ struct NsTile {
     static constexpr int LOADS = T / 64;       // 16-byte transfers of a lane, per operand and step
     static constexpr int PART = T * 128;       // bytes of an operand's step
     static constexpr int BUFFERS = 4;
-    static constexpr int P = T + 2;            // floats between rows of the staged tile: mirrored reads meet each bank once
     f32x16 acc[S][S];
 
     __device__ __forceinline__ void run(const half_t* A, int a0, int a_rows, const half_t* B, int b0, int b_rows, int cols,
@@ -390,30 +389,137 @@ struct NsTile {
         }
         __syncthreads();
     }
-    // the sums of both groups, second first, into LDS: tile[row][col], rows P apart
-    __device__ __forceinline__ void stage(float* tile) {
+    // Adds the two groups' sums.  T = 128: group g is left with blocks j == g (32 rows of B x 64 of A a wave); T = 64: group 0 with
+    // everything.  false: this wave is left with nothing.
+    static constexpr int UC = 32 * S;          // a wave's unit: 32 rows of B by UC of A
+    __device__ __forceinline__ bool merge(char* lds) {
         const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) & 3, group = threadIdx.x >> 8;
-        float* at = tile + ((wave >> 1) * (T / 2) + 4 * (lane >> 5)) * P + (wave & 1) * (T / 2) + (lane & 31);
+        float4* box = (float4*)lds + (wave * S * 2) * 4 * 64 + lane;
+        if constexpr (S == 2) {
+            // (every wave puts the blocks of the other group; boxes: [wave][giver's blocks i][quad])
+            float4* mine = box + group * S * 4 * 64;
 #pragma unroll
-        for (int turn = 1; turn >= 0; --turn) {
-            if (group == turn) {
+            for (int i = 0; i < S; ++i)
 #pragma unroll
-                for (int i = 0; i < S; ++i)
+                for (int q = 0; q < 4; ++q) {
+                    float4 v;
+                    v.x = group ? acc[i][0][4 * q] : acc[i][1][4 * q];
+                    v.y = group ? acc[i][0][4 * q + 1] : acc[i][1][4 * q + 1];
+                    v.z = group ? acc[i][0][4 * q + 2] : acc[i][1][4 * q + 2];
+                    v.w = group ? acc[i][0][4 * q + 3] : acc[i][1][4 * q + 3];
+                    mine[(i * 4 + q) * 64] = v;
+                }
+            __syncthreads();
+            const float4* theirs = box + (group ^ 1) * S * 4 * 64;
 #pragma unroll
-                    for (int j = 0; j < S; ++j)
+            for (int i = 0; i < S; ++i)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            float* p = at + (i * 32 + (e & 3) + 8 * (e >> 2)) * P + j * 32;
-                            const float v = acc[i][j][e] * (NS_UNSCALE * NS_UNSCALE);
-                            *p = turn ? v : *p + v;
-                        }
+                for (int q = 0; q < 4; ++q) {
+                    const float4 v = theirs[(i * 4 + q) * 64];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float own = group ? acc[i][1][4 * q + e] : acc[i][0][4 * q + e];
+                        acc[i][0][4 * q + e] = own + (e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w);
+                    }
+                }
+            __syncthreads();      // (the boxes are free for what follows)
+            return true;
+        } else {
+            if (group) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    box[q * 64] = make_float4(acc[0][0][4 * q], acc[0][0][4 * q + 1], acc[0][0][4 * q + 2], acc[0][0][4 * q + 3]);
             }
             __syncthreads();
+            if (!group) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float4 v = box[q * 64];
+                    acc[0][0][4 * q] += v.x;
+                    acc[0][0][4 * q + 1] += v.y;
+                    acc[0][0][4 * q + 2] += v.z;
+                    acc[0][0][4 * q + 3] += v.w;
+                }
+            }
+            __syncthreads();
+            return !group;
         }
     }
+    // first row (of B's) and column (of A's) of this wave's unit in the tile, and its number
+    __device__ __forceinline__ int unit_row() const {
+        return (threadIdx.x >> 6 & 1) * (T / 2) + (S == 2 ? (threadIdx.x >> 8) * 32 : 0);
+    }
+    __device__ __forceinline__ int unit_col() const { return (threadIdx.x >> 7 & 1) * (T / 2); }
+    static constexpr int UNITS = S == 2 ? 8 : 4;
+    __device__ __forceinline__ int unit() const { return threadIdx.x >> 6; }
+    // quad q of block i of the unit (four columns of one row), as the product left it: scaled by 2^26
+    __device__ __forceinline__ float4 quad(int i, int q) const {
+        return make_float4(acc[i][0][4 * q], acc[i][0][4 * q + 1], acc[i][0][4 * q + 2], acc[i][0][4 * q + 3]);
+    }
+    __device__ __forceinline__ void stage(float* unit) const;
 };
 
-#define NS_LDS(T) (T * 128 * 8)      // four steps' operands; the staged tile is smaller
+#define NS_LDS(T) (T * 128 * 8)      // four steps' operands; the boxes and the staged units are smaller
+
+// A unit in LDS: 32 rows of UC columns, rows UC + 4 floats apart (the lanes that write or read 16 bytes together meet each bank
+// once).  It belongs to one wave (or, in the fold, to the workgroup).
+template <int UC>
+__device__ __forceinline__ void ns_put_quad(float* unit, int i, int q, int lane, float4 v) {
+    const float s = NS_UNSCALE * NS_UNSCALE;
+    *(float4*)(unit + (lane & 31) * (UC + 4) + i * 32 + q * 8 + (lane >> 5) * 4) = make_float4(v.x * s, v.y * s, v.z * s, v.w * s);
+}
+template <int T, bool TR>
+__device__ __forceinline__ void NsTile<T, TR>::stage(float* unit) const {
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) ns_put_quad<UC>(unit, i, q, threadIdx.x & 63, quad(i, q));
+    __builtin_amdgcn_wave_barrier();      // (LDS serves a wave in order)
+}
+// groups of eight of a unit: number `l` of a thread among `threads`; along a row (four lanes a block's row, sixteen rows) or down
+// the rows (four lanes down a column, sixteen columns)
+template <int UC>
+__device__ __forceinline__ void ns_group(int q, int& row, int& col) {
+    row = q >> 2 & 31;
+    col = (q & 3) * 8 + (q >> 7) * 32;
+}
+template <int UC>
+__device__ __forceinline__ void ns_along(const float* unit, int row, int col, float* v) {
+    const float4 a = *(const float4*)(unit + row * (UC + 4) + col), b = *(const float4*)(unit + row * (UC + 4) + col + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+template <int UC>
+__device__ __forceinline__ void ns_down(const float* unit, int q, int& row, int& col, float* v) {
+    row = (q & 3) * 8;
+    col = q >> 2;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = unit[(row + e) * (UC + 4) + col];
+}
+__device__ __forceinline__ void ns_write8(half_t* out, size_t o, const float* v) {
+    half8 hi, lo;
+    ns_split8(v, hi, lo);
+    *(half8*)(out + o) = hi;
+    *(half8*)(out + o + 32) = lo;
+}
+// a unit at rows r0, columns c0 of a symmetric plane pair [kp][kp], and its mirror image unless it lies in a diagonal tile
+template <int UC, int THREADS>
+__device__ __forceinline__ void ns_symmetric(half_t* out, int kp, int r0, int c0, bool diagonal, const float* unit, int t) {
+    float v[8];
+    int row, col;
+#pragma unroll
+    for (int q = t; q < 4 * UC; q += THREADS) {
+        ns_group<UC>(q, row, col);
+        ns_along<UC>(unit, row, col, v);
+        if (r0 + row < kp && c0 + col < kp) ns_write8(out, ns_at(r0 + row, c0 + col, kp), v);
+    }
+    if (diagonal) return;
+#pragma unroll
+    for (int q = t; q < 4 * UC; q += THREADS) {
+        ns_down<UC>(unit, q, row, col, v);
+        if (r0 + row < kp && c0 + col < kp) ns_write8(out, ns_at(c0 + col, r0 + row, kp), v);
+    }
+}
 
 // tile number -> (i, j), i <= j, of a triangle of `t` rows
 __device__ __forceinline__ void ns_pair(int l, int t, int& i, int& j) {
@@ -421,38 +527,18 @@ __device__ __forceinline__ void ns_pair(int l, int t, int& i, int& j) {
     while (l >= t - i) { l -= t - i; ++i; }
     j = i + l;
 }
-
-// rows [r0, r0 + T) and columns [c0, c0 + T) of a symmetric plane pair [kp][kp] from the staged tile, and its mirror image
-template <int T, int P, int THREADS>
-__device__ __forceinline__ void ns_symmetric(half_t* out, int kp, int r0, int c0, const float* tile) {
-    for (int q = threadIdx.x; q < T * T / 8; q += THREADS) {
-        float v[8];
-        half8 hi, lo;
-        // (four lanes along a row of a block, sixteen down its rows: contiguous)
-        int row = q / 4 % T, col = (q & 3) * 8 + q / (4 * T) * 32;
-        if (r0 + row < kp && c0 + col < kp) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = tile[row * P + col + e];
-            ns_split8(v, hi, lo);
-            const size_t o = ns_at(r0 + row, c0 + col, kp);
-            *(half8*)(out + o) = hi;
-            *(half8*)(out + o + 32) = lo;
-        }
-        if (r0 != c0 && c0 + row < kp && r0 + col < kp) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = tile[(col + e) * P + row];
-            ns_split8(v, hi, lo);
-            const size_t o = ns_at(c0 + row, r0 + col, kp);
-            *(half8*)(out + o) = hi;
-            *(half8*)(out + o + 32) = lo;
-        }
-    }
+// workgroup number within a matrix's `count` -> number of its piece of work: consecutive pieces, which share operands, to
+// workgroups 8 apart, which share an XCD and its L2
+__device__ __forceinline__ int ns_order(int at, int count) {
+    const int each = count >> 3, more = count & 7, xcd = at & 7;
+    return xcd * each + min(xcd, more) + (at >> 3);
 }
 
 // G = X^T X, a chunk of n at a time
 template <int T>
 __device__ __forceinline__ void ns_gram(const NsMat& m, int from, char* lds) {
-    int at = blockIdx.x - m.at[NS_GRAM];
+    typedef NsTile<T, true> Tile;
+    int at = ns_order(blockIdx.x - m.at[NS_GRAM], m.tri * m.splits * m.batch);
     const int b = at / (m.tri * m.splits);
     at %= m.tri * m.splits;
     const int split = at / m.tri, l = at % m.tri;
@@ -460,15 +546,20 @@ __device__ __forceinline__ void ns_gram(const NsMat& m, int from, char* lds) {
     ns_pair(l, m.kt, i, j);
     const half_t* x = m.xt[from] + (size_t)b * m.np * m.kp * 2;
     const int c0 = split * m.chunk, c1 = min(m.np, c0 + m.chunk);
-    NsTile<T, true> t;
+    Tile t;
     t.run(x, i * T, m.np, x, j * T, m.np, m.kp, c0, c1, lds);
-    float* tile = (float*)lds;
-    t.stage(tile);
+    if (!t.merge(lds)) return;
+    const int unit = t.unit(), lane = threadIdx.x & 63;
     if (m.splits == 1) {
-        ns_symmetric<T, T + 2, NS_WIDE>(m.g + (size_t)b * m.kp * m.kp * 2, m.kp, i * T, j * T, tile);
-    } else {
-        float* out = m.part + (((size_t)b * m.splits + split) * m.tri + l) * (T * T);
-        for (int q = threadIdx.x; q < T * T; q += NS_WIDE) out[q] = tile[q / T * (T + 2) + q % T];
+        float* mine = (float*)lds + unit * 32 * (Tile::UC + 4);
+        t.stage(mine);
+        ns_symmetric<Tile::UC, 64>(m.g + (size_t)b * m.kp * m.kp * 2, m.kp, j * T + t.unit_row(), i * T + t.unit_col(), i == j, mine, lane);
+    } else {      // [batch][split][tile][unit][quad][lane]
+        float4* out = (float4*)m.part + ((((size_t)b * m.splits + split) * m.tri + l) * Tile::UNITS + unit) * (Tile::S * 4 * 64) + lane;
+#pragma unroll
+        for (int i = 0; i < Tile::S; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) out[(i * 4 + q) * 64] = t.quad(i, q);
     }
 }
 __global__ __launch_bounds__(NS_WIDE) void k_ns_gram(const NsMat* tab, int count, int from) {
@@ -478,57 +569,76 @@ __global__ __launch_bounds__(NS_WIDE) void k_ns_gram(const NsMat* tab, int count
     else ns_gram<64>(m, from, lds);
 }
 
-// the chunks' sums in order, a 32 x 32 block of a tile
-__global__ __launch_bounds__(NS_THREADS) void k_ns_fold(const NsMat* tab, int count) {
-    const NsMat& m = ns_find<NS_FOLD>(tab, count);
-    __shared__ float tile[32 * 34];
-    const int T = m.tile, sub = T / 32;
+// the chunks' sums in order, a unit of a tile
+template <int T>
+__device__ __forceinline__ void ns_fold(const NsMat& m, float* unit) {
+    typedef NsTile<T, true> Tile;
     int at = blockIdx.x - m.at[NS_FOLD];
-    const int b = at / (m.tri * sub * sub);
-    at %= m.tri * sub * sub;
-    const int l = at / (sub * sub), r = at % (sub * sub) / sub * 32, c = at % sub * 32;
+    const int u = at % Tile::UNITS, l = at / Tile::UNITS % m.tri, b = at / Tile::UNITS / m.tri;
     int i, j;
     ns_pair(l, m.kt, i, j);
-    if (i == j && c < r) return;      // (its mirror image writes it)
-    const int row = threadIdx.x >> 3, col = (threadIdx.x & 7) * 4;
-    const float* in = m.part + ((size_t)b * m.splits * m.tri + l) * (T * T) + (r + row) * T + c + col;
-    const size_t next = (size_t)m.tri * T * T;
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const size_t next = (size_t)m.tri * Tile::UNITS * (Tile::S * 4 * 64);
+#pragma unroll
+    for (int s = 0; s < Tile::S; ++s) {
+        const int quad = wave * Tile::S + s;      // (Tile::S * 4 of them by four waves)
+        const float4* in = (const float4*)m.part + (((size_t)b * m.splits * m.tri + l) * Tile::UNITS + u) * (Tile::S * 4 * 64) + quad * 64 + lane;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-    for (int p = 0; p < m.splits; ++p) {
-        const float4 v = *(const float4*)(in + p * next);
-        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        for (int p = 0; p < m.splits; ++p) {
+            const float4 v = in[p * next];
+            sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+        }
+        ns_put_quad<Tile::UC>(unit, quad / 4, quad % 4, lane, sum);
     }
-    float* o = tile + row * 34 + col;
-    o[0] = s.x; o[1] = s.y; o[2] = s.z; o[3] = s.w;
     __syncthreads();
-    ns_symmetric<32, 34, NS_THREADS>(m.g + (size_t)b * m.kp * m.kp * 2, m.kp, i * T + r, j * T + c, tile);
+    const int row = (u & 1) * (T / 2) + (Tile::S == 2 ? (u >> 2) * 32 : 0), col = (u >> 1 & 1) * (T / 2);
+    ns_symmetric<Tile::UC, NS_THREADS>(m.g + (size_t)b * m.kp * m.kp * 2, m.kp, j * T + row, i * T + col, i == j, unit, threadIdx.x);
+}
+__global__ __launch_bounds__(NS_THREADS) void k_ns_fold(const NsMat* tab, int count) {
+    const NsMat& m = ns_find<NS_FOLD>(tab, count);
+    __shared__ __align__(16) float unit[32 * 68];
+    if (m.tile == 128) ns_fold<128>(m, unit);
+    else ns_fold<64>(m, unit);
 }
 
 // P = b G + c G G
 template <int T>
 __device__ __forceinline__ void ns_poly(const NsMat& m, float cb, float cc, char* lds) {
-    const int at = blockIdx.x - m.at[NS_POLY], b = at / m.tri_p;
+    typedef NsTile<T, false> Tile;
+    const int at = ns_order(blockIdx.x - m.at[NS_POLY], m.tri_p * m.batch), b = at / m.tri_p;
     int i, j;
     ns_pair(at % m.tri_p, m.kt_p, i, j);
     const half_t* g = m.g + (size_t)b * m.kp * m.kp * 2;
-    NsTile<T, false> t;
+    Tile t;
     t.run(g, i * T, m.kp, g, j * T, m.kp, m.kp, 0, m.kp, lds);
-    float* tile = (float*)lds;
-    t.stage(tile);
-    for (int q = threadIdx.x; q < T * T / 8; q += NS_WIDE) {
-        const int row = q / 4 % T, col = (q & 3) * 8 + q / (4 * T) * 32;
-        if (i * T + row >= m.kp || j * T + col >= m.kp) continue;
-        const size_t o = ns_at(i * T + row, j * T + col, m.kp);
-        const half8 hi = *(const half8*)(g + o), lo = *(const half8*)(g + o + 32);
+    if (!t.merge(lds)) return;
+    const int lane = threadIdx.x & 63, r0 = j * T + t.unit_row(), c0 = i * T + t.unit_col();
+    float* mine = (float*)lds + t.unit() * 32 * (Tile::UC + 4);
+    constexpr int EACH = Tile::UC / 16;
+    half8 gh[EACH], gl[EACH];
+    int row, col;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float* v = tile + row * (T + 2) + col + e;
-            *v = cc * *v + cb * (((float)hi[e] + (float)lo[e]) * NS_UNSCALE);
-        }
+    for (int l = 0; l < EACH; ++l) {
+        ns_group<Tile::UC>(l * 64 + lane, row, col);
+        const size_t o = ns_at(min(r0 + row, m.kp - 1), min(c0 + col, m.kp - 8), m.kp);
+        gh[l] = *(const half8*)(g + o);
+        gl[l] = *(const half8*)(g + o + 32);
     }
-    __syncthreads();
-    ns_symmetric<T, T + 2, NS_WIDE>(m.p + (size_t)b * m.kp * m.kp * 2, m.kp, i * T, j * T, tile);
+    t.stage(mine);
+#pragma unroll
+    for (int l = 0; l < EACH; ++l) {
+        ns_group<Tile::UC>(l * 64 + lane, row, col);
+        float v[8];
+        ns_along<Tile::UC>(mine, row, col, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = cc * v[e] + cb * (((float)gh[l][e] + (float)gl[l][e]) * NS_UNSCALE);
+        float4* p = (float4*)(mine + row * (Tile::UC + 4) + col);
+        p[0] = make_float4(v[0], v[1], v[2], v[3]);
+        p[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+    __builtin_amdgcn_wave_barrier();
+    ns_symmetric<Tile::UC, 64>(m.p + (size_t)b * m.kp * m.kp * 2, m.kp, r0, c0, i == j, mine, lane);
 }
 __global__ __launch_bounds__(NS_WIDE) void k_ns_poly(const NsMat* tab, int count, float cb, float cc) {
     extern __shared__ __align__(16) char lds[];
@@ -537,68 +647,109 @@ __global__ __launch_bounds__(NS_WIDE) void k_ns_poly(const NsMat* tab, int count
     else ns_poly<64>(m, cb, cc, lds);
 }
 
-__device__ __forceinline__ void ns_out(const NsMat& m, const NsUpdate& up, int b, int r, int c, float v) {
+// eight adjacent elements of an output row (those behind its end are not there)
+__device__ __forceinline__ void ns_out8(const NsMat& m, const NsUpdate& up, int b, int r, int c, const float* v) {
+    if (r >= m.rows || c >= m.cols) return;
     const size_t o = b * m.out_bs + (size_t)r * m.out_ld + c;
+    const bool whole = m.out_vec && c + 8 <= m.cols;
     if (up.on) {
         float* p = (float*)m.out + o;
-        *p = *p * up.decay - m.step * v;
+        if (whole) {
+            const float4 a = ld4(p), d = ld4(p + 4);
+            st4(p, make_float4(a.x * up.decay - m.step * v[0], a.y * up.decay - m.step * v[1], a.z * up.decay - m.step * v[2],
+                               a.w * up.decay - m.step * v[3]));
+            st4(p + 4, make_float4(d.x * up.decay - m.step * v[4], d.y * up.decay - m.step * v[5], d.z * up.decay - m.step * v[6],
+                                   d.w * up.decay - m.step * v[7]));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (c + e < m.cols) p[e] = p[e] * up.decay - m.step * v[e];
+        }
     } else if (m.type == 0) {
-        ((float*)m.out)[o] = v;
+        float* p = (float*)m.out + o;
+        if (whole) {
+            st4(p, make_float4(v[0], v[1], v[2], v[3]));
+            st4(p + 4, make_float4(v[4], v[5], v[6], v[7]));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (c + e < m.cols) p[e] = v[e];
+        }
     } else if (m.type == 1) {
-        st1((bf16_t*)m.out + o, v);
+        bf16_t* p = (bf16_t*)m.out + o;
+        if (whole) {
+            *(uint4*)p = make_uint4(agb_pack2_bf16(v[0], v[1]), agb_pack2_bf16(v[2], v[3]), agb_pack2_bf16(v[4], v[5]),
+                                    agb_pack2_bf16(v[6], v[7]));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (c + e < m.cols) st1(p + e, v[e]);
+        }
     } else {
-        ((half_t*)m.out)[o] = (half_t)v;
+        half_t* p = (half_t*)m.out + o;
+        half8 h;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = (half_t)v[e];
+        if (whole) {
+            *(half8*)p = h;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (c + e < m.cols) p[e] = h[e];
+        }
     }
 }
 
 // X <- a X + X P
 template <int T>
 __device__ __forceinline__ void ns_apply(const NsMat& m, int from, float ca, bool last, const NsUpdate& up, char* lds) {
-    constexpr int EACH = T * T / 8 / NS_WIDE, P = T + 2;
-    int at = blockIdx.x - m.at[NS_APPLY];
+    typedef NsTile<T, false> Tile;
+    int at = ns_order(blockIdx.x - m.at[NS_APPLY], m.nt * m.kt * m.batch);
     const int b = at / (m.nt * m.kt);
     at %= m.nt * m.kt;
-    const int n0 = at / m.kt * T, k0 = at % m.kt * T;
     const size_t plane = (size_t)b * m.np * m.kp * 2;
     const half_t* x = m.xt[from] + plane;
     half_t* out = m.xt[from ^ 1] + plane;
-    NsTile<T, false> t;
-    t.run(x, n0, m.np, m.p + (size_t)b * m.kp * m.kp * 2, k0, m.kp, m.kp, 0, m.kp, lds);
-    float* tile = (float*)lds;
+    Tile t;
+    t.run(m.p + (size_t)b * m.kp * m.kp * 2, at % m.kt * T, m.kp, x, at / m.kt * T, m.np, m.kp, 0, m.kp, lds);
+    const int lane = threadIdx.x & 63, n0 = at / m.kt * T + t.unit_row(), k0 = at % m.kt * T + t.unit_col();
+    constexpr int EACH = Tile::UC / 16;
     half8 xh[EACH], xl[EACH];
+    int row, col;
 #pragma unroll
     for (int l = 0; l < EACH; ++l) {
-        const int q = l * NS_WIDE + threadIdx.x, row = q / 4 % T, col = (q & 3) * 8 + q / (4 * T) * 32;
+        ns_group<Tile::UC>(l * 64 + lane, row, col);
         const size_t o = ns_at(min(n0 + row, m.np - 1), min(k0 + col, m.kp - 8), m.np);
         xh[l] = *(const half8*)(x + o);
         xl[l] = *(const half8*)(x + o + 32);
     }
-    t.stage(tile);
+    if (!t.merge(lds)) return;
+    float* mine = (float*)lds + t.unit() * 32 * (Tile::UC + 4);
+    t.stage(mine);
 #pragma unroll
     for (int l = 0; l < EACH; ++l) {
-        const int q = l * NS_WIDE + threadIdx.x, row = q / 4 % T, col = (q & 3) * 8 + q / (4 * T) * 32;
-        if (n0 + row >= m.np || k0 + col >= m.kp) continue;
+        ns_group<Tile::UC>(l * 64 + lane, row, col);
         float v[8];
+        ns_along<Tile::UC>(mine, row, col, v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float* p = tile + row * P + col + e;
-            v[e] = *p + ca * (((float)xh[l][e] + (float)xl[l][e]) * NS_UNSCALE);
-            if (last) *p = v[e];
-        }
+        for (int e = 0; e < 8; ++e) v[e] += ca * (((float)xh[l][e] + (float)xl[l][e]) * NS_UNSCALE);
         if (!last) {
-            half8 hi, lo;
-            ns_split8(v, hi, lo);
-            const size_t o = ns_at(n0 + row, k0 + col, m.np);
-            *(half8*)(out + o) = hi;
-            *(half8*)(out + o + 32) = lo;
+            if (n0 + row < m.np && k0 + col < m.kp) ns_write8(out, ns_at(n0 + row, k0 + col, m.np), v);
+        } else if (m.tall) {
+            ns_out8(m, up, b, n0 + row, k0 + col, v);
+        } else {
+            float4* p = (float4*)(mine + row * (Tile::UC + 4) + col);
+            p[0] = make_float4(v[0], v[1], v[2], v[3]);
+            p[1] = make_float4(v[4], v[5], v[6], v[7]);
         }
     }
-    if (!last) return;
-    __syncthreads();
-    for (int q = threadIdx.x; q < T * T; q += NS_WIDE) {      // (lanes along the output's rows)
-        const int i = q / T, j = q % T;
-        const int r = (m.tall ? n0 : k0) + i, c = (m.tall ? k0 : n0) + j;
-        if (r < m.rows && c < m.cols) ns_out(m, up, b, r, c, m.tall ? tile[i * P + j] : tile[j * P + i]);
+    if (!last || m.tall) return;
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int l = 0; l < EACH; ++l) {
+        float v[8];
+        ns_down<Tile::UC>(mine, l * 64 + lane, row, col, v);
+        ns_out8(m, up, b, k0 + col, n0 + row, v);
     }
 }
 __global__ __launch_bounds__(NS_WIDE) void k_ns_apply(const NsMat* tab, int count, int from, float ca, int last,
@@ -629,6 +780,8 @@ static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
     m.rows = (int)rows; m.cols = (int)cols; m.batch = (int)batch; m.type = (int)f[NS_TYPE];
     m.tall = rows >= cols;
     m.vec = m.in_ld == cols && m.in_bs % 4 == 0 && f[NS_IN] % 16 == 0 && f[NS_MOM] % 16 == 0;
+    const int esize = m.type == 0 ? 4 : 2;
+    m.out_vec = m.out_ld * esize % 16 == 0 && m.out_bs * esize % 16 == 0 && f[NS_OUT] % 16 == 0;
     m.k = m.tall ? m.cols : m.rows;
     m.n = m.tall ? m.rows : m.cols;
     if (m.k > 16384) return false;
@@ -666,10 +819,10 @@ static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
     m.p = (half_t*)take(g);
     m.part = (float*)take(m.splits > 1 ? (size_t)m.splits * tiles * m.tile * m.tile * 4 : 0);
     m.sq = (double*)take((size_t)m.sums * batch * 8);
-    const long long sub = (m.tile / 32) * (m.tile / 32);
+    const long long units = m.tile == 128 ? 8 : 4;
     const long long wgs[NS_LAUNCHES] = {(long long)m.sums * batch, (long long)(m.kp / 64) * (m.np / 64) * batch, tiles * m.splits,
                                         (long long)m.kt * m.nt * batch, (long long)m.tri_p * batch,
-                                        m.splits > 1 ? tiles * sub : 0};
+                                        m.splits > 1 ? tiles * units : 0};
     for (int i = 0; i < NS_LAUNCHES; ++i) {
         m.at[i] = plan.grid[i];
         if (plan.grid[i] + wgs[i] > 0x7fffffff) return false;
