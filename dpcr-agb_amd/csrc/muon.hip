@@ -24,6 +24,23 @@
 typedef _Float16 half_t;
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+// pointers that come out of a table: global memory, as the compiler cannot know (its accesses would go by way of the LDS counter)
+#define NS_GLOBAL __attribute__((address_space(1)))
+typedef NS_GLOBAL void gvoid;
+typedef NS_GLOBAL char gchar;
+typedef NS_GLOBAL half_t ghalf;
+typedef NS_GLOBAL half8 ghalf8;
+typedef NS_GLOBAL half4 ghalf4;
+typedef NS_GLOBAL float gfloat;
+typedef NS_GLOBAL f32x4 gfloat4;
+typedef NS_GLOBAL double gdouble;
+typedef NS_GLOBAL unsigned short gshort;
+typedef NS_GLOBAL u16x4 gshort4;
+typedef NS_GLOBAL u32x4 guint4;
 
 #define NS_THREADS 256
 #define NS_WIDE 512           // threads of a product's workgroup
@@ -33,9 +50,9 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 #define NS_MAX_STEPS 64
 
 struct __attribute__((aligned(16))) NsMat {
-    const void* in;
-    void* out;
-    float* mom;
+    const gvoid* in;
+    gvoid* out;
+    gfloat* mom;
     long long in_ld, in_bs, out_ld, out_bs;
     int rows, cols, batch, type;      // type of `in` (and of `out` where nothing is updated): 0 fp32, 1 bf16, 2 fp16
     int k, n, kp, np, tall;
@@ -44,11 +61,11 @@ struct __attribute__((aligned(16))) NsMat {
     int tile_p, kt_p, tri_p;                   // tile of P
     int sums;                                  // partial sums of squares per matrix
     float step;
-    half_t *xt[2], *g, *p;                     // planes of matrix 0 of the stack
-    float* part;
-    double* sq;
-    int at[6];      // first workgroup in the launches over: NS_CHUNKs, 64 x 64 blocks of X, G tiles x splits, X tiles, P tiles,
-                    // units of G tiles (fold)
+    ghalf *xt0, *xt1, *g, *p;                  // planes of matrix 0 of the stack
+    gfloat4* part;
+    gdouble* sq;
+    int at[7];      // first workgroup in the launches over: NS_CHUNKs, 64 x 64 blocks of X, G tiles x splits, X tiles, P tiles,
+                    // units of G tiles (fold), whole matrices
 };
 
 // ---- pairs of fp16
@@ -72,24 +89,34 @@ __device__ __forceinline__ size_t ns_at(int row, int col, int rows) {
 }
 
 // which matrix a workgroup belongs to: the last whose first workgroup is not behind it (64 candidates a look)
-enum { NS_SQUARES, NS_PLANES, NS_GRAM, NS_APPLY, NS_POLY, NS_FOLD, NS_LAUNCHES };
+enum { NS_SQUARES, NS_PLANES, NS_GRAM, NS_APPLY, NS_POLY, NS_FOLD, NS_RESIDENT, NS_LAUNCHES };
+// (The descriptor is copied whole, by scalar loads in one go.)
+typedef const __attribute__((address_space(4))) NsMat* NsTab;
 template <int WHICH>
-__device__ __forceinline__ const NsMat& ns_find(const NsMat* tab, int count) {
-    int found = -1;
-    for (int base = 0; base < count; base += 64) {
-        const int i = base + (threadIdx.x & 63);
-        found += __popcll(__ballot(i < count && tab[i].at[WHICH] <= (int)blockIdx.x));
+__device__ __forceinline__ NsMat ns_find(NsTab tab, int count) {
+    int found = 0;
+    if (count > 1) {
+        found = -1;
+        for (int base = 0; base < count; base += 64) {
+            const int i = base + (threadIdx.x & 63);
+            found += __popcll(__ballot(i < count && tab[min(i, count - 1)].at[WHICH] <= (int)blockIdx.x));
+        }
+        found = __builtin_amdgcn_readfirstlane(found);
     }
-    return tab[__builtin_amdgcn_readfirstlane(found)];
+    struct {
+        u32x4 v[sizeof(NsMat) / 16];
+    } raw;
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(NsMat) / 16; ++i) raw.v[i] = ((const __attribute__((address_space(4))) u32x4*)(tab + found))[i];
+    return __builtin_bit_cast(NsMat, raw);
 }
 
 // The table's way to the device: by value, in kernel arguments (a captured call keeps its own), copied by all lanes at once.
-#define NS_TABLE 16
+#define NS_TABLE 12
 struct NsTable {
     NsMat m[NS_TABLE];
 };
-static_assert(sizeof(NsTable) < 3900 && sizeof(NsMat) % 16 == 0, "kernel arguments hold 4 KB");
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+static_assert(sizeof(NsTable) < 3200 && sizeof(NsMat) % 16 == 0, "kernel arguments hold 4 KB");
 __global__ __launch_bounds__(256) void k_ns_table(const NsTable t, u32x4* tab, int pieces) {
     const auto* from = (const __attribute__((address_space(4))) u32x4*)__builtin_amdgcn_kernarg_segment_ptr();      // (t: the first)
     if ((int)threadIdx.x < pieces) tab[threadIdx.x] = from[threadIdx.x];
@@ -100,21 +127,20 @@ struct NsUpdate {
     int on, nesterov;
     float mu, omu, clip, decay;
 };
+__device__ __forceinline__ float ns_value(unsigned short v, int type) {      // (16 bits: bf16 or fp16)
+    return type == 1 ? __uint_as_float((unsigned)v << 16) : (float)__builtin_bit_cast(half_t, v);
+}
 __device__ __forceinline__ float ns_in(const NsMat& m, size_t off) {
-    if (m.type == 0) return ((const float*)m.in)[off];
-    if (m.type == 1) return ld1((const bf16_t*)m.in + off);
-    return (float)((const half_t*)m.in)[off];
+    return m.type == 0 ? ((const gfloat*)m.in)[off] : ns_value(((const gshort*)m.in)[off], m.type);
 }
 __device__ __forceinline__ void ns_in4(const NsMat& m, size_t off, float* v) {      // (aligned)
-    float4 q;
-    if (m.type == 0) q = ld4((const float*)m.in + off);
-    else if (m.type == 1) q = ld4((const bf16_t*)m.in + off);
-    else {
-        typedef _Float16 half4 __attribute__((ext_vector_type(4)));
-        const half4 h = *(const half4*)((const half_t*)m.in + off);
-        q = make_float4((float)h[0], (float)h[1], (float)h[2], (float)h[3]);
+    if (m.type == 0) {
+        const f32x4 q = *(const gfloat4*)((const gfloat*)m.in + off);
+        v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+    } else {
+        const u16x4 q = *(const gshort4*)((const gshort*)m.in + off);
+        v[0] = ns_value(q.x, m.type); v[1] = ns_value(q.y, m.type); v[2] = ns_value(q.z, m.type); v[3] = ns_value(q.w, m.type);
     }
-    v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
 }
 __device__ __forceinline__ float ns_clip(float g, float clip) {      // (NaN stays)
     if (clip > 0.f) g = g > clip ? clip : g < -clip ? -clip : g;
@@ -123,7 +149,7 @@ __device__ __forceinline__ float ns_clip(float g, float clip) {      // (NaN sta
 
 // sums of squares in 64 bits (neither huge nor tiny entries leave the range), and the momentum's update
 __global__ __launch_bounds__(NS_THREADS) void k_ns_squares(const NsMat* tab, int count, const NsUpdate up) {
-    const NsMat& m = ns_find<NS_SQUARES>(tab, count);
+    const NsMat m = ns_find<NS_SQUARES>((NsTab)tab, count);
     const int at = blockIdx.x - m.at[NS_SQUARES], b = at / m.sums, part = at % m.sums;
     const long long total = (long long)m.rows * m.cols, first = (long long)part * NS_CHUNK;
     const long long last = first + NS_CHUNK < total ? first + NS_CHUNK : total;
@@ -136,7 +162,7 @@ __global__ __launch_bounds__(NS_THREADS) void k_ns_squares(const NsMat* tab, int
         if (whole) {
             ns_in4(m, base + i0, v);
             if (up.on) {
-                const float4 q = *(const float4*)(m.mom + i0);
+                const f32x4 q = *(const gfloat4*)(m.mom + i0);
                 mom[0] = q.x; mom[1] = q.y; mom[2] = q.z; mom[3] = q.w;
             }
         } else {
@@ -157,7 +183,7 @@ __global__ __launch_bounds__(NS_THREADS) void k_ns_squares(const NsMat* tab, int
                 v[e] = up.nesterov ? v[e] * up.omu + mom[e] * up.mu : mom[e];
             }
             if (whole) {
-                *(float4*)(m.mom + i0) = make_float4(mom[0], mom[1], mom[2], mom[3]);
+                *(gfloat4*)(m.mom + i0) = f32x4{mom[0], mom[1], mom[2], mom[3]};
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
@@ -179,7 +205,7 @@ __global__ __launch_bounds__(NS_THREADS) void k_ns_squares(const NsMat* tab, int
 
 // X = M / (|M| + eps) as plane pairs, 64 x 64 of [n][k] at a time
 __global__ __launch_bounds__(NS_THREADS) void k_ns_planes(const NsMat* tab, int count, const NsUpdate up, double eps) {
-    const NsMat& m = ns_find<NS_PLANES>(tab, count);
+    const NsMat m = ns_find<NS_PLANES>((NsTab)tab, count);
     const int kb = m.kp / 64, nb = m.np / 64;
     int at = blockIdx.x - m.at[NS_PLANES];
     const int b = at / (kb * nb);
@@ -214,7 +240,7 @@ __global__ __launch_bounds__(NS_THREADS) void k_ns_planes(const NsMat* tab, int 
         else tile[j][i] = v;
     }
     __syncthreads();
-    half_t* xt = m.xt[0] + (size_t)b * m.np * m.kp * 2;
+    ghalf* xt = m.xt0 + (size_t)b * m.np * m.kp * 2;
     for (int q = threadIdx.x; q < 512; q += NS_THREADS) {
         const int row = q >> 2 & 63, col = (q & 3) * 8 + (q >> 8) * 32;
         float v[8];
@@ -223,8 +249,8 @@ __global__ __launch_bounds__(NS_THREADS) void k_ns_planes(const NsMat* tab, int 
         for (int e = 0; e < 8; ++e) v[e] = tile[row][col + e];
         ns_split8(v, hi, lo);
         const size_t o = ns_at(n0 + row, k0 + col, m.np);
-        *(half8*)(xt + o) = hi;
-        *(half8*)(xt + o + 32) = lo;
+        *(ghalf8*)(xt + o) = hi;
+        *(ghalf8*)(xt + o + 32) = lo;
     }
 }
 
@@ -250,7 +276,7 @@ __device__ __forceinline__ half8 ns_read_tr(const char* p, int second) {
 
 // 16 bytes a lane from `from` to LDS at `to` + 16 lane.  (Written out: the compiler would wait for every transfer in flight before
 // any LDS read.  Nothing is returned in registers; the waits are NsTile::run's.)
-__device__ __forceinline__ void ns_transfer(const char* from, unsigned to) {
+__device__ __forceinline__ void ns_transfer(const gchar* from, unsigned to) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory");
 }
 
@@ -262,7 +288,7 @@ struct NsTile {
     static constexpr int BUFFERS = 4;
     f32x16 acc[S][S];
 
-    __device__ __forceinline__ void run(const half_t* A, int a0, int a_rows, const half_t* B, int b0, int b_rows, int cols,
+    __device__ __forceinline__ void run(const ghalf* A, int a0, int a_rows, const ghalf* B, int b0, int b_rows, int cols,
                                         int c0, int c1, char* lds) {
         const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = all & 3, group = all >> 2;
         const int wr = (wave >> 1) * (T / 2), wc = (wave & 1) * (T / 2);
@@ -272,17 +298,17 @@ struct NsTile {
             for (int j = 0; j < S; ++j)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-        const char *pa[LOADS], *pb[LOADS];
+        const gchar *pa[LOADS], *pb[LOADS];
 #pragma unroll
         for (int l = 0; l < LOADS; ++l) {
             if constexpr (TR) {
                 const int row = (all * LOADS + l) * (256 / T) + lane / (T / 4), piece = lane % (T / 4) ^ (4 * (row & 3));
-                pa[l] = (const char*)A + ((size_t)min(a0 / 32 + (piece >> 3), cols / 32 - 1) * a_rows + c0 + row) * 128 + (piece & 7) * 16;
-                pb[l] = (const char*)B + ((size_t)min(b0 / 32 + (piece >> 3), cols / 32 - 1) * b_rows + c0 + row) * 128 + (piece & 7) * 16;
+                pa[l] = (const gchar*)A + ((size_t)min(a0 / 32 + (piece >> 3), cols / 32 - 1) * a_rows + c0 + row) * 128 + (piece & 7) * 16;
+                pb[l] = (const gchar*)B + ((size_t)min(b0 / 32 + (piece >> 3), cols / 32 - 1) * b_rows + c0 + row) * 128 + (piece & 7) * 16;
             } else {
                 const int row = (all * LOADS + l) * 8 + (lane >> 3), piece = (lane & 7) ^ ((row >> 1) & 7);
-                pa[l] = (const char*)A + ((size_t)(c0 / 32) * a_rows + min(a0 + row, a_rows - 1)) * 128 + piece * 16;
-                pb[l] = (const char*)B + ((size_t)(c0 / 32) * b_rows + min(b0 + row, b_rows - 1)) * 128 + piece * 16;
+                pa[l] = (const gchar*)A + ((size_t)(c0 / 32) * a_rows + min(a0 + row, a_rows - 1)) * 128 + piece * 16;
+                pb[l] = (const gchar*)B + ((size_t)(c0 / 32) * b_rows + min(b0 + row, b_rows - 1)) * 128 + piece * 16;
             }
         }
         // a step further: 32 rows, or the next block of 32 columns
@@ -496,15 +522,15 @@ __device__ __forceinline__ void ns_down(const float* unit, int q, int& row, int&
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = unit[(row + e) * (UC + 4) + col];
 }
-__device__ __forceinline__ void ns_write8(half_t* out, size_t o, const float* v) {
+__device__ __forceinline__ void ns_write8(ghalf* out, size_t o, const float* v) {
     half8 hi, lo;
     ns_split8(v, hi, lo);
-    *(half8*)(out + o) = hi;
-    *(half8*)(out + o + 32) = lo;
+    *(ghalf8*)(out + o) = hi;
+    *(ghalf8*)(out + o + 32) = lo;
 }
 // a unit at rows r0, columns c0 of a symmetric plane pair [kp][kp], and its mirror image unless it lies in a diagonal tile
 template <int UC, int THREADS>
-__device__ __forceinline__ void ns_symmetric(half_t* out, int kp, int r0, int c0, bool diagonal, const float* unit, int t) {
+__device__ __forceinline__ void ns_symmetric(ghalf* out, int kp, int r0, int c0, bool diagonal, const float* unit, int t) {
     float v[8];
     int row, col;
 #pragma unroll
@@ -544,7 +570,7 @@ __device__ __forceinline__ void ns_gram(const NsMat& m, int from, char* lds) {
     const int split = at / m.tri, l = at % m.tri;
     int i, j;
     ns_pair(l, m.kt, i, j);
-    const half_t* x = m.xt[from] + (size_t)b * m.np * m.kp * 2;
+    const ghalf* x = (from ? m.xt1 : m.xt0) + (size_t)b * m.np * m.kp * 2;
     const int c0 = split * m.chunk, c1 = min(m.np, c0 + m.chunk);
     Tile t;
     t.run(x, i * T, m.np, x, j * T, m.np, m.kp, c0, c1, lds);
@@ -555,16 +581,19 @@ __device__ __forceinline__ void ns_gram(const NsMat& m, int from, char* lds) {
         t.stage(mine);
         ns_symmetric<Tile::UC, 64>(m.g + (size_t)b * m.kp * m.kp * 2, m.kp, j * T + t.unit_row(), i * T + t.unit_col(), i == j, mine, lane);
     } else {      // [batch][split][tile][unit][quad][lane]
-        float4* out = (float4*)m.part + ((((size_t)b * m.splits + split) * m.tri + l) * Tile::UNITS + unit) * (Tile::S * 4 * 64) + lane;
+        gfloat4* out = m.part + ((((size_t)b * m.splits + split) * m.tri + l) * Tile::UNITS + unit) * (Tile::S * 4 * 64) + lane;
 #pragma unroll
         for (int i = 0; i < Tile::S; ++i)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) out[(i * 4 + q) * 64] = t.quad(i, q);
+            for (int q = 0; q < 4; ++q) {
+                const float4 v = t.quad(i, q);
+                out[(i * 4 + q) * 64] = f32x4{v.x, v.y, v.z, v.w};
+            }
     }
 }
 __global__ __launch_bounds__(NS_WIDE) void k_ns_gram(const NsMat* tab, int count, int from) {
     extern __shared__ __align__(16) char lds[];
-    const NsMat& m = ns_find<NS_GRAM>(tab, count);
+    const NsMat m = ns_find<NS_GRAM>((NsTab)tab, count);
     if (m.tile == 128) ns_gram<128>(m, from, lds);
     else ns_gram<64>(m, from, lds);
 }
@@ -582,11 +611,11 @@ __device__ __forceinline__ void ns_fold(const NsMat& m, float* unit) {
 #pragma unroll
     for (int s = 0; s < Tile::S; ++s) {
         const int quad = wave * Tile::S + s;      // (Tile::S * 4 of them by four waves)
-        const float4* in = (const float4*)m.part + (((size_t)b * m.splits * m.tri + l) * Tile::UNITS + u) * (Tile::S * 4 * 64) + quad * 64 + lane;
+        const gfloat4* in = m.part + (((size_t)b * m.splits * m.tri + l) * Tile::UNITS + u) * (Tile::S * 4 * 64) + quad * 64 + lane;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
         for (int p = 0; p < m.splits; ++p) {
-            const float4 v = in[p * next];
+            const f32x4 v = in[p * next];
             sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
         }
         ns_put_quad<Tile::UC>(unit, quad / 4, quad % 4, lane, sum);
@@ -596,7 +625,7 @@ __device__ __forceinline__ void ns_fold(const NsMat& m, float* unit) {
     ns_symmetric<Tile::UC, NS_THREADS>(m.g + (size_t)b * m.kp * m.kp * 2, m.kp, j * T + row, i * T + col, i == j, unit, threadIdx.x);
 }
 __global__ __launch_bounds__(NS_THREADS) void k_ns_fold(const NsMat* tab, int count) {
-    const NsMat& m = ns_find<NS_FOLD>(tab, count);
+    const NsMat m = ns_find<NS_FOLD>((NsTab)tab, count);
     __shared__ __align__(16) float unit[32 * 68];
     if (m.tile == 128) ns_fold<128>(m, unit);
     else ns_fold<64>(m, unit);
@@ -609,7 +638,7 @@ __device__ __forceinline__ void ns_poly(const NsMat& m, float cb, float cc, char
     const int at = ns_order(blockIdx.x - m.at[NS_POLY], m.tri_p * m.batch), b = at / m.tri_p;
     int i, j;
     ns_pair(at % m.tri_p, m.kt_p, i, j);
-    const half_t* g = m.g + (size_t)b * m.kp * m.kp * 2;
+    const ghalf* g = m.g + (size_t)b * m.kp * m.kp * 2;
     Tile t;
     t.run(g, i * T, m.kp, g, j * T, m.kp, m.kp, 0, m.kp, lds);
     if (!t.merge(lds)) return;
@@ -622,8 +651,8 @@ __device__ __forceinline__ void ns_poly(const NsMat& m, float cb, float cc, char
     for (int l = 0; l < EACH; ++l) {
         ns_group<Tile::UC>(l * 64 + lane, row, col);
         const size_t o = ns_at(min(r0 + row, m.kp - 1), min(c0 + col, m.kp - 8), m.kp);
-        gh[l] = *(const half8*)(g + o);
-        gl[l] = *(const half8*)(g + o + 32);
+        gh[l] = *(const ghalf8*)(g + o);
+        gl[l] = *(const ghalf8*)(g + o + 32);
     }
     t.stage(mine);
 #pragma unroll
@@ -642,60 +671,47 @@ __device__ __forceinline__ void ns_poly(const NsMat& m, float cb, float cc, char
 }
 __global__ __launch_bounds__(NS_WIDE) void k_ns_poly(const NsMat* tab, int count, float cb, float cc) {
     extern __shared__ __align__(16) char lds[];
-    const NsMat& m = ns_find<NS_POLY>(tab, count);
+    const NsMat m = ns_find<NS_POLY>((NsTab)tab, count);
     if (m.tile_p == 128) ns_poly<128>(m, cb, cc, lds);
     else ns_poly<64>(m, cb, cc, lds);
 }
 
+// two values as 16-bit ones
+__device__ __forceinline__ unsigned ns_pack(float a, float b, int type) {
+    if (type == 1) return agb_pack2_bf16(a, b);
+    return __builtin_bit_cast(unsigned short, (half_t)a) | (unsigned)__builtin_bit_cast(unsigned short, (half_t)b) << 16;
+}
 // eight adjacent elements of an output row (those behind its end are not there)
 __device__ __forceinline__ void ns_out8(const NsMat& m, const NsUpdate& up, int b, int r, int c, const float* v) {
     if (r >= m.rows || c >= m.cols) return;
     const size_t o = b * m.out_bs + (size_t)r * m.out_ld + c;
     const bool whole = m.out_vec && c + 8 <= m.cols;
-    if (up.on) {
-        float* p = (float*)m.out + o;
+    if (up.on || m.type == 0) {
+        gfloat* p = (gfloat*)m.out + o;
         if (whole) {
-            const float4 a = ld4(p), d = ld4(p + 4);
-            st4(p, make_float4(a.x * up.decay - m.step * v[0], a.y * up.decay - m.step * v[1], a.z * up.decay - m.step * v[2],
-                               a.w * up.decay - m.step * v[3]));
-            st4(p + 4, make_float4(d.x * up.decay - m.step * v[4], d.y * up.decay - m.step * v[5], d.z * up.decay - m.step * v[6],
-                                   d.w * up.decay - m.step * v[7]));
+            f32x4 a = {v[0], v[1], v[2], v[3]}, d = {v[4], v[5], v[6], v[7]};
+            if (up.on) {
+                a = *(gfloat4*)p * up.decay - m.step * a;
+                d = *(gfloat4*)(p + 4) * up.decay - m.step * d;
+            }
+            *(gfloat4*)p = a;
+            *(gfloat4*)(p + 4) = d;
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (c + e < m.cols) p[e] = p[e] * up.decay - m.step * v[e];
-        }
-    } else if (m.type == 0) {
-        float* p = (float*)m.out + o;
-        if (whole) {
-            st4(p, make_float4(v[0], v[1], v[2], v[3]));
-            st4(p + 4, make_float4(v[4], v[5], v[6], v[7]));
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (c + e < m.cols) p[e] = v[e];
-        }
-    } else if (m.type == 1) {
-        bf16_t* p = (bf16_t*)m.out + o;
-        if (whole) {
-            *(uint4*)p = make_uint4(agb_pack2_bf16(v[0], v[1]), agb_pack2_bf16(v[2], v[3]), agb_pack2_bf16(v[4], v[5]),
-                                    agb_pack2_bf16(v[6], v[7]));
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (c + e < m.cols) st1(p + e, v[e]);
+                if (c + e < m.cols) p[e] = up.on ? p[e] * up.decay - m.step * v[e] : v[e];
         }
     } else {
-        half_t* p = (half_t*)m.out + o;
-        half8 h;
+        gshort* p = (gshort*)m.out + o;
+        u32x4 w;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] = (half_t)v[e];
+        for (int e = 0; e < 4; ++e) w[e] = ns_pack(v[2 * e], v[2 * e + 1], m.type);
         if (whole) {
-            *(half8*)p = h;
+            *(guint4*)p = w;
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (c + e < m.cols) p[e] = h[e];
+                if (c + e < m.cols) p[e] = (unsigned short)(w[e / 2] >> 16 * (e & 1));
         }
     }
 }
@@ -708,8 +724,8 @@ __device__ __forceinline__ void ns_apply(const NsMat& m, int from, float ca, boo
     const int b = at / (m.nt * m.kt);
     at %= m.nt * m.kt;
     const size_t plane = (size_t)b * m.np * m.kp * 2;
-    const half_t* x = m.xt[from] + plane;
-    half_t* out = m.xt[from ^ 1] + plane;
+    const ghalf* x = (from ? m.xt1 : m.xt0) + plane;
+    ghalf* out = (from ? m.xt0 : m.xt1) + plane;
     Tile t;
     t.run(m.p + (size_t)b * m.kp * m.kp * 2, at % m.kt * T, m.kp, x, at / m.kt * T, m.np, m.kp, 0, m.kp, lds);
     const int lane = threadIdx.x & 63, n0 = at / m.kt * T + t.unit_row(), k0 = at % m.kt * T + t.unit_col();
@@ -720,8 +736,8 @@ __device__ __forceinline__ void ns_apply(const NsMat& m, int from, float ca, boo
     for (int l = 0; l < EACH; ++l) {
         ns_group<Tile::UC>(l * 64 + lane, row, col);
         const size_t o = ns_at(min(n0 + row, m.np - 1), min(k0 + col, m.kp - 8), m.np);
-        xh[l] = *(const half8*)(x + o);
-        xl[l] = *(const half8*)(x + o + 32);
+        xh[l] = *(const ghalf8*)(x + o);
+        xl[l] = *(const ghalf8*)(x + o + 32);
     }
     if (!t.merge(lds)) return;
     float* mine = (float*)lds + t.unit() * 32 * (Tile::UC + 4);
@@ -755,9 +771,320 @@ __device__ __forceinline__ void ns_apply(const NsMat& m, int from, float ca, boo
 __global__ __launch_bounds__(NS_WIDE) void k_ns_apply(const NsMat* tab, int count, int from, float ca, int last,
                                                       const NsUpdate up) {
     extern __shared__ __align__(16) char lds[];
-    const NsMat& m = ns_find<NS_APPLY>(tab, count);
+    const NsMat m = ns_find<NS_APPLY>((NsTab)tab, count);
     if (m.tile == 128) ns_apply<128>(m, from, ca, last, up, lds);
     else ns_apply<64>(m, from, ca, last, up, lds);
+}
+
+// ---- small matrices: everything in one workgroup, X, G and P in LDS (two launches fewer than one iteration above takes)
+// kp = 64 with np <= 256, or kp = np = 128.  Products as above, by 32 x 32 blocks of the result spread over eight waves (G and P
+// of kp = 64: four blocks, each by two waves with half of the sum), here with lo lo as well: nothing is bound by the matrix pipe.
+// LDS: X [block of 32 columns][n][128 bytes], then G / P [block][k][128 bytes], piece q of row r at place q ^ (r / 2 % 8), then
+// 16 KB of half sums.
+#define NS_RES_ROWS 256
+#define NS_RES_GROUPS 4      // groups of eight elements of a thread: 256 * 64 / 8 / 512
+#define NS_RES_BLOCKS 2      // 32 x 32 blocks of X of a wave: 256 / 32 * 2 / 8
+struct NsCoef {
+    float v[3 * NS_MAX_STEPS];
+};
+
+__device__ __forceinline__ int ns_place(int rows, int row, int piece, int blk) {
+    return (blk * rows + row) * 128 + ((piece ^ ((row >> 1) & 7)) << 4);
+}
+__device__ __forceinline__ void ns_mfma4(f32x16& acc, half8 ah, half8 al, half8 bh, half8 bl) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bl, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, acc, 0, 0, 0);
+}
+// rows of A (block ia) times rows of B (block ib) over STEPS steps of 16 columns from step s0 (even)
+template <int STEPS>
+__device__ __forceinline__ void ns_rows(f32x16& acc, const char* A, int a_rows, int ia, const char* B, int b_rows, int ib, int s0) {
+    const int lane = threadIdx.x & 63, ra = ia * 32 + (lane & 31), rb = ib * 32 + (lane & 31);
+    const int xa = (ra >> 1 & 7) << 4, xb = (rb >> 1 & 7) << 4, first = (lane >> 5) << 4;
+    A += (s0 >> 1) * a_rows * 128 + ra * 128;
+    B += (s0 >> 1) * b_rows * 128 + rb * 128;
+#pragma unroll 2
+    for (int s = 0; s < STEPS; ++s) {
+        const int piece = first + (s & 1) * 32;
+        const char *pa = A + (s >> 1) * a_rows * 128, *pb = B + (s >> 1) * b_rows * 128;
+        ns_mfma4(acc, *(const half8*)(pa + (piece ^ xa)), *(const half8*)(pa + (piece ^ xa ^ 64)), *(const half8*)(pb + (piece ^ xb)),
+                 *(const half8*)(pb + (piece ^ xb ^ 64)));
+    }
+}
+// columns ia and ib (blocks of 32) of X over 16-row steps [s0, s1), an even number of them
+__device__ __forceinline__ void ns_columns(f32x16& acc, const char* X, int rows, int ia, int ib, int s0, int s1) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, q = (lane & 15) >> 2, p = lane & 3, chunk = 2 * (g & 1) + (p >> 1);
+    const int r0 = 8 * (g >> 1) + q, r1 = r0 + 4;
+    const int first = ns_place(0, r0, chunk, 0) + (p & 1) * 8, second = ns_place(0, r1, chunk, 0) + (p & 1) * 8;
+    for (int s = s0; s < s1; s += 2) {
+        const char *A = X + (ia * rows + s * 16) * 128, *B = X + (ib * rows + s * 16) * 128;
+        auto read = [&](const char* base, int flip) {
+            const s16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(base + (first ^ flip)));
+            const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(base + (second ^ flip)));
+            return __builtin_bit_cast(half8, __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+        ns_mfma4(acc, read(A, 0), read(A, 64), read(B, 0), read(B, 64));
+        A += 16 * 128;
+        B += 16 * 128;
+        ns_mfma4(acc, read(A, 0), read(A, 64), read(B, 0), read(B, 64));
+    }
+}
+// quad q of a block: columns ia * 32 + 8 q + 4 (lane / 32) .. + 3 of row ib * 32 + lane % 32, as hi and lo of [block][rows] planes
+__device__ __forceinline__ char* ns_quad_at(char* planes, int rows, int ia, int ib, int q) {
+    const int lane = threadIdx.x & 63;
+    return planes + ns_place(rows, ib * 32 + (lane & 31), q, ia) + (lane >> 5) * 8;
+}
+__device__ __forceinline__ char* ns_lo(char* base, char* at) { return base + ((at - base) ^ 64); }
+__device__ __forceinline__ void ns_quad_put(char* planes, int rows, int ia, int ib, int q, const float* v) {
+    char* at = ns_quad_at(planes, rows, ia, ib, q);
+    half4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        half_t h, l;
+        ns_split(v[e], h, l);
+        hi[e] = h;
+        lo[e] = l;
+    }
+    *(half4*)at = hi;
+    *(half4*)ns_lo(planes, at) = lo;
+}
+__device__ __forceinline__ void ns_quad_get(char* planes, int rows, int ia, int ib, int q, float* v) {
+    char* at = ns_quad_at(planes, rows, ia, ib, q);
+    const half4 hi = *(const half4*)at, lo = *(const half4*)ns_lo(planes, at);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = ((float)hi[e] + (float)lo[e]) * NS_UNSCALE;
+}
+__device__ __forceinline__ void ns_zero(f32x16& a) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) a[e] = 0.f;
+}
+
+template <int KP>
+__device__ __forceinline__ void ns_resident(const NsMat& m, int b, const NsUpdate& up, double eps, const float* abc, int steps,
+                                            char* X, double* red) {
+    constexpr int KB = KP / 32, GROUPS8 = KP / 8, MINE = KP == 64 ? 1 : 2;      // MINE: blocks of G of a wave
+    const int np = m.np, t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    char* G = X + np * KP * 4;
+    float4* box = (float4*)(G + KP * KP * 4) + (wave & 3) * 256 + lane;
+    // M, its momentum's update, its norm: a wave takes 64 rows n of eight columns k.  (Loads without branches, from the last row
+    // or column where there is none: all in flight together.)
+    float u[NS_RES_GROUPS][8];
+    const int groups = np / 64 * GROUPS8;      // of a matrix; this wave's: wave, wave + 8, ...
+    auto first_of = [&](int group, long long ld) { return min(group / GROUPS8 * 64 + lane, m.n - 1) * (m.tall ? ld : 1); };
+    auto column_of = [&](int group, int e, long long ld) { return min(group % GROUPS8 * 8 + e, m.k - 1) * (m.tall ? 1 : ld); };
+    if (m.type == 0) {
+        const gfloat* in = (const gfloat*)m.in + b * m.in_bs;
+#pragma unroll
+        for (int l = 0; l < NS_RES_GROUPS; ++l)
+            if (l * 8 + wave < groups) {
+                const gfloat* p = in + first_of(l * 8 + wave, m.in_ld);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) u[l][e] = p[column_of(l * 8 + wave, e, m.in_ld)];
+            }
+    } else {
+        const gshort* in = (const gshort*)m.in + b * m.in_bs;
+        unsigned short raw[NS_RES_GROUPS][8];
+#pragma unroll
+        for (int l = 0; l < NS_RES_GROUPS; ++l)
+            if (l * 8 + wave < groups) {
+                const gshort* p = in + first_of(l * 8 + wave, m.in_ld);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) raw[l][e] = p[column_of(l * 8 + wave, e, m.in_ld)];
+            }
+#pragma unroll
+        for (int l = 0; l < NS_RES_GROUPS; ++l)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                u[l][e] = ns_value(raw[l][e], m.type);
+    }
+    double s = 0;
+#pragma unroll
+    for (int l = 0; l < NS_RES_GROUPS; ++l) {
+        const int group = l * 8 + wave, n = group / GROUPS8 * 64 + lane, k = group % GROUPS8 * 8;
+        if (group >= groups) continue;
+        float mom[8];
+        gfloat* pm = m.mom + first_of(group, m.cols);
+        if (up.on) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mom[e] = pm[column_of(group, e, m.cols)];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bool there = n < m.n && k + e < m.k;
+            float v = u[l][e];
+            if (up.on) {
+                v = ns_clip(v, up.clip);
+                mom[e] = mom[e] * up.mu + v * up.omu;
+                if (there) pm[column_of(group, e, m.cols)] = mom[e];
+                v = up.nesterov ? v * up.omu + mom[e] * up.mu : mom[e];
+            }
+            u[l][e] = there ? v : 0.f;
+            s += (double)u[l][e] * u[l][e];
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if (lane == 0) red[wave] = s;
+    __syncthreads();
+    s = ((red[0] + red[1]) + (red[2] + red[3])) + ((red[4] + red[5]) + (red[6] + red[7]));
+    const double norm = sqrt(s) + eps;
+#pragma unroll
+    for (int l = 0; l < NS_RES_GROUPS; ++l) {
+        const int group = l * 8 + wave;
+        if (group >= groups) continue;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u[l][e] = (float)(u[l][e] / norm);
+        half8 hi, lo;
+        ns_split8(u[l], hi, lo);
+        const int at = ns_place(np, group / GROUPS8 * 64 + lane, group % GROUPS8 & 3, group % GROUPS8 >> 2);
+        *(half8*)(X + at) = hi;
+        *(half8*)(X + (at ^ 64)) = lo;
+    }
+    __syncthreads();
+    const int half = KP == 64 ? wave >> 2 : 0;
+    auto block = [&](int l, int& ia, int& ib) {
+        ia = KP == 64 ? wave >> 1 & 1 : wave >> 1;
+        ib = KP == 64 ? wave & 1 : (wave & 1) * 2 + l;
+    };
+    // the two half sums of a block of kp = 64 (second half first into its box); ends with everybody's products done
+    auto join = [&](f32x16& acc) {
+        if (KP == 64 && half) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) box[q * 64] = make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
+        }
+        __syncthreads();
+        if (KP == 64 && !half) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float4 v = box[q * 64];
+                acc[4 * q] += v.x;
+                acc[4 * q + 1] += v.y;
+                acc[4 * q + 2] += v.z;
+                acc[4 * q + 3] += v.w;
+            }
+        }
+    };
+    const float unscale = NS_UNSCALE * NS_UNSCALE;
+    f32x16 x[NS_RES_BLOCKS];
+    for (int step = 0; step < steps; ++step) {
+        const float ca = abc[3 * step], cb = abc[3 * step + 1], cc = abc[3 * step + 2];
+        f32x16 acc[MINE];
+        // G = X^T X
+#pragma unroll
+        for (int l = 0; l < MINE; ++l) {
+            int ia, ib;
+            block(l, ia, ib);
+            ns_zero(acc[l]);
+            if (KP == 64) ns_columns(acc[l], X, np, ia, ib, half * (np / 32), (half + 1) * (np / 32));
+            else ns_columns(acc[l], X, np, ia, ib, 0, np / 16);
+        }
+        join(acc[0]);
+        if (!half) {
+#pragma unroll
+            for (int l = 0; l < MINE; ++l) {
+                int ia, ib;
+                block(l, ia, ib);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float v[4] = {acc[l][4 * q] * unscale, acc[l][4 * q + 1] * unscale, acc[l][4 * q + 2] * unscale,
+                                        acc[l][4 * q + 3] * unscale};
+                    ns_quad_put(G, KP, ia, ib, q, v);
+                }
+            }
+        }
+        __syncthreads();
+        // P = b G + c G G, in G's place
+#pragma unroll
+        for (int l = 0; l < MINE; ++l) {
+            int ia, ib;
+            block(l, ia, ib);
+            ns_zero(acc[l]);
+            ns_rows<KP == 64 ? 2 : 8>(acc[l], G, KP, ia, G, KP, ib, half * 2);
+        }
+        join(acc[0]);
+        if (!half) {
+#pragma unroll
+            for (int l = 0; l < MINE; ++l) {
+                int ia, ib;
+                block(l, ia, ib);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    float v[4];
+                    ns_quad_get(G, KP, ia, ib, q, v);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = cb * v[e] + cc * (acc[l][4 * q + e] * unscale);
+                    ns_quad_put(G, KP, ia, ib, q, v);
+                }
+            }
+        }
+        __syncthreads();
+        // X <- a X + X P: every product first, then every block in its place
+#pragma unroll
+        for (int l = 0; l < NS_RES_BLOCKS; ++l) {
+            const int unit = l * 8 + wave;
+            if (unit < np / 32 * KB) {
+                ns_zero(x[l]);
+                ns_rows<KP / 16>(x[l], G, KP, unit % KB, X, np, unit / KB, 0);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int l = 0; l < NS_RES_BLOCKS; ++l) {
+            const int unit = l * 8 + wave;
+            if (unit < np / 32 * KB) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    float v[4];
+                    ns_quad_get(X, np, unit % KB, unit / KB, q, v);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[l][4 * q + e] = v[e] = x[l][4 * q + e] * unscale + ca * v[e];
+                    ns_quad_put(X, np, unit % KB, unit / KB, q, v);
+                }
+            }
+        }
+        __syncthreads();
+    }
+    // out of the registers of the last step: row n, columns k of a lane's quads
+    const long long row = m.tall ? m.out_ld : 1, col = m.tall ? 1 : m.out_ld;
+#pragma unroll
+    for (int l = 0; l < NS_RES_BLOCKS; ++l) {
+        const int unit = l * 8 + wave, n = unit / KB * 32 + (lane & 31), k0 = unit % KB * 32 + 4 * (lane >> 5);
+        if (unit >= np / 32 * KB) continue;
+        const long long base = b * m.out_bs + min(n, m.n - 1) * row;
+        if (up.on || m.type == 0) {
+            gfloat* p = (gfloat*)m.out + base;
+            float old[16];
+            if (up.on) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) old[i] = p[min(k0 + (i >> 2) * 8 + (i & 3), m.k - 1) * col];
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int k = k0 + (i >> 2) * 8 + (i & 3);
+                if (n < m.n && k < m.k) p[k * col] = up.on ? old[i] * up.decay - m.step * x[l][i] : x[l][i];
+            }
+        } else {
+            gshort* p = (gshort*)m.out + base;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int k = k0 + (i >> 2) * 8 + (i & 3);
+                if (n < m.n && k < m.k) p[k * col] = (unsigned short)ns_pack(x[l][i], x[l][i], m.type);
+            }
+        }
+    }
+}
+__global__ __launch_bounds__(NS_WIDE) void k_ns_resident(const NsTable args, const NsMat* tab, int count, const NsUpdate up, double eps,
+                                                         const NsCoef coef, int steps) {
+    extern __shared__ __align__(16) char lds[];
+    __shared__ double red[8];
+    __shared__ float abc[3 * NS_MAX_STEPS];
+    // (a list that fits travels in the arguments alone; those are far away: everything is read at once, at the start)
+    const NsMat m = ns_find<NS_RESIDENT>(tab ? (NsTab)tab : (NsTab)__builtin_amdgcn_kernarg_segment_ptr(), count);
+    if ((int)threadIdx.x < 3 * steps) abc[threadIdx.x] = coef.v[threadIdx.x];
+    const int b = blockIdx.x - m.at[NS_RESIDENT];
+    if (m.kp == 64) ns_resident<64>(m, b, up, eps, abc, steps, lds, red);
+    else ns_resident<128>(m, b, up, eps, abc, steps, lds, red);
 }
 
 // ---- host side
@@ -769,13 +1096,14 @@ struct NsPlan {
     size_t bytes;
     int grid[NS_LAUNCHES];
     bool wide, wide_p;      // a tile of 128 among those of G and X; of P
+    int lds;                // bytes of the largest matrix that is taken whole
 };
 
 // One matrix stack's part of the workspace and of the launches.  false: a size that is not taken.
 static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
     const long long rows = f[NS_ROWS], cols = f[NS_COLS], batch = f[NS_BATCH];
     if (rows < 1 || cols < 1 || batch < 1 || rows > NS_MAX_SIDE || cols > NS_MAX_SIDE || batch > (1 << 20)) return false;
-    m.in = (const void*)f[NS_IN]; m.out = (void*)f[NS_OUT]; m.mom = (float*)f[NS_MOM];
+    m.in = (const gvoid*)f[NS_IN]; m.out = (gvoid*)f[NS_OUT]; m.mom = (gfloat*)f[NS_MOM];
     m.in_ld = f[NS_IN_LD]; m.in_bs = f[NS_IN_BS]; m.out_ld = f[NS_OUT_LD]; m.out_bs = f[NS_OUT_BS];
     m.rows = (int)rows; m.cols = (int)cols; m.batch = (int)batch; m.type = (int)f[NS_TYPE];
     m.tall = rows >= cols;
@@ -804,29 +1132,37 @@ static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
     m.tile_p = (long long)k64 * (k64 + 1) / 2 * m.batch <= 512 ? 64 : 128;
     m.kt_p = agb_cdiv(m.kp, m.tile_p);
     m.tri_p = m.kt_p * (m.kt_p + 1) / 2;
-    plan.wide |= m.tile == 128;
-    plan.wide_p |= m.tile_p == 128;
     m.sums = agb_cdiv((long long)rows * cols, NS_CHUNK);
-    const size_t x = (size_t)m.np * m.kp * 4 * batch, g = (size_t)m.kp * m.kp * 4 * batch;
+    // (measured, 64 x 64: 21 us whole, 111 us in tiles; the limits: LDS, and what a thread holds of X)
+    const bool whole = (m.kp == 64 && m.np <= NS_RES_ROWS) || (m.kp == 128 && m.np == 128);
+    if (whole) {
+        const int lds = m.np * m.kp * 4 + m.kp * m.kp * 4 + (m.kp == 64 ? 16384 : 0);
+        if (lds > plan.lds) plan.lds = lds;
+    } else {
+        plan.wide |= m.tile == 128;
+        plan.wide_p |= m.tile_p == 128;
+    }
+    const size_t x = whole ? 0 : (size_t)m.np * m.kp * 4 * batch, g = whole ? 0 : (size_t)m.kp * m.kp * 4 * batch;
     auto take = [&](size_t n) {
         char* p = ws ? ws + plan.bytes : nullptr;
         plan.bytes += (n + 255) / 256 * 256;
         return p;
     };
-    m.xt[0] = (half_t*)take(x);
-    m.xt[1] = (half_t*)take(x);
-    m.g = (half_t*)take(g);
-    m.p = (half_t*)take(g);
-    m.part = (float*)take(m.splits > 1 ? (size_t)m.splits * tiles * m.tile * m.tile * 4 : 0);
-    m.sq = (double*)take((size_t)m.sums * batch * 8);
+    m.xt0 = (ghalf*)take(x);
+    m.xt1 = (ghalf*)take(x);
+    m.g = (ghalf*)take(g);
+    m.p = (ghalf*)take(g);
+    m.part = (gfloat4*)take(m.splits > 1 && !whole ? (size_t)m.splits * tiles * m.tile * m.tile * 4 : 0);
+    m.sq = (gdouble*)take(whole ? 0 : (size_t)m.sums * batch * 8);
     const long long units = m.tile == 128 ? 8 : 4;
     const long long wgs[NS_LAUNCHES] = {(long long)m.sums * batch, (long long)(m.kp / 64) * (m.np / 64) * batch, tiles * m.splits,
                                         (long long)m.kt * m.nt * batch, (long long)m.tri_p * batch,
-                                        m.splits > 1 ? tiles * units : 0};
+                                        m.splits > 1 ? tiles * units : 0, batch};
     for (int i = 0; i < NS_LAUNCHES; ++i) {
         m.at[i] = plan.grid[i];
-        if (plan.grid[i] + wgs[i] > 0x7fffffff) return false;
-        plan.grid[i] += (int)wgs[i];
+        const long long more = whole == (i == NS_RESIDENT) ? wgs[i] : 0;
+        if (plan.grid[i] + more > 0x7fffffff) return false;
+        plan.grid[i] += (int)more;
     }
     return true;
 }
@@ -885,15 +1221,25 @@ static int ns_run(const char* name, const long long* fields, int count, int step
             ns_plan(fields + (size_t)(base + i) * NS_FIELDS, m[i], (char*)workspace, plan);
             m[i].step = step ? step[base + i] : 0.f;
         }
-        hipLaunchKernelGGL(k_ns_table, dim3(1), dim3(256), 0, st, t, (u32x4*)(tab + base), (int)(some * sizeof(NsMat) / 16));
+        if (count <= NS_TABLE && !plan.grid[NS_SQUARES]) tab = nullptr;      // (every matrix is taken whole: no table)
+        else hipLaunchKernelGGL(k_ns_table, dim3(1), dim3(256), 0, st, t, (u32x4*)(tab + base), (int)(some * sizeof(NsMat) / 16));
+    }
+    const int* grid = plan.grid;
+    if (grid[NS_RESIDENT]) {
+        const hipError_t e = hipFuncSetAttribute((const void*)k_ns_resident, hipFuncAttributeMaxDynamicSharedMemorySize, plan.lds);
+        if (e != hipSuccess) { agb_set_error("%s: %s", name, hipGetErrorString(e)); return AGB_ELAUNCH; }
+        NsCoef all = {};
+        for (int i = 0; i < 3 * steps; ++i) all.v[i] = coef[i];
+        if (tab) t = {};
+        hipLaunchKernelGGL(k_ns_resident, dim3(grid[NS_RESIDENT]), dim3(NS_WIDE), plan.lds, st, t, tab, count, up, eps, all, steps);
         AGB_CHECK_LAUNCH(name);
     }
+    if (!grid[NS_SQUARES]) return AGB_OK;
     for (const void* k : {(const void*)k_ns_gram, (const void*)k_ns_poly, (const void*)k_ns_apply}) {
         const hipError_t e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, NS_LDS(128));
         if (e != hipSuccess) { agb_set_error("%s: %s", name, hipGetErrorString(e)); return AGB_ELAUNCH; }
     }
     const int lds = plan.wide ? NS_LDS(128) : NS_LDS(64), lds_p = plan.wide_p ? NS_LDS(128) : NS_LDS(64);
-    const int* grid = plan.grid;
     hipLaunchKernelGGL(k_ns_squares, dim3(grid[NS_SQUARES]), dim3(NS_THREADS), 0, st, tab, count, up);
     hipLaunchKernelGGL(k_ns_planes, dim3(grid[NS_PLANES]), dim3(NS_THREADS), 0, st, tab, count, up, eps);
     for (int i = 0; i < steps; ++i) {
