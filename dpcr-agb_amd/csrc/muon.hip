@@ -776,14 +776,14 @@ __global__ __launch_bounds__(NS_WIDE) void k_ns_apply(const NsMat* tab, int coun
     else ns_apply<64>(m, from, ca, last, up, lds);
 }
 
-// ---- small matrices: everything in one workgroup, X, G and P in LDS (two launches fewer than one iteration above takes)
-// kp = 64 with np <= 256, or kp = np = 128.  Products as above, by 32 x 32 blocks of the result spread over eight waves (G and P
-// of kp = 64: four blocks, each by two waves with half of the sum), here with lo lo as well: nothing is bound by the matrix pipe.
-// LDS: X [block of 32 columns][n][128 bytes], then G / P [block][k][128 bytes], piece q of row r at place q ^ (r / 2 % 8), then
-// 16 KB of half sums.
+// ---- small matrices: everything in one workgroup, X, G and P in LDS (one launch instead of 17)
+// kp = 64 with np <= 256, or kp = np = 128.  Products by 16 x 16 blocks of the result spread over eight waves: what an iteration
+// takes is latency — the products' chains, the splitting of what they leave, five meetings — and small blocks shorten each.
+// kp = 64 adds lo lo: its short sums round so little that the dropped term would show.
+// LDS: X [block of 32 columns][n][128 bytes], then G / P [block][k][128 bytes], piece q of row r at place q ^ (r / 2 % 8).
 #define NS_RES_ROWS 256
 #define NS_RES_GROUPS 4      // groups of eight elements of a thread: 256 * 64 / 8 / 512
-#define NS_RES_BLOCKS 2      // 32 x 32 blocks of X of a wave: 256 / 32 * 2 / 8
+#define NS_RES_UNITS 4       // pairs of 16 x 16 blocks of X of a wave: 256 / 16 * 2 / 8
 struct NsCoef {
     float v[3 * NS_MAX_STEPS];
 };
@@ -791,53 +791,40 @@ struct NsCoef {
 __device__ __forceinline__ int ns_place(int rows, int row, int piece, int blk) {
     return (blk * rows + row) * 128 + ((piece ^ ((row >> 1) & 7)) << 4);
 }
-__device__ __forceinline__ void ns_mfma4(f32x16& acc, half8 ah, half8 al, half8 bh, half8 bl) {
-    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bl, acc, 0, 0, 0);
-    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, acc, 0, 0, 0);
-    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, acc, 0, 0, 0);
-    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, acc, 0, 0, 0);
+// operand of a 16 x 16 x 32 product: rows block * 16 .. + 15 of planes, columns of block `s` of 32
+__device__ __forceinline__ void ns_row16(const char* planes, int rows, int block, int s, half8& hi, half8& lo) {
+    const int lane = threadIdx.x & 63, at = ns_place(rows, block * 16 + (lane & 15), lane >> 4, s);
+    hi = *(const half8*)(planes + at);
+    lo = *(const half8*)(planes + (at ^ 64));
 }
-// rows of A (block ia) times rows of B (block ib) over STEPS steps of 16 columns from step s0 (even)
-template <int STEPS>
-__device__ __forceinline__ void ns_rows(f32x16& acc, const char* A, int a_rows, int ia, const char* B, int b_rows, int ib, int s0) {
-    const int lane = threadIdx.x & 63, ra = ia * 32 + (lane & 31), rb = ib * 32 + (lane & 31);
-    const int xa = (ra >> 1 & 7) << 4, xb = (rb >> 1 & 7) << 4, first = (lane >> 5) << 4;
-    A += (s0 >> 1) * a_rows * 128 + ra * 128;
-    B += (s0 >> 1) * b_rows * 128 + rb * 128;
-#pragma unroll 2
-    for (int s = 0; s < STEPS; ++s) {
-        const int piece = first + (s & 1) * 32;
-        const char *pa = A + (s >> 1) * a_rows * 128, *pb = B + (s >> 1) * b_rows * 128;
-        ns_mfma4(acc, *(const half8*)(pa + (piece ^ xa)), *(const half8*)(pa + (piece ^ xa ^ 64)), *(const half8*)(pb + (piece ^ xb)),
-                 *(const half8*)(pb + (piece ^ xb ^ 64)));
-    }
+// ... columns block * 16 .. + 15, rows s * 32 .. + 31
+__device__ __forceinline__ void ns_column16(const char* planes, int rows, int block, int s, half8& hi, half8& lo) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, q = (lane & 15) >> 2, p = lane & 3, chunk = 2 * (block & 1) + (p >> 1);
+    const int first = ns_place(rows, s * 32 + 8 * g + q, chunk, block >> 1) + (p & 1) * 8;
+    const int second = ns_place(rows, s * 32 + 8 * g + q + 4, chunk, block >> 1) + (p & 1) * 8;
+    auto read = [&](int flip) {
+        const s16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(planes + (first ^ flip)));
+        const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(planes + (second ^ flip)));
+        return __builtin_bit_cast(half8, __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    hi = read(0);
+    lo = read(64);
 }
-// columns ia and ib (blocks of 32) of X over 16-row steps [s0, s1), an even number of them
-__device__ __forceinline__ void ns_columns(f32x16& acc, const char* X, int rows, int ia, int ib, int s0, int s1) {
-    const int lane = threadIdx.x & 63, g = lane >> 4, q = (lane & 15) >> 2, p = lane & 3, chunk = 2 * (g & 1) + (p >> 1);
-    const int r0 = 8 * (g >> 1) + q, r1 = r0 + 4;
-    const int first = ns_place(0, r0, chunk, 0) + (p & 1) * 8, second = ns_place(0, r1, chunk, 0) + (p & 1) * 8;
-    for (int s = s0; s < s1; s += 2) {
-        const char *A = X + (ia * rows + s * 16) * 128, *B = X + (ib * rows + s * 16) * 128;
-        auto read = [&](const char* base, int flip) {
-            const s16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(base + (first ^ flip)));
-            const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(base + (second ^ flip)));
-            return __builtin_bit_cast(half8, __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7));
-        };
-        ns_mfma4(acc, read(A, 0), read(A, 64), read(B, 0), read(B, 64));
-        A += 16 * 128;
-        B += 16 * 128;
-        ns_mfma4(acc, read(A, 0), read(A, 64), read(B, 0), read(B, 64));
-    }
+// LOLO: the fourth product too
+template <bool LOLO>
+__device__ __forceinline__ void ns_mfma(f32x4& acc, half8 ah, half8 al, half8 bh, half8 bl) {
+    if constexpr (LOLO) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, bl, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, bh, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bl, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bh, acc, 0, 0, 0);
 }
-// quad q of a block: columns ia * 32 + 8 q + 4 (lane / 32) .. + 3 of row ib * 32 + lane % 32, as hi and lo of [block][rows] planes
-__device__ __forceinline__ char* ns_quad_at(char* planes, int rows, int ia, int ib, int q) {
+// A lane's four sums of a 16 x 16 product: columns ia * 16 + 4 (lane / 16) .. + 3 of row ib * 16 + lane % 16
+__device__ __forceinline__ int ns_quad_at(int rows, int ia, int ib) {
     const int lane = threadIdx.x & 63;
-    return planes + ns_place(rows, ib * 32 + (lane & 31), q, ia) + (lane >> 5) * 8;
+    return ns_place(rows, ib * 16 + (lane & 15), 2 * (ia & 1) + (lane >> 5), ia >> 1) + (lane >> 4 & 1) * 8;
 }
-__device__ __forceinline__ char* ns_lo(char* base, char* at) { return base + ((at - base) ^ 64); }
-__device__ __forceinline__ void ns_quad_put(char* planes, int rows, int ia, int ib, int q, const float* v) {
-    char* at = ns_quad_at(planes, rows, ia, ib, q);
+__device__ __forceinline__ void ns_quad_put(char* planes, int rows, int ia, int ib, const float* v) {
+    const int at = ns_quad_at(rows, ia, ib);
     half4 hi, lo;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -846,27 +833,24 @@ __device__ __forceinline__ void ns_quad_put(char* planes, int rows, int ia, int 
         hi[e] = h;
         lo[e] = l;
     }
-    *(half4*)at = hi;
-    *(half4*)ns_lo(planes, at) = lo;
+    *(half4*)(planes + at) = hi;
+    *(half4*)(planes + (at ^ 64)) = lo;
 }
-__device__ __forceinline__ void ns_quad_get(char* planes, int rows, int ia, int ib, int q, float* v) {
-    char* at = ns_quad_at(planes, rows, ia, ib, q);
-    const half4 hi = *(const half4*)at, lo = *(const half4*)ns_lo(planes, at);
+__device__ __forceinline__ void ns_quad_get(const char* planes, int rows, int ia, int ib, float* v) {
+    const int at = ns_quad_at(rows, ia, ib);
+    const half4 hi = *(const half4*)(planes + at), lo = *(const half4*)(planes + (at ^ 64));
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = ((float)hi[e] + (float)lo[e]) * NS_UNSCALE;
-}
-__device__ __forceinline__ void ns_zero(f32x16& a) {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) a[e] = 0.f;
 }
 
 template <int KP>
 __device__ __forceinline__ void ns_resident(const NsMat& m, int b, const NsUpdate& up, double eps, const float* abc, int steps,
                                             char* X, double* red) {
-    constexpr int KB = KP / 32, GROUPS8 = KP / 8, MINE = KP == 64 ? 1 : 2;      // MINE: blocks of G of a wave
+    // G and P: a wave's blocks of 16 x 16 are TA by TB; X: PAIRS pairs of blocks along k, a wave keeps to one pair
+    constexpr int GROUPS8 = KP / 8, TA = KP == 64 ? 1 : 2, TB = KP == 64 ? 2 : 4, PAIRS = KP / 32, SUM = KP / 32;
+    constexpr bool LOLO = KP == 64;
     const int np = m.np, t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     char* G = X + np * KP * 4;
-    float4* box = (float4*)(G + KP * KP * 4) + (wave & 3) * 256 + lane;
     // M, its momentum's update, its norm: a wave takes 64 rows n of eight columns k.  (Loads without branches, from the last row
     // or column where there is none: all in flight together.)
     float u[NS_RES_GROUPS][8];
@@ -942,134 +926,126 @@ __device__ __forceinline__ void ns_resident(const NsMat& m, int b, const NsUpdat
         *(half8*)(X + (at ^ 64)) = lo;
     }
     __syncthreads();
-    const int half = KP == 64 ? wave >> 2 : 0;
-    auto block = [&](int l, int& ia, int& ib) {
-        ia = KP == 64 ? wave >> 1 & 1 : wave >> 1;
-        ib = KP == 64 ? wave & 1 : (wave & 1) * 2 + l;
-    };
-    // the two half sums of a block of kp = 64 (second half first into its box); ends with everybody's products done
-    auto join = [&](f32x16& acc) {
-        if (KP == 64 && half) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) box[q * 64] = make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
-        }
-        __syncthreads();
-        if (KP == 64 && !half) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const float4 v = box[q * 64];
-                acc[4 * q] += v.x;
-                acc[4 * q + 1] += v.y;
-                acc[4 * q + 2] += v.z;
-                acc[4 * q + 3] += v.w;
-            }
-        }
-    };
     const float unscale = NS_UNSCALE * NS_UNSCALE;
-    f32x16 x[NS_RES_BLOCKS];
+    const int ia0 = (wave >> 1) * TA, ib0 = (wave & 1) * TB, pair = wave & (PAIRS - 1);
+    f32x4 x[NS_RES_UNITS][2];
     for (int step = 0; step < steps; ++step) {
         const float ca = abc[3 * step], cb = abc[3 * step + 1], cc = abc[3 * step + 2];
-        f32x16 acc[MINE];
+        f32x4 acc[TA][TB];
         // G = X^T X
 #pragma unroll
-        for (int l = 0; l < MINE; ++l) {
-            int ia, ib;
-            block(l, ia, ib);
-            ns_zero(acc[l]);
-            if (KP == 64) ns_columns(acc[l], X, np, ia, ib, half * (np / 32), (half + 1) * (np / 32));
-            else ns_columns(acc[l], X, np, ia, ib, 0, np / 16);
+        for (int i = 0; i < TA; ++i)
+#pragma unroll
+            for (int j = 0; j < TB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < np / 32; ++s) {
+            half8 ah[TA], al[TA], bh[TB], bl[TB];
+#pragma unroll
+            for (int i = 0; i < TA; ++i) ns_column16(X, np, ia0 + i, s, ah[i], al[i]);
+#pragma unroll
+            for (int j = 0; j < TB; ++j) ns_column16(X, np, ib0 + j, s, bh[j], bl[j]);
+#pragma unroll
+            for (int i = 0; i < TA; ++i)
+#pragma unroll
+                for (int j = 0; j < TB; ++j) ns_mfma<LOLO>(acc[i][j], ah[i], al[i], bh[j], bl[j]);
         }
-        join(acc[0]);
-        if (!half) {
 #pragma unroll
-            for (int l = 0; l < MINE; ++l) {
-                int ia, ib;
-                block(l, ia, ib);
+        for (int i = 0; i < TA; ++i)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const float v[4] = {acc[l][4 * q] * unscale, acc[l][4 * q + 1] * unscale, acc[l][4 * q + 2] * unscale,
-                                        acc[l][4 * q + 3] * unscale};
-                    ns_quad_put(G, KP, ia, ib, q, v);
-                }
+            for (int j = 0; j < TB; ++j) {
+                const float v[4] = {acc[i][j][0] * unscale, acc[i][j][1] * unscale, acc[i][j][2] * unscale, acc[i][j][3] * unscale};
+                ns_quad_put(G, KP, ia0 + i, ib0 + j, v);
+                acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
             }
-        }
         __syncthreads();
         // P = b G + c G G, in G's place
 #pragma unroll
-        for (int l = 0; l < MINE; ++l) {
-            int ia, ib;
-            block(l, ia, ib);
-            ns_zero(acc[l]);
-            ns_rows<KP == 64 ? 2 : 8>(acc[l], G, KP, ia, G, KP, ib, half * 2);
+        for (int s = 0; s < SUM; ++s) {
+            half8 ah[TA], al[TA], bh[TB], bl[TB];
+#pragma unroll
+            for (int i = 0; i < TA; ++i) ns_row16(G, KP, ia0 + i, s, ah[i], al[i]);
+#pragma unroll
+            for (int j = 0; j < TB; ++j) ns_row16(G, KP, ib0 + j, s, bh[j], bl[j]);
+#pragma unroll
+            for (int i = 0; i < TA; ++i)
+#pragma unroll
+                for (int j = 0; j < TB; ++j) ns_mfma<LOLO>(acc[i][j], ah[i], al[i], bh[j], bl[j]);
         }
-        join(acc[0]);
-        if (!half) {
+        __syncthreads();
 #pragma unroll
-            for (int l = 0; l < MINE; ++l) {
-                int ia, ib;
-                block(l, ia, ib);
+        for (int i = 0; i < TA; ++i)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    float v[4];
-                    ns_quad_get(G, KP, ia, ib, q, v);
+            for (int j = 0; j < TB; ++j) {
+                float v[4];
+                ns_quad_get(G, KP, ia0 + i, ib0 + j, v);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = cb * v[e] + cc * (acc[l][4 * q + e] * unscale);
-                    ns_quad_put(G, KP, ia, ib, q, v);
+                for (int e = 0; e < 4; ++e) v[e] = cb * v[e] + cc * (acc[i][j][e] * unscale);
+                ns_quad_put(G, KP, ia0 + i, ib0 + j, v);
+            }
+        __syncthreads();
+        // X <- a X + X P: every product first, then every block in its place
+        {
+            half8 ph[2][SUM], pl[2][SUM];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int s = 0; s < SUM; ++s) ns_row16(G, KP, pair * 2 + i, s, ph[i][s], pl[i][s]);
+#pragma unroll
+            for (int l = 0; l < NS_RES_UNITS; ++l) {
+                const int n = (l * 8 + wave) / PAIRS;
+                if (n < np / 16) {
+                    x[l][0] = x[l][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int s = 0; s < SUM; ++s) {
+                        half8 xh, xl;
+                        ns_row16(X, np, n, s, xh, xl);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) ns_mfma<LOLO>(x[l][i], ph[i][s], pl[i][s], xh, xl);
+                    }
                 }
             }
         }
         __syncthreads();
-        // X <- a X + X P: every product first, then every block in its place
 #pragma unroll
-        for (int l = 0; l < NS_RES_BLOCKS; ++l) {
-            const int unit = l * 8 + wave;
-            if (unit < np / 32 * KB) {
-                ns_zero(x[l]);
-                ns_rows<KP / 16>(x[l], G, KP, unit % KB, X, np, unit / KB, 0);
-            }
-        }
-        __syncthreads();
+        for (int l = 0; l < NS_RES_UNITS; ++l) {
+            const int n = (l * 8 + wave) / PAIRS;
+            if (n < np / 16) {
 #pragma unroll
-        for (int l = 0; l < NS_RES_BLOCKS; ++l) {
-            const int unit = l * 8 + wave;
-            if (unit < np / 32 * KB) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
+                for (int i = 0; i < 2; ++i) {
                     float v[4];
-                    ns_quad_get(X, np, unit % KB, unit / KB, q, v);
+                    ns_quad_get(X, np, pair * 2 + i, n, v);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[l][4 * q + e] = v[e] = x[l][4 * q + e] * unscale + ca * v[e];
-                    ns_quad_put(X, np, unit % KB, unit / KB, q, v);
+                    for (int e = 0; e < 4; ++e) x[l][i][e] = v[e] = x[l][i][e] * unscale + ca * v[e];
+                    ns_quad_put(X, np, pair * 2 + i, n, v);
                 }
             }
         }
         __syncthreads();
     }
-    // out of the registers of the last step: row n, columns k of a lane's quads
+    // out of the registers of the last step: row n, four columns k
     const long long row = m.tall ? m.out_ld : 1, col = m.tall ? 1 : m.out_ld;
 #pragma unroll
-    for (int l = 0; l < NS_RES_BLOCKS; ++l) {
-        const int unit = l * 8 + wave, n = unit / KB * 32 + (lane & 31), k0 = unit % KB * 32 + 4 * (lane >> 5);
-        if (unit >= np / 32 * KB) continue;
+    for (int l = 0; l < NS_RES_UNITS; ++l) {
+        const int n = (l * 8 + wave) / PAIRS * 16 + (lane & 15);
+        if ((l * 8 + wave) / PAIRS >= np / 16) continue;
         const long long base = b * m.out_bs + min(n, m.n - 1) * row;
-        if (up.on || m.type == 0) {
-            gfloat* p = (gfloat*)m.out + base;
-            float old[16];
-            if (up.on) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) old[i] = p[min(k0 + (i >> 2) * 8 + (i & 3), m.k - 1) * col];
-            }
+        for (int i = 0; i < 2; ++i) {
+            const int k0 = (pair * 2 + i) * 16 + 4 * (lane >> 4);
+            if (up.on || m.type == 0) {
+                gfloat* p = (gfloat*)m.out + base;
+                float old[4];
+                if (up.on) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int k = k0 + (i >> 2) * 8 + (i & 3);
-                if (n < m.n && k < m.k) p[k * col] = up.on ? old[i] * up.decay - m.step * x[l][i] : x[l][i];
-            }
-        } else {
-            gshort* p = (gshort*)m.out + base;
+                    for (int e = 0; e < 4; ++e) old[e] = p[min(k0 + e, m.k - 1) * col];
+                }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int k = k0 + (i >> 2) * 8 + (i & 3);
-                if (n < m.n && k < m.k) p[k * col] = (unsigned short)ns_pack(x[l][i], x[l][i], m.type);
+                for (int e = 0; e < 4; ++e)
+                    if (n < m.n && k0 + e < m.k) p[(k0 + e) * col] = up.on ? old[e] * up.decay - m.step * x[l][i][e] : x[l][i][e];
+            } else {
+                gshort* p = (gshort*)m.out + base;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n < m.n && k0 + e < m.k) p[(k0 + e) * col] = (unsigned short)ns_pack(x[l][i][e], x[l][i][e], m.type);
             }
         }
     }
@@ -1136,7 +1112,7 @@ static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
     // (measured, 64 x 64: 21 us whole, 111 us in tiles; the limits: LDS, and what a thread holds of X)
     const bool whole = (m.kp == 64 && m.np <= NS_RES_ROWS) || (m.kp == 128 && m.np == 128);
     if (whole) {
-        const int lds = m.np * m.kp * 4 + m.kp * m.kp * 4 + (m.kp == 64 ? 16384 : 0);
+        const int lds = m.np * m.kp * 4 + m.kp * m.kp * 4;
         if (lds > plan.lds) plan.lds = lds;
     } else {
         plan.wide |= m.tile == 128;
