@@ -68,17 +68,18 @@ struct __attribute__((aligned(16))) NsMat {
                     // units of G tiles (fold), whole matrices
 };
 
-// ---- pairs of fp16
-__device__ __forceinline__ void ns_split(float v, half_t& hi, half_t& lo) {
-    const float s = v * NS_SCALE;
+// ---- pairs of fp16: hi + lo = s, the value times 2^13 (everything between the first split and the output carries that factor;
+// a product's sums carry its square).  fmaf with a converted half is one instruction (v_fma_mix_f32).
+__device__ __forceinline__ void ns_split(float s, half_t& hi, half_t& lo) {
     hi = (half_t)s;
-    lo = (half_t)(s - (float)hi);
+    lo = (half_t)__builtin_fmaf((float)hi, -1.f, s);
 }
-__device__ __forceinline__ void ns_split8(const float* v, half8& hi, half8& lo) {
+__device__ __forceinline__ float ns_pair_sum(half_t hi, half_t lo) { return __builtin_fmaf((float)hi, 1.f, (float)lo); }
+__device__ __forceinline__ void ns_split8(const float* s, half8& hi, half8& lo) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         half_t h, l;
-        ns_split(v[e], h, l);
+        ns_split(s[e], h, l);
         hi[e] = h;
         lo[e] = l;
     }
@@ -221,7 +222,7 @@ __global__ __launch_bounds__(NS_THREADS) void k_ns_planes(const NsMat* tab, int 
         if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
         __syncthreads();
     }
-    const double norm = sqrt(red[0]) + eps;
+    const double inverse = 1 / (sqrt(red[0]) + eps);      // (0 / 0, inf 0: NaN as by division)
     // rows of M along threadIdx / 64, columns along the lanes; tile[n][k]
     for (int i = threadIdx.x >> 6; i < 64; i += NS_THREADS / 64) {
         const int j = threadIdx.x & 63;
@@ -234,7 +235,7 @@ __global__ __launch_bounds__(NS_THREADS) void k_ns_planes(const NsMat* tab, int 
                 const float mom = m.mom[(size_t)r * m.cols + c];
                 v = up.nesterov ? v * up.omu + mom * up.mu : mom;
             }
-            v = (float)(v / norm);
+            v = (float)(v * inverse) * NS_SCALE;
         }
         if (m.tall) tile[i][j] = v;
         else tile[j][i] = v;
@@ -491,7 +492,7 @@ struct NsTile {
 // once).  It belongs to one wave (or, in the fold, to the workgroup).
 template <int UC>
 __device__ __forceinline__ void ns_put_quad(float* unit, int i, int q, int lane, float4 v) {
-    const float s = NS_UNSCALE * NS_UNSCALE;
+    const float s = NS_UNSCALE;
     *(float4*)(unit + (lane & 31) * (UC + 4) + i * 32 + q * 8 + (lane >> 5) * 4) = make_float4(v.x * s, v.y * s, v.z * s, v.w * s);
 }
 template <int T, bool TR>
@@ -661,7 +662,7 @@ __device__ __forceinline__ void ns_poly(const NsMat& m, float cb, float cc, char
         float v[8];
         ns_along<Tile::UC>(mine, row, col, v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = cc * v[e] + cb * (((float)gh[l][e] + (float)gl[l][e]) * NS_UNSCALE);
+        for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(cc, v[e], cb * ns_pair_sum(gh[l][e], gl[l][e]));
         float4* p = (float4*)(mine + row * (Tile::UC + 4) + col);
         p[0] = make_float4(v[0], v[1], v[2], v[3]);
         p[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -748,7 +749,7 @@ __device__ __forceinline__ void ns_apply(const NsMat& m, int from, float ca, boo
         float v[8];
         ns_along<Tile::UC>(mine, row, col, v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += ca * (((float)xh[l][e] + (float)xl[l][e]) * NS_UNSCALE);
+        for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(ca, ns_pair_sum(xh[l][e], xl[l][e]), v[e]) * (last ? NS_UNSCALE : 1.f);
         if (!last) {
             if (n0 + row < m.np && k0 + col < m.kp) ns_write8(out, ns_at(n0 + row, k0 + col, m.np), v);
         } else if (m.tall) {
@@ -782,8 +783,6 @@ __global__ __launch_bounds__(NS_WIDE) void k_ns_apply(const NsMat* tab, int coun
 // kp = 64 adds lo lo: its short sums round so little that the dropped term would show.
 // LDS: X [block of 32 columns][n][128 bytes], then G / P [block][k][128 bytes], piece q of row r at place q ^ (r / 2 % 8).
 #define NS_RES_ROWS 256
-#define NS_RES_GROUPS 4      // groups of eight elements of a thread: 256 * 64 / 8 / 512
-#define NS_RES_UNITS 4       // pairs of 16 x 16 blocks of X of a wave: 256 / 16 * 2 / 8
 struct NsCoef {
     float v[3 * NS_MAX_STEPS];
 };
@@ -791,20 +790,25 @@ struct NsCoef {
 __device__ __forceinline__ int ns_place(int rows, int row, int piece, int blk) {
     return (blk * rows + row) * 128 + ((piece ^ ((row >> 1) & 7)) << 4);
 }
-// operand of a 16 x 16 x 32 product: rows block * 16 .. + 15 of planes, columns of block `s` of 32
-__device__ __forceinline__ void ns_row16(const char* planes, int rows, int block, int s, half8& hi, half8& lo) {
-    const int lane = threadIdx.x & 63, at = ns_place(rows, block * 16 + (lane & 15), lane >> 4, s);
-    hi = *(const half8*)(planes + at);
-    lo = *(const half8*)(planes + (at ^ 64));
+// Operands of 16 x 16 x 32 products out of planes of ROWS rows.  Rows block * 16 .. + 15, columns of block `s` of 32: `at` as
+// ns_row_at says, s * ROWS * 128 further (an immediate).
+__device__ __forceinline__ int ns_row_at(int rows, int block) {
+    const int lane = threadIdx.x & 63;
+    return ns_place(rows, block * 16 + (lane & 15), lane >> 4, 0);
 }
-// ... columns block * 16 .. + 15, rows s * 32 .. + 31
-__device__ __forceinline__ void ns_column16(const char* planes, int rows, int block, int s, half8& hi, half8& lo) {
-    const int lane = threadIdx.x & 63, g = lane >> 4, q = (lane & 15) >> 2, p = lane & 3, chunk = 2 * (block & 1) + (p >> 1);
-    const int first = ns_place(rows, s * 32 + 8 * g + q, chunk, block >> 1) + (p & 1) * 8;
-    const int second = ns_place(rows, s * 32 + 8 * g + q + 4, chunk, block >> 1) + (p & 1) * 8;
+__device__ __forceinline__ void ns_row16(const char* planes, int at, int offset, half8& hi, half8& lo) {
+    hi = *(const half8*)(planes + at + offset);
+    lo = *(const half8*)(planes + (at ^ 64) + offset);
+}
+// ... columns block * 16 .. + 15, rows s * 32 .. + 31: s * 32 * 128 further
+__device__ __forceinline__ int ns_column_at(int rows, int block, int second) {
+    const int lane = threadIdx.x & 63, q = (lane & 15) >> 2, p = lane & 3;
+    return ns_place(rows, 8 * (lane >> 4) + q + 4 * second, 2 * (block & 1) + (p >> 1), block >> 1) + (p & 1) * 8;
+}
+__device__ __forceinline__ void ns_column16(const char* planes, int first, int second, int offset, half8& hi, half8& lo) {
     auto read = [&](int flip) {
-        const s16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(planes + (first ^ flip)));
-        const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(planes + (second ^ flip)));
+        const s16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(planes + (first ^ flip) + offset));
+        const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(planes + (second ^ flip) + offset));
         return __builtin_bit_cast(half8, __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7));
     };
     hi = read(0);
@@ -840,27 +844,28 @@ __device__ __forceinline__ void ns_quad_get(const char* planes, int rows, int ia
     const int at = ns_quad_at(rows, ia, ib);
     const half4 hi = *(const half4*)(planes + at), lo = *(const half4*)(planes + (at ^ 64));
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = ((float)hi[e] + (float)lo[e]) * NS_UNSCALE;
+    for (int e = 0; e < 4; ++e) v[e] = ns_pair_sum(hi[e], lo[e]);
 }
 
-template <int KP>
+template <int KP, int NP>
 __device__ __forceinline__ void ns_resident(const NsMat& m, int b, const NsUpdate& up, double eps, const float* abc, int steps,
                                             char* X, double* red) {
     // G and P: a wave's blocks of 16 x 16 are TA by TB; X: PAIRS pairs of blocks along k, a wave keeps to one pair
     constexpr int GROUPS8 = KP / 8, TA = KP == 64 ? 1 : 2, TB = KP == 64 ? 2 : 4, PAIRS = KP / 32, SUM = KP / 32;
     constexpr bool LOLO = KP == 64;
-    const int np = m.np, t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    char* G = X + np * KP * 4;
+    constexpr int GROUPS = (NP / 64 * GROUPS8 + 7) / 8, UNITS = (NP / 16 * PAIRS + 7) / 8;      // of a wave, rounded up
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    char* G = X + NP * KP * 4;
     // M, its momentum's update, its norm: a wave takes 64 rows n of eight columns k.  (Loads without branches, from the last row
     // or column where there is none: all in flight together.)
-    float u[NS_RES_GROUPS][8];
-    const int groups = np / 64 * GROUPS8;      // of a matrix; this wave's: wave, wave + 8, ...
+    float u[GROUPS][8];
+    const int groups = NP / 64 * GROUPS8;      // of a matrix; this wave's: wave, wave + 8, ...
     auto first_of = [&](int group, long long ld) { return min(group / GROUPS8 * 64 + lane, m.n - 1) * (m.tall ? ld : 1); };
     auto column_of = [&](int group, int e, long long ld) { return min(group % GROUPS8 * 8 + e, m.k - 1) * (m.tall ? 1 : ld); };
     if (m.type == 0) {
         const gfloat* in = (const gfloat*)m.in + b * m.in_bs;
 #pragma unroll
-        for (int l = 0; l < NS_RES_GROUPS; ++l)
+        for (int l = 0; l < GROUPS; ++l)
             if (l * 8 + wave < groups) {
                 const gfloat* p = in + first_of(l * 8 + wave, m.in_ld);
 #pragma unroll
@@ -868,23 +873,23 @@ __device__ __forceinline__ void ns_resident(const NsMat& m, int b, const NsUpdat
             }
     } else {
         const gshort* in = (const gshort*)m.in + b * m.in_bs;
-        unsigned short raw[NS_RES_GROUPS][8];
+        unsigned short raw[GROUPS][8];
 #pragma unroll
-        for (int l = 0; l < NS_RES_GROUPS; ++l)
+        for (int l = 0; l < GROUPS; ++l)
             if (l * 8 + wave < groups) {
                 const gshort* p = in + first_of(l * 8 + wave, m.in_ld);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) raw[l][e] = p[column_of(l * 8 + wave, e, m.in_ld)];
             }
 #pragma unroll
-        for (int l = 0; l < NS_RES_GROUPS; ++l)
+        for (int l = 0; l < GROUPS; ++l)
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 u[l][e] = ns_value(raw[l][e], m.type);
     }
     double s = 0;
 #pragma unroll
-    for (int l = 0; l < NS_RES_GROUPS; ++l) {
+    for (int l = 0; l < GROUPS; ++l) {
         const int group = l * 8 + wave, n = group / GROUPS8 * 64 + lane, k = group % GROUPS8 * 8;
         if (group >= groups) continue;
         float mom[8];
@@ -912,63 +917,82 @@ __device__ __forceinline__ void ns_resident(const NsMat& m, int b, const NsUpdat
     if (lane == 0) red[wave] = s;
     __syncthreads();
     s = ((red[0] + red[1]) + (red[2] + red[3])) + ((red[4] + red[5]) + (red[6] + red[7]));
-    const double norm = sqrt(s) + eps;
+    const double inverse = 1 / (sqrt(s) + eps);
 #pragma unroll
-    for (int l = 0; l < NS_RES_GROUPS; ++l) {
+    for (int l = 0; l < GROUPS; ++l) {
         const int group = l * 8 + wave;
         if (group >= groups) continue;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) u[l][e] = (float)(u[l][e] / norm);
+        for (int e = 0; e < 8; ++e) u[l][e] = (float)(u[l][e] * inverse) * NS_SCALE;
         half8 hi, lo;
         ns_split8(u[l], hi, lo);
-        const int at = ns_place(np, group / GROUPS8 * 64 + lane, group % GROUPS8 & 3, group % GROUPS8 >> 2);
+        const int at = ns_place(NP, group / GROUPS8 * 64 + lane, group % GROUPS8 & 3, group % GROUPS8 >> 2);
         *(half8*)(X + at) = hi;
         *(half8*)(X + (at ^ 64)) = lo;
     }
     __syncthreads();
-    const float unscale = NS_UNSCALE * NS_UNSCALE;
     const int ia0 = (wave >> 1) * TA, ib0 = (wave & 1) * TB, pair = wave & (PAIRS - 1);
-    f32x4 x[NS_RES_UNITS][2];
+    f32x4 x[UNITS][2];
     for (int step = 0; step < steps; ++step) {
-        const float ca = abc[3 * step], cb = abc[3 * step + 1], cc = abc[3 * step + 2];
+        const float ca = abc[3 * step], cb = abc[3 * step + 1], cc = abc[3 * step + 2] * NS_UNSCALE;
         f32x4 acc[TA][TB];
-        // G = X^T X
+        auto clear = [&]() {
 #pragma unroll
-        for (int i = 0; i < TA; ++i)
+            for (int i = 0; i < TA; ++i)
 #pragma unroll
-            for (int j = 0; j < TB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < np / 32; ++s) {
-            half8 ah[TA], al[TA], bh[TB], bl[TB];
-#pragma unroll
-            for (int i = 0; i < TA; ++i) ns_column16(X, np, ia0 + i, s, ah[i], al[i]);
-#pragma unroll
-            for (int j = 0; j < TB; ++j) ns_column16(X, np, ib0 + j, s, bh[j], bl[j]);
+                for (int j = 0; j < TB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        };
+        auto multiply = [&](const half8* ah, const half8* al, const half8* bh, const half8* bl) {
 #pragma unroll
             for (int i = 0; i < TA; ++i)
 #pragma unroll
                 for (int j = 0; j < TB; ++j) ns_mfma<LOLO>(acc[i][j], ah[i], al[i], bh[j], bl[j]);
+        };
+        // G = X^T X
+        {
+            int a1[TA], a2[TA], b1[TB], b2[TB];
+#pragma unroll
+            for (int i = 0; i < TA; ++i) { a1[i] = ns_column_at(NP, ia0 + i, 0); a2[i] = ns_column_at(NP, ia0 + i, 1); }
+#pragma unroll
+            for (int j = 0; j < TB; ++j) { b1[j] = ns_column_at(NP, ib0 + j, 0); b2[j] = ns_column_at(NP, ib0 + j, 1); }
+            clear();
+#pragma unroll 2
+            for (int s = 0; s < NP / 32; ++s) {
+                half8 ah[TA], al[TA], bh[TB], bl[TB];
+#pragma unroll
+                for (int i = 0; i < TA; ++i) ns_column16(X, a1[i], a2[i], s * 4096, ah[i], al[i]);
+#pragma unroll
+                for (int j = 0; j < TB; ++j) ns_column16(X, b1[j], b2[j], s * 4096, bh[j], bl[j]);
+                multiply(ah, al, bh, bl);
+            }
         }
 #pragma unroll
         for (int i = 0; i < TA; ++i)
 #pragma unroll
             for (int j = 0; j < TB; ++j) {
-                const float v[4] = {acc[i][j][0] * unscale, acc[i][j][1] * unscale, acc[i][j][2] * unscale, acc[i][j][3] * unscale};
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * NS_UNSCALE;
                 ns_quad_put(G, KP, ia0 + i, ib0 + j, v);
-                acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
             }
         __syncthreads();
         // P = b G + c G G, in G's place
+        clear();
+        {
+            int a1[TA], b1[TB];
 #pragma unroll
-        for (int s = 0; s < SUM; ++s) {
-            half8 ah[TA], al[TA], bh[TB], bl[TB];
+            for (int i = 0; i < TA; ++i) a1[i] = ns_row_at(KP, ia0 + i);
 #pragma unroll
-            for (int i = 0; i < TA; ++i) ns_row16(G, KP, ia0 + i, s, ah[i], al[i]);
+            for (int j = 0; j < TB; ++j) b1[j] = ns_row_at(KP, ib0 + j);
 #pragma unroll
-            for (int j = 0; j < TB; ++j) ns_row16(G, KP, ib0 + j, s, bh[j], bl[j]);
+            for (int s = 0; s < SUM; ++s) {
+                half8 ah[TA], al[TA], bh[TB], bl[TB];
 #pragma unroll
-            for (int i = 0; i < TA; ++i)
+                for (int i = 0; i < TA; ++i) ns_row16(G, a1[i], s * KP * 128, ah[i], al[i]);
 #pragma unroll
-                for (int j = 0; j < TB; ++j) ns_mfma<LOLO>(acc[i][j], ah[i], al[i], bh[j], bl[j]);
+                for (int j = 0; j < TB; ++j) ns_row16(G, b1[j], s * KP * 128, bh[j], bl[j]);
+                multiply(ah, al, bh, bl);
+            }
         }
         __syncthreads();
 #pragma unroll
@@ -978,7 +1002,7 @@ __device__ __forceinline__ void ns_resident(const NsMat& m, int b, const NsUpdat
                 float v[4];
                 ns_quad_get(G, KP, ia0 + i, ib0 + j, v);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = cb * v[e] + cc * (acc[i][j][e] * unscale);
+                for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(cc, acc[i][j][e], cb * v[e]);
                 ns_quad_put(G, KP, ia0 + i, ib0 + j, v);
             }
         __syncthreads();
@@ -988,16 +1012,17 @@ __device__ __forceinline__ void ns_resident(const NsMat& m, int b, const NsUpdat
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int s = 0; s < SUM; ++s) ns_row16(G, KP, pair * 2 + i, s, ph[i][s], pl[i][s]);
+                for (int s = 0; s < SUM; ++s) ns_row16(G, ns_row_at(KP, pair * 2 + i), s * KP * 128, ph[i][s], pl[i][s]);
 #pragma unroll
-            for (int l = 0; l < NS_RES_UNITS; ++l) {
+            for (int l = 0; l < UNITS; ++l) {
                 const int n = (l * 8 + wave) / PAIRS;
-                if (n < np / 16) {
+                if (n < NP / 16) {
                     x[l][0] = x[l][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    const int at = ns_row_at(NP, n);
 #pragma unroll
                     for (int s = 0; s < SUM; ++s) {
                         half8 xh, xl;
-                        ns_row16(X, np, n, s, xh, xl);
+                        ns_row16(X, at, s * NP * 128, xh, xl);
 #pragma unroll
                         for (int i = 0; i < 2; ++i) ns_mfma<LOLO>(x[l][i], ph[i][s], pl[i][s], xh, xl);
                     }
@@ -1006,16 +1031,16 @@ __device__ __forceinline__ void ns_resident(const NsMat& m, int b, const NsUpdat
         }
         __syncthreads();
 #pragma unroll
-        for (int l = 0; l < NS_RES_UNITS; ++l) {
+        for (int l = 0; l < UNITS; ++l) {
             const int n = (l * 8 + wave) / PAIRS;
-            if (n < np / 16) {
+            if (n < NP / 16) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     float v[4];
-                    ns_quad_get(X, np, pair * 2 + i, n, v);
+                    ns_quad_get(X, NP, pair * 2 + i, n, v);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[l][i][e] = v[e] = x[l][i][e] * unscale + ca * v[e];
-                    ns_quad_put(X, np, pair * 2 + i, n, v);
+                    for (int e = 0; e < 4; ++e) x[l][i][e] = v[e] = __builtin_fmaf(x[l][i][e], NS_UNSCALE, ca * v[e]);
+                    ns_quad_put(X, NP, pair * 2 + i, n, v);
                 }
             }
         }
@@ -1024,10 +1049,12 @@ __device__ __forceinline__ void ns_resident(const NsMat& m, int b, const NsUpdat
     // out of the registers of the last step: row n, four columns k
     const long long row = m.tall ? m.out_ld : 1, col = m.tall ? 1 : m.out_ld;
 #pragma unroll
-    for (int l = 0; l < NS_RES_UNITS; ++l) {
+    for (int l = 0; l < UNITS; ++l) {
         const int n = (l * 8 + wave) / PAIRS * 16 + (lane & 15);
-        if ((l * 8 + wave) / PAIRS >= np / 16) continue;
+        if ((l * 8 + wave) / PAIRS >= NP / 16) continue;
         const long long base = b * m.out_bs + min(n, m.n - 1) * row;
+        x[l][0] *= NS_UNSCALE;
+        x[l][1] *= NS_UNSCALE;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int k0 = (pair * 2 + i) * 16 + 4 * (lane >> 4);
@@ -1059,8 +1086,11 @@ __global__ __launch_bounds__(NS_WIDE) void k_ns_resident(const NsTable args, con
     const NsMat m = ns_find<NS_RESIDENT>(tab ? (NsTab)tab : (NsTab)__builtin_amdgcn_kernarg_segment_ptr(), count);
     if ((int)threadIdx.x < 3 * steps) abc[threadIdx.x] = coef.v[threadIdx.x];
     const int b = blockIdx.x - m.at[NS_RESIDENT];
-    if (m.kp == 64) ns_resident<64>(m, b, up, eps, abc, steps, lds, red);
-    else ns_resident<128>(m, b, up, eps, abc, steps, lds, red);
+    if (m.kp == 128) ns_resident<128, 128>(m, b, up, eps, abc, steps, lds, red);
+    else if (m.np == 64) ns_resident<64, 64>(m, b, up, eps, abc, steps, lds, red);
+    else if (m.np == 128) ns_resident<64, 128>(m, b, up, eps, abc, steps, lds, red);
+    else if (m.np == 192) ns_resident<64, 192>(m, b, up, eps, abc, steps, lds, red);
+    else ns_resident<64, 256>(m, b, up, eps, abc, steps, lds, red);
 }
 
 // ---- host side
