@@ -9,11 +9,13 @@
 //     S0[p] = sum du, S1[p] = sum du zhat over the rows of plot p; every parameter gradient follows from these two:
 //     dgate = keep scale (w S1 + b S0), dscale = sum_p keep gate (w S1 + b S0), dw = sum_p f S1, db = sum_p f S0.
 // Bound: HBM.  Forward 3 N C e bytes (z, r, y; + h), backward 5 N C e (z, r, dy, dz, dr; + dh).
-// A row belongs to G lanes (8 .. 64 of one wave, 256 for the widest rows) that hold V pieces of W channels each: W = 4 where
-// widths, strides and addresses allow 4-channel accesses, else 1.  A workgroup owns a contiguous run of rows and walks it plot
-// segment by plot segment; each (run, plot) pair leaves ONE partial column sum in slot run + plot — both only grow along the
-// rows, so the slots are distinct and runs + plots + 1 of them are enough — folded in slot order: no atomics, results repeat
-// bit for bit.
+// A row belongs to G lanes (8 .. 64 of one wave, 256 for the widest rows) that hold V pieces of 16 bytes each where widths,
+// strides and addresses allow, single channels otherwise; the next row is in flight while one is worked on.  A workgroup owns a
+// contiguous run of rows and walks it plot segment by plot segment; each (run, plot) pair leaves ONE partial column sum in slot
+// run + plot — both only grow along the rows, so the slots are distinct and runs + plots + 1 of them are enough — folded in slot
+// order: no atomics, results repeat bit for bit.
+// What a bf16 element may cost beside HBM is about 60 vector instructions (37 T lane-instructions/s against 1 T elements/s at 5
+// to 6 bytes): hence the fused parameters f w and f b, the one exponential that value and slope of the GELU share, no compares.
 #include "agb_common.h"
 
 #define RN_THREADS 256
@@ -61,45 +63,69 @@ __device__ __forceinline__ float rn_sum(float v, float* red, int& turn) {
     return v;
 }
 
+typedef unsigned rn_u32x4 __attribute__((ext_vector_type(4)));
+// a piece of W channels as it lies in memory: 16 bytes (W = 4 fp32, 8 bf16) or one channel
 template <typename T, int W>
-__device__ __forceinline__ void rn_load(const T* p, float* v) {
-    if constexpr (W == 4) {
-        const float4 q = ld4(p);
-        v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-    } else {
-        v[0] = ld1(p);
-    }
-}
-template <typename T, int W>
-__device__ __forceinline__ void rn_store(T* p, const float* v) {
-    if constexpr (W == 4) st4(p, make_float4(v[0], v[1], v[2], v[3]));
-    else st1(p, v[0]);
-}
-
-// a row's pieces (0 behind the last channel or where `on` is false); parameters: `other` where there is no vector
-template <typename T, int W, int G, int V>
-__device__ __forceinline__ void rn_row(const void* base, long long ld, long long row, int lane, int C, bool on, float* v) {
-    const T* p = (const T*)base + row * ld;
+struct RnPiece {
+    rn_u32x4 raw;
+    __device__ __forceinline__ void load(const T* p) { raw = *(const rn_u32x4*)p; }
+    __device__ __forceinline__ void clear() { raw = rn_u32x4{0, 0, 0, 0}; }
+    __device__ __forceinline__ void get(float* v) const {
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int c = (j * G + lane) * W;
-        if (on && c < C) {
-            rn_load<T, W>(p + c, v + j * W);
+            for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(raw[e]);
         } else {
 #pragma unroll
-            for (int e = 0; e < W; ++e) v[j * W + e] = 0.f;
+            for (int e = 0; e < 4; ++e) {
+                v[2 * e] = __uint_as_float(raw[e] << 16);
+                v[2 * e + 1] = __uint_as_float(raw[e] & 0xFFFF0000u);
+            }
         }
     }
-}
+    static __device__ __forceinline__ void put(T* p, const float* v) {
+        rn_u32x4 q;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[e] = sizeof(T) == 4 ? __float_as_uint(v[e]) : agb_pack2_bf16(v[2 * e], v[2 * e + 1]);
+        *(rn_u32x4*)p = q;
+    }
+};
+template <typename T>
+struct RnPiece<T, 1> {
+    float raw;
+    __device__ __forceinline__ void load(const T* p) { raw = ld1(p); }
+    __device__ __forceinline__ void clear() { raw = 0.f; }
+    __device__ __forceinline__ void get(float* v) const { *v = raw; }
+    static __device__ __forceinline__ void put(T* p, const float* v) { st1(p, *v); }
+};
+
+// a row's pieces: zeros behind the last channel, where there is no matrix and where `on` is false
+template <typename T, int W, int G, int V>
+struct RnRow {
+    RnPiece<T, W> piece[V];
+    __device__ __forceinline__ void load(const void* base, long long ld, long long row, int lane, int C, bool on) {
+        const T* p = (const T*)base + row * ld;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = (j * G + lane) * W;
+            if (on && base && c < C) piece[j].load(p + c);
+            else piece[j].clear();
+        }
+    }
+    __device__ __forceinline__ void get(float* v) const {
+#pragma unroll
+        for (int j = 0; j < V; ++j) piece[j].get(v + j * W);
+    }
+};
 template <typename T, int W, int G, int V>
 __device__ __forceinline__ void rn_put(void* base, long long ld, long long row, int lane, int C, bool on, const float* v) {
     T* p = (T*)base + row * ld;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const int c = (j * G + lane) * W;
-        if (on && c < C) rn_store<T, W>(p + c, v + j * W);
+        if (on && c < C) RnPiece<T, W>::put(p + c, v + j * W);
     }
 }
+// a parameter vector's values: `other` where there is none, 0 behind the last channel
 template <int W, int G, int V>
 __device__ __forceinline__ void rn_vec(const float* p, int lane, int C, float other, float* v) {
 #pragma unroll
@@ -111,25 +137,23 @@ __device__ __forceinline__ void rn_vec(const float* p, int lane, int C, float ot
         }
 }
 
-// x <- xhat in place (0 behind the last channel: the sums below run over every piece), returns rstd
+// x <- xhat in place, returns rstd; 0 for both where `on` is false.  there[j]: 1 for a piece of channels, 0 behind the last
+// channel (where x is 0 and stays 0)
 template <int W, int G, int V>
-__device__ __forceinline__ float rn_normalise(float* x, int lane, int C, bool rms, float eps, float* red, int& turn) {
-    const float inv = 1.f / (float)C;
-    float mean = 0.f;
+__device__ __forceinline__ float rn_normalise(float* x, const float* there, float inv, bool rms, float eps, bool on, float* red, int& turn) {
     if (!rms) {
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < V * W; ++i) s += x[i];
-        mean = rn_sum<G>(s, red, turn) * inv;
+        const float mean = rn_sum<G>(s, red, turn) * inv;
+#pragma unroll
+        for (int i = 0; i < V * W; ++i) x[i] = __builtin_fmaf(-mean, there[i / W], x[i]);
     }
     float q = 0.f;
 #pragma unroll
-    for (int i = 0; i < V * W; ++i) {
-        const int c = ((i / W) * G + lane) * W + i % W;
-        x[i] = c < C ? x[i] - mean : 0.f;
-        q += x[i] * x[i];
-    }
-    const float rstd = 1.f / sqrtf(rn_sum<G>(q, red, turn) * inv + eps);
+    for (int i = 0; i < V * W; ++i) q = __builtin_fmaf(x[i], x[i], q);
+    float rstd = rsqrtf(__builtin_fmaf(rn_sum<G>(q, red, turn), inv, eps));
+    rstd = on ? rstd : 0.f;
 #pragma unroll
     for (int i = 0; i < V * W; ++i) x[i] *= rstd;
     return rstd;
@@ -137,15 +161,28 @@ __device__ __forceinline__ float rn_normalise(float* x, int lane, int C, bool rm
 
 // d <- rstd (d - [mean d] - xhat mean(d xhat))
 template <int W, int G, int V>
-__device__ __forceinline__ void rn_norm_grad(float* d, const float* xhat, float rstd, int C, bool rms, float* red, int& turn) {
-    const float inv = 1.f / (float)C;
+__device__ __forceinline__ void rn_norm_grad(float* d, const float* xhat, float rstd, float inv, bool rms, float* red, int& turn) {
     float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-    for (int i = 0; i < V * W; ++i) { s0 += d[i]; s1 += d[i] * xhat[i]; }
-    s1 = rn_sum<G>(s1, red, turn) * inv;
-    s0 = rms ? 0.f : rn_sum<G>(s0, red, turn) * inv;
+    for (int i = 0; i < V * W; ++i) { s0 += d[i]; s1 = __builtin_fmaf(d[i], xhat[i], s1); }
+    s1 = rn_sum<G>(s1, red, turn) * inv * rstd;
+    s0 = rms ? 0.f : rn_sum<G>(s0, red, turn) * inv * rstd;
 #pragma unroll
-    for (int i = 0; i < V * W; ++i) d[i] = rstd * (d[i] - s0 - xhat[i] * s1);
+    for (int i = 0; i < V * W; ++i) d[i] = __builtin_fmaf(-xhat[i], s1, __builtin_fmaf(d[i], rstd, -s0));
+}
+
+// GELU u Phi(u) and its slope Phi(u) + u phi(u).  Phi(-|u|) = erfc(|u| / sqrt 2) / 2 by Abramowitz and Stegun 7.1.26 (error of
+// erf at most 1.5e-7), whose exponential is phi's: 20 instructions for both, where the library's erff and an exponential take 60.
+__device__ __forceinline__ void rn_gelu(float u, float& y, float& slope) {
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.23164189f, __builtin_fabsf(u), 1.f));      // 0.3275911 / sqrt 2
+    const float e = __builtin_amdgcn_exp2f(u * u * -0.72134752f);
+    float p = __builtin_fmaf(t, 0.5307027145f, -0.7265760135f);
+    p = __builtin_fmaf(t, p, 0.7107068705f);
+    p = __builtin_fmaf(t, p, -0.142248368f);
+    p = __builtin_fmaf(t, p, 0.127414796f);
+    const float tail = p * t * e, cdf = u > 0.f ? 1.f - tail : tail;
+    y = u * cdf;
+    slope = __builtin_fmaf(u * 0.39894228f, e, cdf);
 }
 
 // the plot of a row: how many of ptr[1 .. B] are <= row (B: behind the last plot)
@@ -159,17 +196,20 @@ __device__ __forceinline__ int rn_plot(const int32_t* ptr, int B, int row) {
     return lo;
 }
 
-// keep[p] gate[p] scale of plot p; 0 behind the last plot (such a row is handed on as act(r))
+// f w and f b with f = keep[p] gate[p] scale of plot p; 0 behind the last plot (such a row is handed on as act(r))
 template <int W, int G, int V>
-__device__ __forceinline__ void rn_factor(const RnArgs& a, int p, int lane, float* f) {
-    rn_vec<W, G, V>(a.scale, lane, a.C, 1.f, f);
-    if (!a.ptr) return;
-    const float k = p >= a.B ? 0.f : a.keep ? a.keep[p] : 1.f;
+__device__ __forceinline__ void rn_factor(const RnArgs& a, int p, int lane, float* fw, float* fb) {
+    const float k = !a.ptr ? 1.f : p >= a.B ? 0.f : a.keep ? a.keep[p] : 1.f;
 #pragma unroll
     for (int i = 0; i < V * W; ++i) {
         const int c = ((i / W) * G + lane) * W + i % W;
-        const float g = (a.gate && p < a.B && c < a.C) ? a.gate[(size_t)p * a.C + c] : 1.f;
-        f[i] *= k * g;
+        float f = c < a.C ? k : 0.f;
+        if (c < a.C) {
+            if (a.scale) f *= a.scale[c];
+            if (a.gate && p < a.B) f *= a.gate[(size_t)p * a.C + c];
+        }
+        fw[i] = f * (a.w && c < a.C ? a.w[c] : 1.f);
+        fb[i] = f * (a.b && c < a.C ? a.b[c] : 0.f);
     }
 }
 
@@ -178,18 +218,20 @@ template <typename T, int W, int G, int V, bool BWD, bool NEXT>
 __global__ __launch_bounds__(RN_THREADS) void k_rownorm(const RnArgs a) {
     constexpr int N = V * W, GROUPS = RN_THREADS / G;
     constexpr int SUMS = NEXT ? 4 : 2;
+    typedef RnRow<T, W, G, V> Row;
     __shared__ float red[8];
     __shared__ float fold[(BWD && GROUPS > 1) ? RN_THREADS * N : 1];
     const int lane = threadIdx.x & (G - 1), group = threadIdx.x / G;
     int turn = 0;
     const int first = blockIdx.x * a.rows;
     const int last = min(a.n, first + a.rows);
-    float w[N], b[N], w2[NEXT ? N : 1], b2[NEXT ? N : 1];
-    rn_vec<W, G, V>(a.w, lane, a.C, 1.f, w);
-    rn_vec<W, G, V>(a.b, lane, a.C, 0.f, b);
+    const float inv = 1.f / (float)a.C;
+    float there[V], w2[NEXT ? N : 1], b2[(NEXT && !BWD) ? N : 1];
+#pragma unroll
+    for (int j = 0; j < V; ++j) there[j] = (j * G + lane) * W < a.C ? 1.f : 0.f;
     if constexpr (NEXT) {
         rn_vec<W, G, V>(a.w2, lane, a.C, 1.f, w2);
-        rn_vec<W, G, V>(a.b2, lane, a.C, 0.f, b2);
+        if constexpr (!BWD) rn_vec<W, G, V>(a.b2, lane, a.C, 0.f, b2);
     }
     int row0 = first;
     int p = a.ptr ? rn_plot(a.ptr, a.B, first) : 0;
@@ -200,77 +242,95 @@ __global__ __launch_bounds__(RN_THREADS) void k_rownorm(const RnArgs a) {
             if (p < a.B) end = min(last, a.ptr[p + 1]);
         }
         const bool live = !a.ptr || p < a.B;      // (rows behind the last plot: y = act(r), dz = 0 whatever z holds)
-        float f[N], sums[BWD ? SUMS : 1][N];
-        rn_factor<W, G, V>(a, p, lane, f);
+        float fw[N], fb[N], sums[BWD ? SUMS : 1][N];
+        rn_factor<W, G, V>(a, p, lane, fw, fb);
         if constexpr (BWD) {
 #pragma unroll
             for (int s = 0; s < SUMS; ++s)
 #pragma unroll
                 for (int i = 0; i < N; ++i) sums[s][i] = 0.f;
         }
+        Row z, r, dy, dh;
+        auto fetch = [&](int at) {
+            const long long row = at + group;
+            const bool on = row < end;
+            z.load(a.z, a.ldz, row, lane, a.C, on);
+            r.load(a.r, a.ldr, row, lane, a.C, on);
+            if constexpr (BWD) dy.load(a.dy, a.lddy, row, lane, a.C, on);
+            if constexpr (BWD && NEXT) dh.load(a.dh, a.lddh, row, lane, a.C, on);
+        };
+        fetch(row0);
         for (int at = row0; at < end; at += GROUPS) {      // (every lane takes every turn: the sums need whole groups)
             const long long row = at + group;
             const bool on = row < end;
-            float x[N], u[N];
-            rn_row<T, W, G, V>(a.z, a.ldz, row, lane, a.C, on, x);
-            if (a.r) rn_row<T, W, G, V>(a.r, a.ldr, row, lane, a.C, on, u);
-            else {
+            float x[N], u[N], g[BWD ? N : 1], h[(BWD && NEXT) ? N : 1];
+            z.get(x);
+            r.get(u);
+            if constexpr (BWD) dy.get(g);
+            if constexpr (BWD && NEXT) dh.get(h);
+            if (at + GROUPS < end) fetch(at + GROUPS);
+            const float rstd = rn_normalise<W, G, V>(x, there, inv, a.rms, a.eps, on, red, turn);
+            if (!live) {
 #pragma unroll
-                for (int i = 0; i < N; ++i) u[i] = 0.f;
+                for (int i = 0; i < N; ++i) x[i] = 0.f;
             }
-            float dy[BWD ? N : 1], dh[(BWD && NEXT) ? N : 1];
-            if constexpr (BWD) {
-                if (a.dy) rn_row<T, W, G, V>(a.dy, a.lddy, row, lane, a.C, on, dy);
-                else {
 #pragma unroll
-                    for (int i = 0; i < N; ++i) dy[i] = 0.f;
-                }
-                if constexpr (NEXT) rn_row<T, W, G, V>(a.dh, a.lddh, row, lane, a.C, on, dh);
-            }
-            const float rstd = rn_normalise<W, G, V>(x, lane, a.C, a.rms, a.eps, red, turn);
-#pragma unroll
-            for (int i = 0; i < N; ++i) u[i] = live ? u[i] + f[i] * (x[i] * w[i] + b[i]) : u[i];
+            for (int i = 0; i < N; ++i) u[i] = __builtin_fmaf(fw[i], x[i], u[i] + fb[i]);
             if constexpr (!BWD) {
+                if (a.act == ACT_GELU) {
 #pragma unroll
-                for (int i = 0; i < N; ++i) u[i] = act_fwd(u[i], a.act);
+                    for (int i = 0; i < N; ++i) {
+                        float slope;
+                        rn_gelu(u[i], u[i], slope);
+                    }
+                } else if (a.act == ACT_RELU) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) u[i] = act_fwd(u[i], ACT_RELU);
+                }
                 if (a.y) rn_put<T, W, G, V>(a.y, a.ldy, row, lane, a.C, on, u);
                 if constexpr (NEXT) {
-                    rn_normalise<W, G, V>(u, lane, a.C, a.rms, a.eps2, red, turn);
+                    rn_normalise<W, G, V>(u, there, inv, a.rms, a.eps2, on, red, turn);
 #pragma unroll
-                    for (int i = 0; i < N; ++i) u[i] = u[i] * w2[i] + b2[i];
+                    for (int i = 0; i < N; ++i) u[i] = __builtin_fmaf(u[i], w2[i], b2[i]);
                     rn_put<T, W, G, V>(a.h, a.ldh, row, lane, a.C, on, u);
                 }
             } else {
                 float slope[N];
+                if (a.act == ACT_GELU) {
 #pragma unroll
-                for (int i = 0; i < N; ++i) act_fwd_grad(u[i], a.act, &u[i], &slope[i]);
+                    for (int i = 0; i < N; ++i) rn_gelu(u[i], u[i], slope[i]);
+                } else if (a.act == ACT_RELU) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) act_fwd_grad(u[i], ACT_RELU, &u[i], &slope[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) slope[i] = 1.f;
+                }
                 if constexpr (NEXT) {
-                    const float rstd2 = rn_normalise<W, G, V>(u, lane, a.C, a.rms, a.eps2, red, turn);
+                    const float rstd2 = rn_normalise<W, G, V>(u, there, inv, a.rms, a.eps2, on, red, turn);
                     float d[N];
 #pragma unroll
                     for (int i = 0; i < N; ++i) {
-                        sums[2][i] += dh[i];
-                        sums[3][i] += on ? dh[i] * u[i] : 0.f;
-                        d[i] = dh[i] * w2[i];
+                        sums[2][i] += h[i];
+                        sums[3][i] = __builtin_fmaf(h[i], u[i], sums[3][i]);
+                        d[i] = h[i] * w2[i];
                     }
-                    rn_norm_grad<W, G, V>(d, u, rstd2, a.C, a.rms, red, turn);
+                    rn_norm_grad<W, G, V>(d, u, rstd2, inv, a.rms, red, turn);
 #pragma unroll
-                    for (int i = 0; i < N; ++i) dy[i] += d[i];
+                    for (int i = 0; i < N; ++i) g[i] += d[i];
                 }
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    dy[i] *= slope[i];
-                    sums[0][i] += on ? dy[i] : 0.f;
-                    sums[1][i] += on ? dy[i] * x[i] : 0.f;
+                    g[i] *= slope[i];
+                    sums[0][i] += g[i];
+                    sums[1][i] = __builtin_fmaf(g[i], x[i], sums[1][i]);
                 }
-                if (a.dr) rn_put<T, W, G, V>(a.dr, a.lddr, row, lane, a.C, on, dy);
+                if (a.dr) rn_put<T, W, G, V>(a.dr, a.lddr, row, lane, a.C, on, g);
                 if (a.dz) {
 #pragma unroll
-                    for (int i = 0; i < N; ++i) dy[i] *= f[i] * w[i];
-                    rn_norm_grad<W, G, V>(dy, x, rstd, a.C, a.rms, red, turn);
-#pragma unroll
-                    for (int i = 0; i < N; ++i) dy[i] = live ? dy[i] : 0.f;
-                    rn_put<T, W, G, V>(a.dz, a.lddz, row, lane, a.C, on, dy);
+                    for (int i = 0; i < N; ++i) g[i] *= fw[i];
+                    rn_norm_grad<W, G, V>(g, x, live ? rstd : 0.f, inv, a.rms, red, turn);
+                    rn_put<T, W, G, V>(a.dz, a.lddz, row, lane, a.C, on, g);
                 }
             }
         }
@@ -292,7 +352,7 @@ __global__ __launch_bounds__(RN_THREADS) void k_rownorm(const RnArgs a) {
                     for (int c = threadIdx.x; c < a.C; c += RN_THREADS) {
                         float v = 0.f;
 #pragma unroll
-                        for (int g = 0; g < GROUPS; ++g) v += fold[g * (G * N) + c];
+                        for (int q = 0; q < GROUPS; ++q) v += fold[q * (G * N) + c];
                         out[(size_t)s * a.C + c] = v;
                     }
                 }
@@ -303,13 +363,24 @@ __global__ __launch_bounds__(RN_THREADS) void k_rownorm(const RnArgs a) {
     }
 }
 
-// ---- folds of the partial column sums: 32 channels x 32 slots at a time, in slot order per lane, lanes in order.
+// ---- folds of the partial column sums: 32 channels x 32 slots at a time, in slot order per lane, lanes in order.  Many runs are
+// folded to blocks of 64 slots first, whose sums lie by the same rule at block + plot.
 struct RnFold {
     const float *part, *w, *b, *gate, *keep, *scale;
     const int32_t* ptr;
-    float *plots, *dgate, *dw, *db, *dscale, *dw2, *db2;
+    float *blocks, *plots, *dgate, *dw, *db, *dscale, *dw2, *db2;
     int n, C, B, rows, sums, runs;
 };
+// first and last (exclusive) slot of plot p (B: the rows behind the last plot)
+__device__ __forceinline__ void rn_slots(const RnFold& a, int p, int& s0, int& s1) {
+    s0 = 0;
+    s1 = a.runs;
+    if (a.ptr) {
+        const int lo = p == 0 ? 0 : min(max(a.ptr[p], 0), a.n), hi = p == a.B ? a.n : min(max(a.ptr[p + 1], 0), a.n);
+        s0 = lo / a.rows + p;
+        s1 = hi > lo ? (hi - 1) / a.rows + p + 1 : s0;
+    }
+}
 
 __device__ __forceinline__ float rn_fold32(float v, float (*t)[33]) {
     const int c = threadIdx.x & 31, k = threadIdx.x >> 5;
@@ -333,21 +404,54 @@ __device__ __forceinline__ void rn_finish(const RnFold& a, int c, const float* s
     }
 }
 
-// per plot (blockIdx.y; B: the rows behind the last plot): the sum of its slots -> plots[p][sums][C] and the gate's gradient;
-// without plots straight to the parameter gradients
+// slots [64 y, 64 y + 64), plot by plot
+__global__ __launch_bounds__(1024) void k_rownorm_fold_slots(const RnFold a) {
+    __shared__ float t[32][33];
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5, first = blockIdx.y * 64;
+    int p = 0, s0, s1;
+    if (a.ptr) {      // the first plot that ends behind `first`
+        int hi = a.B;
+        while (p < hi) {
+            const int mid = (p + hi) >> 1;
+            rn_slots(a, mid, s0, s1);
+            if (s1 > first) hi = mid;
+            else p = mid + 1;
+        }
+    }
+    for (; p <= a.B; ++p) {
+        rn_slots(a, p, s0, s1);
+        if (s0 >= first + 64) return;
+        s0 = max(s0, first);
+        s1 = min(s1, first + 64);
+        if (s0 >= s1) continue;
+        for (int i = 0; i < a.sums; ++i) {
+            float v = 0.f;
+            if (c < a.C)
+                for (int s = s0 + k; s < s1; s += 32) v += a.part[((size_t)s * a.sums + i) * a.C + c];
+            v = rn_fold32(v, t);
+            if (k == 0 && c < a.C) a.blocks[((size_t)(blockIdx.y + p) * a.sums + i) * a.C + c] = v;
+        }
+    }
+}
+
+// per plot (blockIdx.y): the sum of its blocks, or slots -> plots[p][sums][C] and the gate's gradient; without plots straight to
+// the parameter gradients
 __global__ __launch_bounds__(1024) void k_rownorm_fold_plots(const RnFold a) {
     __shared__ float t[32][33];
     const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5, p = blockIdx.y;
-    int s0 = 0, s1 = a.runs;
-    if (a.ptr) {
-        const int lo = p == 0 ? 0 : min(max(a.ptr[p], 0), a.n), hi = p == a.B ? a.n : min(max(a.ptr[p + 1], 0), a.n);
-        s0 = lo / a.rows + p;
-        s1 = hi > lo ? (hi - 1) / a.rows + p + 1 : s0;
+    int s0, s1;
+    rn_slots(a, p, s0, s1);
+    const float* from = a.part;
+    if (a.blocks) {
+        from = a.blocks;
+        const bool any = s1 > s0;
+        s1 = any ? (s1 - 1) / 64 + p + 1 : 0;
+        s0 = any ? s0 / 64 + p : 0;
     }
     float v[4] = {0.f, 0.f, 0.f, 0.f};
     if (c < a.C)
         for (int s = s0 + k; s < s1; s += 32)
-            for (int i = 0; i < a.sums; ++i) v[i] += a.part[((size_t)s * a.sums + i) * a.C + c];
+            for (int i = 0; i < a.sums; ++i) v[i] += from[((size_t)s * a.sums + i) * a.C + c];
     for (int i = 0; i < a.sums; ++i) v[i] = rn_fold32(v[i], t);
     if (k || c >= a.C) return;
     if (!a.ptr) { rn_finish(a, c, v); return; }
@@ -373,8 +477,8 @@ __global__ __launch_bounds__(1024) void k_rownorm_fold(const RnFold a) {
 }
 
 // ---- host side
-// lanes a row gets and pieces a lane: as few lanes as hold the row with one piece each (more rows in flight, shorter sums), up
-// to four pieces of a whole wave, then the whole workgroup
+// lanes a row gets and pieces a lane: as few lanes as hold the row with one piece each (more rows in flight, shorter sums), then
+// 16 channels a lane of a whole wave, then the whole workgroup
 template <bool BWD, bool NEXT, typename T, int W>
 static void rn_launch(const RnArgs& a, int runs, hipStream_t st) {
 #define RN_GO(G, V)                                                                                         \
@@ -388,51 +492,57 @@ static void rn_launch(const RnArgs& a, int runs, hipStream_t st) {
     if (pieces <= 32) RN_GO(32, 1);
     if (pieces <= 64) RN_GO(64, 1);
     if (pieces <= 128) RN_GO(64, 2);
-    if (pieces <= 256) RN_GO(64, 4);
     if constexpr (W == 1) {
+        if (pieces <= 256) RN_GO(64, 4);
         if (pieces <= 512) RN_GO(64, 8);
         if (pieces <= 1024) RN_GO(256, 4);
         if (pieces <= 2048) RN_GO(256, 8);
         RN_GO(256, 16);
-    } else {
+    } else if constexpr (W == 4) {
+        if (pieces <= 256) RN_GO(64, 4);
         if (pieces <= 512) RN_GO(256, 2);
         RN_GO(256, 4);
+    } else {
+        if (pieces <= 256) RN_GO(256, 1);
+        RN_GO(256, 2);
     }
 #undef RN_GO
 }
 
-static int rn_groups(int C, bool vec) {
-    const int pieces = vec ? agb_cdiv(C, 4) : C;
-    if (pieces <= 8) return 32;
-    if (pieces <= 16) return 16;
-    if (pieces <= 32) return 8;
-    if (pieces <= (vec ? 256 : 512)) return 4;
-    return 1;
+// rows that a workgroup takes at once (the fewest over the layouts above: what a run is cut by does not depend on alignment)
+static int rn_groups(int C) {
+    const int lanes = agb_cdiv(C, 8);
+    return lanes <= 8 ? 32 : lanes <= 16 ? 16 : lanes <= 32 ? 8 : 4;
 }
 
-// rows of a run: at least four turns of the workgroup's groups, at most RN_RUNS runs
+// rows of a run: at most RN_RUNS runs, whole turns
 #define RN_RUNS 2048
 static int rn_rows(int n, int C) {
-    const int least = 4 * rn_groups(C, C % 4 == 0), even = agb_cdiv(n, RN_RUNS);
-    return even > least ? even : least;
+    const int groups = rn_groups(C);
+    return agb_cdiv(agb_cdiv(n > 0 ? n : 1, RN_RUNS), groups) * groups;
 }
+// (measured, 211000 x 64: 2048 slots folded at once 43 us, by blocks 5)
+static int rn_blocks(int runs, int B) { return runs > 128 ? agb_cdiv((long long)runs + B + 1, 64) : 0; }
 
-static bool rn_vec_ok(const RnArgs& a, int esize) {
-    if (a.C % 4) return false;
+template <typename T>
+static bool rn_vec_ok(const RnArgs& a) {
+    const int W = 16 / (int)sizeof(T);
+    if (a.C % W) return false;
     const void* p[] = {a.z, a.r, a.dy, a.dh, a.y, a.h, a.dz, a.dr};
     const long long ld[] = {a.ldz, a.ldr, a.lddy, a.lddh, a.ldy, a.ldh, a.lddz, a.lddr};
     for (int i = 0; i < 8; ++i)
-        if (p[i] && ((uintptr_t)p[i] % (4 * esize) || ld[i] % 4)) return false;
+        if (p[i] && ((uintptr_t)p[i] % 16 || ld[i] % W)) return false;
     return true;
 }
 
 template <typename T>
 static int rn_run(const RnArgs& a, bool bwd, hipStream_t st) {
     const int runs = agb_cdiv(a.n, a.rows);
-    const bool vec = rn_vec_ok(a, sizeof(T));
+    const bool vec = rn_vec_ok<T>(a);
+    constexpr int W = 16 / sizeof(T);
 #define RN_DIR(BWD, NEXT)                                       \
     do {                                                        \
-        if (vec) rn_launch<BWD, NEXT, T, 4>(a, runs, st);       \
+        if (vec) rn_launch<BWD, NEXT, T, W>(a, runs, st);       \
         else rn_launch<BWD, NEXT, T, 1>(a, runs, st);           \
     } while (0)
     if (bwd) {
@@ -478,8 +588,9 @@ int agb_rownorm_fwd(const void* Z, long long ldz, const void* R, long long ldr, 
 
 size_t agb_rownorm_bwd_workspace_bytes(int n, int C, int B, int next) {
     if (n < 0 || C < 1 || C > RN_MAX_C || B < 0) return 0;
-    const size_t slots = (size_t)agb_cdiv(n, rn_rows(n, C)) + B + 1;
-    return (slots + B + 1) * (next ? 4 : 2) * (size_t)C * sizeof(float);
+    const int runs = agb_cdiv(n, rn_rows(n, C)), blocks = rn_blocks(runs, B);
+    const size_t slots = (size_t)runs + B + 1, more = blocks ? (size_t)blocks + B + 1 : 0;
+    return (slots + more + B + 1) * (next ? 4 : 2) * (size_t)C * sizeof(float);
 }
 
 int agb_rownorm_bwd(const void* Z, long long ldz, const void* R, long long ldr, const void* dY, long long lddy, const void* dH,
@@ -516,8 +627,17 @@ int agb_rownorm_bwd(const void* Z, long long ldz, const void* R, long long ldr, 
     RnFold f = {};
     f.part = a.part; f.w = w; f.b = b; f.gate = gate; f.keep = keep; f.scale = scale; f.ptr = ptr;
     f.n = n; f.C = C; f.B = ptr ? B : 0; f.rows = a.rows; f.sums = a.next ? 4 : 2; f.runs = agb_cdiv(n, a.rows);
+    const int blocks = rn_blocks(f.runs, f.B);
     f.plots = a.part + ((size_t)f.runs + f.B + 1) * f.sums * C;
+    if (blocks) {
+        f.blocks = f.plots;
+        f.plots = f.blocks + ((size_t)blocks + f.B + 1) * f.sums * C;
+    }
     f.dw = dw; f.db = db; f.dgate = dgate; f.dscale = dscale; f.dw2 = dw2; f.db2 = db2;
+    if (blocks) {
+        hipLaunchKernelGGL(k_rownorm_fold_slots, dim3(agb_cdiv(C, 32), blocks), dim3(1024), 0, st, f);
+        AGB_CHECK_LAUNCH("agb_rownorm_fold_slots");
+    }
     hipLaunchKernelGGL(k_rownorm_fold_plots, dim3(agb_cdiv(C, 32), ptr ? B + 1 : 1), dim3(1024), 0, st, f);
     AGB_CHECK_LAUNCH("agb_rownorm_fold_plots");
     if (ptr && (dw || db || dscale || dw2 || db2)) {
