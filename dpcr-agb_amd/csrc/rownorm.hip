@@ -125,16 +125,33 @@ __device__ __forceinline__ void rn_put(void* base, long long ld, long long row, 
         if (on && c < C) RnPiece<T, W>::put(p + c, v + j * W);
     }
 }
-// a parameter vector's values: `other` where there is none, 0 behind the last channel
+// a parameter vector's values: `other` where there is none, 0 behind the last channel.  No branch between the loads: all are in
+// flight together (a load, a branch and a use at a time they were most of a short call's time).
+struct __attribute__((packed, aligned(4))) RnFour {
+    float v[4];
+};
 template <int W, int G, int V>
 __device__ __forceinline__ void rn_vec(const float* p, int lane, int C, float other, float* v) {
 #pragma unroll
-    for (int j = 0; j < V; ++j)
+    for (int i = 0; i < V * W; ++i) v[i] = other;
+    if (p) {
 #pragma unroll
-        for (int e = 0; e < W; ++e) {
-            const int c = (j * G + lane) * W + e;
-            v[j * W + e] = c < C ? (p ? p[c] : other) : 0.f;
+        for (int j = 0; j < V; ++j) {
+            const float* q = p + min((j * G + lane) * W, C - W);      // (W > 1: C is a multiple of W)
+            if constexpr (W == 1) {
+                v[j] = *q;
+            } else {
+#pragma unroll
+                for (int e = 0; e < W; e += 4) {
+                    const RnFour f = *(const RnFour*)(q + e);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[j * W + e + i] = f.v[i];
+                }
+            }
         }
+    }
+#pragma unroll
+    for (int i = 0; i < V * W; ++i) v[i] = ((i / W) * G + lane) * W < C ? v[i] : 0.f;
 }
 
 // x <- xhat in place, returns rstd; 0 for both where `on` is false.  there[j]: 1 for a piece of channels, 0 behind the last
@@ -185,31 +202,30 @@ __device__ __forceinline__ void rn_gelu(float u, float& y, float& slope) {
     slope = __builtin_fmaf(u * 0.39894228f, e, cdf);
 }
 
-// the plot of a row: how many of ptr[1 .. B] are <= row (B: behind the last plot)
+// the plot of a row: how many of ptr[1 .. B] are <= row (B: behind the last plot), 64 looks at once
 __device__ __forceinline__ int rn_plot(const int32_t* ptr, int B, int row) {
-    int lo = 0, hi = B;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (ptr[mid + 1] <= row) lo = mid + 1;
-        else hi = mid;
+    int p = 0;
+    for (int base = 0; base < B; base += 64) {
+        const int i = base + (threadIdx.x & 63);
+        p += __popcll(__ballot(i < B && ptr[min(i, B - 1) + 1] <= row));
     }
-    return lo;
+    return __builtin_amdgcn_readfirstlane(p);
 }
 
 // f w and f b with f = keep[p] gate[p] scale of plot p; 0 behind the last plot (such a row is handed on as act(r))
 template <int W, int G, int V>
 __device__ __forceinline__ void rn_factor(const RnArgs& a, int p, int lane, float* fw, float* fb) {
     const float k = !a.ptr ? 1.f : p >= a.B ? 0.f : a.keep ? a.keep[p] : 1.f;
+    float scale[V * W], gate[V * W];
+    rn_vec<W, G, V>(a.w, lane, a.C, 1.f, fw);
+    rn_vec<W, G, V>(a.b, lane, a.C, 0.f, fb);
+    rn_vec<W, G, V>(a.scale, lane, a.C, 1.f, scale);
+    rn_vec<W, G, V>(a.gate && p < a.B ? a.gate + (size_t)p * a.C : nullptr, lane, a.C, 1.f, gate);
 #pragma unroll
     for (int i = 0; i < V * W; ++i) {
-        const int c = ((i / W) * G + lane) * W + i % W;
-        float f = c < a.C ? k : 0.f;
-        if (c < a.C) {
-            if (a.scale) f *= a.scale[c];
-            if (a.gate && p < a.B) f *= a.gate[(size_t)p * a.C + c];
-        }
-        fw[i] = f * (a.w && c < a.C ? a.w[c] : 1.f);
-        fb[i] = f * (a.b && c < a.C ? a.b[c] : 0.f);
+        const float f = k * scale[i] * gate[i];
+        fw[i] *= f;
+        fb[i] *= f;
     }
 }
 
@@ -234,13 +250,9 @@ __global__ __launch_bounds__(RN_THREADS) void k_rownorm(const RnArgs a) {
         if constexpr (!BWD) rn_vec<W, G, V>(a.b2, lane, a.C, 0.f, b2);
     }
     int row0 = first;
-    int p = a.ptr ? rn_plot(a.ptr, a.B, first) : 0;
     while (row0 < last) {
-        int end = last;
-        if (a.ptr) {
-            while (p < a.B && a.ptr[p + 1] <= row0) ++p;
-            if (p < a.B) end = min(last, a.ptr[p + 1]);
-        }
+        const int p = a.ptr ? rn_plot(a.ptr, a.B, row0) : 0;
+        const int end = a.ptr && p < a.B ? min(last, a.ptr[p + 1]) : last;
         const bool live = !a.ptr || p < a.B;      // (rows behind the last plot: y = act(r), dz = 0 whatever z holds)
         float fw[N], fb[N], sums[BWD ? SUMS : 1][N];
         rn_factor<W, G, V>(a, p, lane, fw, fb);
@@ -409,15 +421,12 @@ __global__ __launch_bounds__(1024) void k_rownorm_fold_slots(const RnFold a) {
     __shared__ float t[32][33];
     const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5, first = blockIdx.y * 64;
     int p = 0, s0, s1;
-    if (a.ptr) {      // the first plot that ends behind `first`
-        int hi = a.B;
-        while (p < hi) {
-            const int mid = (p + hi) >> 1;
-            rn_slots(a, mid, s0, s1);
-            if (s1 > first) hi = mid;
-            else p = mid + 1;
-        }
+    for (int base = 0; a.ptr && base <= a.B; base += 64) {      // the first plot that ends behind `first`, 64 looks at once
+        const int i = base + (threadIdx.x & 63);
+        rn_slots(a, min(i, a.B), s0, s1);
+        p += __popcll(__ballot(i <= a.B && s1 <= first));
     }
+    p = __builtin_amdgcn_readfirstlane(p);
     for (; p <= a.B; ++p) {
         rn_slots(a, p, s0, s1);
         if (s0 >= first + 64) return;
