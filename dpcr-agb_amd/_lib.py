@@ -173,6 +173,10 @@ def stream():
     return torch.cuda.current_stream().cuda_stream
 
 
+def current_device():
+    return _cur_device() if _cur_device is not None else torch.cuda.current_device()
+
+
 _FN = {}     # entry point name -> ctypes function (one dictionary lookup per launch instead of load() + getattr)
 # An input pipeline that reads counts back asynchronously (instance/kpconv.py: the wait-free input pyramid) registers a
 # callable here: it is given a turn every POLL_EVERY library calls — i.e. every ~0.5 ms while a step is being enqueued —
@@ -203,11 +207,16 @@ def last_kernel():
     return load().agb_last_kernel().decode()
 
 
+_SIZE_FN = {}
+
+
 def size_call(name, *args):
     """Host helper that returns a byte count (size_t), e.g. the *_workspace_bytes functions."""
-    fn = getattr(load(), name)
-    fn.restype = ctypes.c_size_t
-    return int(fn(*args))
+    fn = _SIZE_FN.get(name)
+    if fn is None:
+        fn = _SIZE_FN[name] = getattr(load(), name)
+        fn.restype = ctypes.c_size_t
+    return fn(*args)
 
 
 def hash_capacity(n):

@@ -57,8 +57,9 @@ struct __attribute__((aligned(16))) NsMat {
     int rows, cols, batch, type;      // type of `in` (and of `out` where nothing is updated): 0 fp32, 1 bf16, 2 fp16
     int k, n, kp, np, tall;
     int vec, out_vec;                 // input contiguous and aligned: four elements at a time; output rows aligned: eight
-    int tile, kt, nt, tri, splits, chunk;      // tile of G and X; tiles along k and n; tiles on and above the diagonal
+    int tile, kt, tri, splits, chunk;          // tile of G: along k, on and above the diagonal; chunks of n
     int tile_p, kt_p, tri_p;                   // tile of P
+    int tile_x, kt_x, nt_x;                    // tile of X
     int sums;                                  // partial sums of squares per matrix
     float step;
     ghalf *xt0, *xt1, *g, *p;                  // planes of matrix 0 of the stack
@@ -94,13 +95,13 @@ enum { NS_SQUARES, NS_PLANES, NS_GRAM, NS_APPLY, NS_POLY, NS_FOLD, NS_RESIDENT, 
 // (The descriptor is copied whole, by scalar loads in one go.)
 typedef const __attribute__((address_space(4))) NsMat* NsTab;
 template <int WHICH>
-__device__ __forceinline__ NsMat ns_find(NsTab tab, int count) {
+__device__ __forceinline__ NsMat ns_find(NsTab tab, int count, int wg) {
     int found = 0;
     if (count > 1) {
         found = -1;
         for (int base = 0; base < count; base += 64) {
             const int i = base + (threadIdx.x & 63);
-            found += __popcll(__ballot(i < count && tab[min(i, count - 1)].at[WHICH] <= (int)blockIdx.x));
+            found += __popcll(__ballot(i < count && tab[min(i, count - 1)].at[WHICH] <= wg));
         }
         found = __builtin_amdgcn_readfirstlane(found);
     }
@@ -150,49 +151,57 @@ __device__ __forceinline__ float ns_clip(float g, float clip) {      // (NaN sta
 
 // sums of squares in 64 bits (neither huge nor tiny entries leave the range), and the momentum's update
 __global__ __launch_bounds__(NS_THREADS) void k_ns_squares(const NsMat* tab, int count, const NsUpdate up) {
-    const NsMat m = ns_find<NS_SQUARES>((NsTab)tab, count);
+    const NsMat m = ns_find<NS_SQUARES>((NsTab)tab, count, blockIdx.x);
     const int at = blockIdx.x - m.at[NS_SQUARES], b = at / m.sums, part = at % m.sums;
     const long long total = (long long)m.rows * m.cols, first = (long long)part * NS_CHUNK;
     const long long last = first + NS_CHUNK < total ? first + NS_CHUNK : total;
     const bool linear = m.in_ld == m.cols;
     const long long base = b * m.in_bs;
-    double s = 0;
-    for (long long i0 = first + threadIdx.x * 4; i0 < last; i0 += NS_THREADS * 4) {
-        float v[4], mom[4];
-        const bool whole = m.vec && i0 + 4 <= last;
-        if (whole) {
-            ns_in4(m, base + i0, v);
+    // (all of a thread's loads first)
+    constexpr int TURNS = NS_CHUNK / (4 * NS_THREADS);
+    float v[TURNS][4], mom[TURNS][4];
+#pragma unroll
+    for (int l = 0; l < TURNS; ++l) {
+        const long long i0 = first + (l * NS_THREADS + threadIdx.x) * 4;
+        if (m.vec && i0 + 4 <= last) {
+            ns_in4(m, base + i0, v[l]);
             if (up.on) {
                 const f32x4 q = *(const gfloat4*)(m.mom + i0);
-                mom[0] = q.x; mom[1] = q.y; mom[2] = q.z; mom[3] = q.w;
+                mom[l][0] = q.x; mom[l][1] = q.y; mom[l][2] = q.z; mom[l][3] = q.w;
             }
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const long long i = i0 + e;
-                v[e] = mom[e] = 0.f;
-                if (i >= last) continue;
-                v[e] = ns_in(m, linear ? base + i : base + i / m.cols * m.in_ld + i % m.cols);
-                if (up.on) mom[e] = m.mom[i];
+                v[l][e] = mom[l][e] = 0.f;
+                if (i < last) {
+                    v[l][e] = ns_in(m, linear ? base + i : base + i / m.cols * m.in_ld + i % m.cols);
+                    if (up.on) mom[l][e] = m.mom[i];
+                }
             }
         }
+    }
+    double s = 0;
+#pragma unroll
+    for (int l = 0; l < TURNS; ++l) {
+        const long long i0 = first + (l * NS_THREADS + threadIdx.x) * 4;
         if (up.on) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                v[e] = ns_clip(v[e], up.clip);
-                mom[e] = mom[e] * up.mu + v[e] * up.omu;
-                v[e] = up.nesterov ? v[e] * up.omu + mom[e] * up.mu : mom[e];
+                v[l][e] = ns_clip(v[l][e], up.clip);
+                mom[l][e] = mom[l][e] * up.mu + v[l][e] * up.omu;
+                v[l][e] = up.nesterov ? v[l][e] * up.omu + mom[l][e] * up.mu : mom[l][e];
             }
-            if (whole) {
-                *(gfloat4*)(m.mom + i0) = f32x4{mom[0], mom[1], mom[2], mom[3]};
+            if (m.vec && i0 + 4 <= last) {
+                *(gfloat4*)(m.mom + i0) = f32x4{mom[l][0], mom[l][1], mom[l][2], mom[l][3]};
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (i0 + e < last) m.mom[i0 + e] = mom[e];
+                    if (i0 + e < last) m.mom[i0 + e] = mom[l][e];
             }
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s += (double)v[e] * v[e];
+        for (int e = 0; e < 4; ++e) s += (double)v[l][e] * v[l][e];
     }
     __shared__ double red[NS_THREADS];
     red[threadIdx.x] = s;
@@ -206,7 +215,7 @@ __global__ __launch_bounds__(NS_THREADS) void k_ns_squares(const NsMat* tab, int
 
 // X = M / (|M| + eps) as plane pairs, 64 x 64 of [n][k] at a time
 __global__ __launch_bounds__(NS_THREADS) void k_ns_planes(const NsMat* tab, int count, const NsUpdate up, double eps) {
-    const NsMat m = ns_find<NS_PLANES>((NsTab)tab, count);
+    const NsMat m = ns_find<NS_PLANES>((NsTab)tab, count, blockIdx.x);
     const int kb = m.kp / 64, nb = m.np / 64;
     int at = blockIdx.x - m.at[NS_PLANES];
     const int b = at / (kb * nb);
@@ -214,6 +223,17 @@ __global__ __launch_bounds__(NS_THREADS) void k_ns_planes(const NsMat* tab, int 
     const int n0 = at / kb * 64, k0 = at % kb * 64;
     __shared__ double red[NS_THREADS];
     __shared__ float tile[64][65];
+    // rows of M along threadIdx / 64, columns along the lanes; all of a thread's loads first, from the last row or column where
+    // there is none
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int r0 = (m.tall ? n0 : k0) + wave, c = (m.tall ? k0 : n0) + lane;
+    float v[16], mom[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int r = min(r0 + 4 * i, m.rows - 1), q = min(c, m.cols - 1);
+        v[i] = ns_in(m, b * m.in_bs + r * m.in_ld + q);
+        if (up.on) mom[i] = m.mom[(size_t)r * m.cols + q];
+    }
     double s = 0;
     for (int i = threadIdx.x; i < m.sums; i += NS_THREADS) s += m.sq[(size_t)b * m.sums + i];
     red[threadIdx.x] = s;
@@ -223,32 +243,27 @@ __global__ __launch_bounds__(NS_THREADS) void k_ns_planes(const NsMat* tab, int 
         __syncthreads();
     }
     const double inverse = 1 / (sqrt(red[0]) + eps);      // (0 / 0, inf 0: NaN as by division)
-    // rows of M along threadIdx / 64, columns along the lanes; tile[n][k]
-    for (int i = threadIdx.x >> 6; i < 64; i += NS_THREADS / 64) {
-        const int j = threadIdx.x & 63;
-        const int r = (m.tall ? n0 : k0) + i, c = (m.tall ? k0 : n0) + j;
-        float v = 0.f;
-        if (r < m.rows && c < m.cols) {
-            v = ns_in(m, b * m.in_bs + r * m.in_ld + c);
-            if (up.on) {
-                v = ns_clip(v, up.clip);
-                const float mom = m.mom[(size_t)r * m.cols + c];
-                v = up.nesterov ? v * up.omu + mom * up.mu : mom;
-            }
-            v = (float)(v * inverse) * NS_SCALE;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int j = wave + 4 * i;
+        float x = v[i];
+        if (up.on) {
+            x = ns_clip(x, up.clip);
+            x = up.nesterov ? x * up.omu + mom[i] * up.mu : mom[i];
         }
-        if (m.tall) tile[i][j] = v;
-        else tile[j][i] = v;
+        x = r0 + 4 * i < m.rows && c < m.cols ? (float)(x * inverse) * NS_SCALE : 0.f;
+        if (m.tall) tile[j][lane] = x;
+        else tile[lane][j] = x;
     }
     __syncthreads();
     ghalf* xt = m.xt0 + (size_t)b * m.np * m.kp * 2;
     for (int q = threadIdx.x; q < 512; q += NS_THREADS) {
         const int row = q >> 2 & 63, col = (q & 3) * 8 + (q >> 8) * 32;
-        float v[8];
+        float x[8];
         half8 hi, lo;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = tile[row][col + e];
-        ns_split8(v, hi, lo);
+        for (int e = 0; e < 8; ++e) x[e] = tile[row][col + e];
+        ns_split8(x, hi, lo);
         const size_t o = ns_at(n0 + row, k0 + col, m.np);
         *(ghalf8*)(xt + o) = hi;
         *(ghalf8*)(xt + o + 32) = lo;
@@ -592,11 +607,15 @@ __device__ __forceinline__ void ns_gram(const NsMat& m, int from, char* lds) {
             }
     }
 }
+// (WIDE: some tile is 128 x 128.  Without, half the registers: two workgroups a CU.)
+template <bool WIDE>
 __global__ __launch_bounds__(NS_WIDE) void k_ns_gram(const NsMat* tab, int count, int from) {
     extern __shared__ __align__(16) char lds[];
-    const NsMat m = ns_find<NS_GRAM>((NsTab)tab, count);
-    if (m.tile == 128) ns_gram<128>(m, from, lds);
-    else ns_gram<64>(m, from, lds);
+    const NsMat m = ns_find<NS_GRAM>((NsTab)tab, count, blockIdx.x);
+    if constexpr (WIDE) {
+        if (m.tile == 128) return ns_gram<128>(m, from, lds);
+    }
+    ns_gram<64>(m, from, lds);
 }
 
 // the chunks' sums in order, a unit of a tile
@@ -626,7 +645,7 @@ __device__ __forceinline__ void ns_fold(const NsMat& m, float* unit) {
     ns_symmetric<Tile::UC, NS_THREADS>(m.g + (size_t)b * m.kp * m.kp * 2, m.kp, j * T + row, i * T + col, i == j, unit, threadIdx.x);
 }
 __global__ __launch_bounds__(NS_THREADS) void k_ns_fold(const NsMat* tab, int count) {
-    const NsMat m = ns_find<NS_FOLD>((NsTab)tab, count);
+    const NsMat m = ns_find<NS_FOLD>((NsTab)tab, count, blockIdx.x);
     __shared__ __align__(16) float unit[32 * 68];
     if (m.tile == 128) ns_fold<128>(m, unit);
     else ns_fold<64>(m, unit);
@@ -670,11 +689,14 @@ __device__ __forceinline__ void ns_poly(const NsMat& m, float cb, float cc, char
     __builtin_amdgcn_wave_barrier();
     ns_symmetric<Tile::UC, 64>(m.p + (size_t)b * m.kp * m.kp * 2, m.kp, r0, c0, i == j, mine, lane);
 }
+template <bool WIDE>
 __global__ __launch_bounds__(NS_WIDE) void k_ns_poly(const NsMat* tab, int count, float cb, float cc) {
     extern __shared__ __align__(16) char lds[];
-    const NsMat m = ns_find<NS_POLY>((NsTab)tab, count);
-    if (m.tile_p == 128) ns_poly<128>(m, cb, cc, lds);
-    else ns_poly<64>(m, cb, cc, lds);
+    const NsMat m = ns_find<NS_POLY>((NsTab)tab, count, blockIdx.x);
+    if constexpr (WIDE) {
+        if (m.tile_p == 128) return ns_poly<128>(m, cb, cc, lds);
+    }
+    ns_poly<64>(m, cb, cc, lds);
 }
 
 // two values as 16-bit ones
@@ -719,17 +741,17 @@ __device__ __forceinline__ void ns_out8(const NsMat& m, const NsUpdate& up, int 
 
 // X <- a X + X P
 template <int T>
-__device__ __forceinline__ void ns_apply(const NsMat& m, int from, float ca, bool last, const NsUpdate& up, char* lds) {
+__device__ __forceinline__ void ns_apply(const NsMat& m, int wg, int from, float ca, bool last, const NsUpdate& up, char* lds) {
     typedef NsTile<T, false> Tile;
-    int at = ns_order(blockIdx.x - m.at[NS_APPLY], m.nt * m.kt * m.batch);
-    const int b = at / (m.nt * m.kt);
-    at %= m.nt * m.kt;
+    int at = ns_order(wg - m.at[NS_APPLY], m.nt_x * m.kt_x * m.batch);
+    const int b = at / (m.nt_x * m.kt_x);
+    at %= m.nt_x * m.kt_x;
     const size_t plane = (size_t)b * m.np * m.kp * 2;
     const ghalf* x = (from ? m.xt1 : m.xt0) + plane;
     ghalf* out = (from ? m.xt0 : m.xt1) + plane;
     Tile t;
-    t.run(m.p + (size_t)b * m.kp * m.kp * 2, at % m.kt * T, m.kp, x, at / m.kt * T, m.np, m.kp, 0, m.kp, lds);
-    const int lane = threadIdx.x & 63, n0 = at / m.kt * T + t.unit_row(), k0 = at % m.kt * T + t.unit_col();
+    t.run(m.p + (size_t)b * m.kp * m.kp * 2, at % m.kt_x * T, m.kp, x, at / m.kt_x * T, m.np, m.kp, 0, m.kp, lds);
+    const int lane = threadIdx.x & 63, n0 = at / m.kt_x * T + t.unit_row(), k0 = at % m.kt_x * T + t.unit_col();
     constexpr int EACH = Tile::UC / 16;
     half8 xh[EACH], xl[EACH];
     int row, col;
@@ -769,14 +791,6 @@ __device__ __forceinline__ void ns_apply(const NsMat& m, int from, float ca, boo
         ns_out8(m, up, b, k0 + col, n0 + row, v);
     }
 }
-__global__ __launch_bounds__(NS_WIDE) void k_ns_apply(const NsMat* tab, int count, int from, float ca, int last,
-                                                      const NsUpdate up) {
-    extern __shared__ __align__(16) char lds[];
-    const NsMat m = ns_find<NS_APPLY>((NsTab)tab, count);
-    if (m.tile == 128) ns_apply<128>(m, from, ca, last, up, lds);
-    else ns_apply<64>(m, from, ca, last, up, lds);
-}
-
 // ---- small matrices: everything in one workgroup, X, G and P in LDS (one launch instead of 17)
 // kp = 64 with np <= 256, or kp = np = 128.  Products by 16 x 16 blocks of the result spread over eight waves: what an iteration
 // takes is latency — the products' chains, the splitting of what they leave, five meetings — and small blocks shorten each.
@@ -1077,31 +1091,65 @@ __device__ __forceinline__ void ns_resident(const NsMat& m, int b, const NsUpdat
         }
     }
 }
-__global__ __launch_bounds__(NS_WIDE) void k_ns_resident(const NsTable args, const NsMat* tab, int count, const NsUpdate up, double eps,
-                                                         const NsCoef coef, int steps) {
-    extern __shared__ __align__(16) char lds[];
+__device__ __forceinline__ void ns_resident_any(const NsMat& m, int b, const NsUpdate& up, double eps, const NsCoef& coef, int steps,
+                                                char* lds) {
     __shared__ double red[8];
     __shared__ float abc[3 * NS_MAX_STEPS];
-    // (a list that fits travels in the arguments alone; those are far away: everything is read at once, at the start)
-    const NsMat m = ns_find<NS_RESIDENT>(tab ? (NsTab)tab : (NsTab)__builtin_amdgcn_kernarg_segment_ptr(), count);
     if ((int)threadIdx.x < 3 * steps) abc[threadIdx.x] = coef.v[threadIdx.x];
-    const int b = blockIdx.x - m.at[NS_RESIDENT];
     if (m.kp == 128) ns_resident<128, 128>(m, b, up, eps, abc, steps, lds, red);
     else if (m.np == 64) ns_resident<64, 64>(m, b, up, eps, abc, steps, lds, red);
     else if (m.np == 128) ns_resident<64, 128>(m, b, up, eps, abc, steps, lds, red);
     else if (m.np == 192) ns_resident<64, 192>(m, b, up, eps, abc, steps, lds, red);
     else ns_resident<64, 256>(m, b, up, eps, abc, steps, lds, red);
 }
+__global__ __launch_bounds__(NS_WIDE) void k_ns_resident(const NsTable args, const NsMat* tab, int count, const NsUpdate up, double eps,
+                                                         const NsCoef coef, int steps) {
+    extern __shared__ __align__(16) char lds[];
+    // (a list that fits travels in the arguments alone; those are far away: everything is read at once, at the start)
+    const NsMat m = ns_find<NS_RESIDENT>(tab ? (NsTab)tab : (NsTab)__builtin_amdgcn_kernarg_segment_ptr(), count, blockIdx.x);
+    ns_resident_any(m, blockIdx.x - m.at[NS_RESIDENT], up, eps, coef, steps, lds);
+}
+
+template <bool WIDE>
+__device__ __forceinline__ void ns_apply_any(const NsMat& m, int wg, int from, float ca, bool last, const NsUpdate& up, char* lds) {
+    if constexpr (WIDE) {
+        if (m.tile_x == 128) return ns_apply<128>(m, wg, from, ca, last, up, lds);
+    }
+    ns_apply<64>(m, wg, from, ca, last, up, lds);
+}
+template <bool WIDE>
+__global__ __launch_bounds__(NS_WIDE) void k_ns_apply(const NsMat* tab, int count, int from, float ca, int last,
+                                                      const NsUpdate up) {
+    extern __shared__ __align__(16) char lds[];
+    const NsMat m = ns_find<NS_APPLY>((NsTab)tab, count, blockIdx.x);
+    ns_apply_any<WIDE>(m, blockIdx.x, from, ca, last, up, lds);
+}
+// The last step of a list that also has matrices that are taken whole: those, by the first workgroups, beside the others' tiles
+// (SENet14: seven such matrices take 60 us, on seven CUs).
+template <bool WIDE>
+__global__ __launch_bounds__(NS_WIDE) void k_ns_last(const NsMat* tab, int count, int from, float ca, const NsUpdate up, int whole,
+                                                     double eps, const NsCoef coef, int steps) {
+    extern __shared__ __align__(16) char lds[];
+    if ((int)blockIdx.x < whole) {
+        const NsMat m = ns_find<NS_RESIDENT>((NsTab)tab, count, blockIdx.x);
+        ns_resident_any(m, blockIdx.x - m.at[NS_RESIDENT], up, eps, coef, steps, lds);
+    } else {
+        const int wg = blockIdx.x - whole;
+        const NsMat m = ns_find<NS_APPLY>((NsTab)tab, count, wg);
+        ns_apply_any<WIDE>(m, wg, from, ca, true, up, lds);
+    }
+}
 
 // ---- host side
 // fields of a matrix stack in the callers' table (int64 each)
 enum { NS_IN, NS_OUT, NS_MOM, NS_ROWS, NS_COLS, NS_BATCH, NS_IN_LD, NS_IN_BS, NS_OUT_LD, NS_OUT_BS, NS_TYPE, NS_FIELDS };
 #define NS_MAX_SIDE (1 << 24)
+#define NS_HALF_DEVICE 160
 
 struct NsPlan {
     size_t bytes;
     int grid[NS_LAUNCHES];
-    bool wide, wide_p;      // a tile of 128 among those of G and X; of P
+    bool wide, wide_p, wide_x;      // a tile of 128 among those of G, P, X
     int lds;                // bytes of the largest matrix that is taken whole
 };
 
@@ -1121,17 +1169,30 @@ static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
     if (m.k > 16384) return false;
     m.kp = agb_cdiv(m.k, 64) * 64;
     m.np = agb_cdiv(m.n, 64) * 64;
+    // Products: a workgroup of T = 128 (one a CU) takes about 6 us and 0.65 us for each 32 of the sum, one of T = 64 (two a CU)
+    // 5 and 0.25 (measured).  T = 128 where its tiles fill half of the device.
+    auto tiles_of = [](long long down, long long across, int T, int batch) { return agb_cdiv(down, T) * (long long)agb_cdiv(across, T) * batch; };
+    m.tile_x = m.kp >= 256 && tiles_of(m.np, m.kp, 128, m.batch) >= NS_HALF_DEVICE ? 128 : 64;
+    m.kt_x = agb_cdiv(m.kp, m.tile_x);
+    m.nt_x = agb_cdiv(m.np, m.tile_x);
     m.tile = m.kp >= 256 ? 128 : 64;
     m.kt = agb_cdiv(m.kp, m.tile);
-    m.nt = agb_cdiv(m.np, m.tile);
     m.tri = m.kt * (m.kt + 1) / 2;
     const long long tiles = (long long)m.tri * m.batch;
-    // G: enough chunks of n for a workgroup per CU, none shorter than eight steps.  (By the matrix alone: what else is in the
-    // list does not change a result.)
-    int splits = tiles >= 256 ? 1 : agb_cdiv(256, tiles);
-    if (splits > m.np / 512) splits = m.np / 512;
-    if (splits < 1) splits = 1;
-    m.chunk = agb_cdiv(agb_cdiv(m.np, splits), 64) * 64;
+    // G: the number of chunks of n that takes least by those figures, with 6 us for the fold that more than one needs; none
+    // shorter than 512.  (By the matrix alone: what else is in the list does not change a result.)
+    double best = 1e30;
+    m.chunk = m.np;
+    for (int splits = 1; splits <= 64 && (splits == 1 || m.np / splits >= 512); ++splits) {
+        const int chunk = agb_cdiv(agb_cdiv(m.np, splits), 64) * 64, real = agb_cdiv(m.np, chunk);
+        const double wgs = (double)tiles * real, slots = m.tile == 128 ? 256 : 512;
+        const double rounds = wgs <= slots ? 1 : (double)agb_cdiv((long long)wgs, (long long)slots);
+        const double us = rounds * (m.tile == 128 ? 6 + chunk * (0.65 / 32) : 5 + chunk * (0.25 / 32)) + (real > 1 ? 6 + wgs * 0.01 : 0);
+        if (us < best) {
+            best = us;
+            m.chunk = chunk;
+        }
+    }
     m.splits = agb_cdiv(m.np, m.chunk);
     // P: k products a sum and few tiles: 64 x 64 as long as those fit the device twice
     const int k64 = m.kp / 64;
@@ -1146,6 +1207,7 @@ static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
         if (lds > plan.lds) plan.lds = lds;
     } else {
         plan.wide |= m.tile == 128;
+        plan.wide_x |= m.tile_x == 128;
         plan.wide_p |= m.tile_p == 128;
     }
     const size_t x = whole ? 0 : (size_t)m.np * m.kp * 4 * batch, g = whole ? 0 : (size_t)m.kp * m.kp * 4 * batch;
@@ -1162,7 +1224,7 @@ static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
     m.sq = (gdouble*)take(whole ? 0 : (size_t)m.sums * batch * 8);
     const long long units = m.tile == 128 ? 8 : 4;
     const long long wgs[NS_LAUNCHES] = {(long long)m.sums * batch, (long long)(m.kp / 64) * (m.np / 64) * batch, tiles * m.splits,
-                                        (long long)m.kt * m.nt * batch, (long long)m.tri_p * batch,
+                                        (long long)m.kt_x * m.nt_x * batch, (long long)m.tri_p * batch,
                                         m.splits > 1 ? tiles * units : 0, batch};
     for (int i = 0; i < NS_LAUNCHES; ++i) {
         m.at[i] = plan.grid[i];
@@ -1231,30 +1293,47 @@ static int ns_run(const char* name, const long long* fields, int count, int step
         else hipLaunchKernelGGL(k_ns_table, dim3(1), dim3(256), 0, st, t, (u32x4*)(tab + base), (int)(some * sizeof(NsMat) / 16));
     }
     const int* grid = plan.grid;
-    if (grid[NS_RESIDENT]) {
+    NsCoef all = {};
+    for (int i = 0; i < 3 * steps; ++i) all.v[i] = coef[i];
+    if (!grid[NS_SQUARES]) {
         const hipError_t e = hipFuncSetAttribute((const void*)k_ns_resident, hipFuncAttributeMaxDynamicSharedMemorySize, plan.lds);
         if (e != hipSuccess) { agb_set_error("%s: %s", name, hipGetErrorString(e)); return AGB_ELAUNCH; }
-        NsCoef all = {};
-        for (int i = 0; i < 3 * steps; ++i) all.v[i] = coef[i];
         if (tab) t = {};
         hipLaunchKernelGGL(k_ns_resident, dim3(grid[NS_RESIDENT]), dim3(NS_WIDE), plan.lds, st, t, tab, count, up, eps, all, steps);
         AGB_CHECK_LAUNCH(name);
+        return AGB_OK;
     }
-    if (!grid[NS_SQUARES]) return AGB_OK;
-    for (const void* k : {(const void*)k_ns_gram, (const void*)k_ns_poly, (const void*)k_ns_apply}) {
+    for (const void* k : {(const void*)k_ns_gram<true>, (const void*)k_ns_poly<true>, (const void*)k_ns_apply<true>, (const void*)k_ns_last<true>,
+                          (const void*)k_ns_last<false>}) {
         const hipError_t e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, NS_LDS(128));
         if (e != hipSuccess) { agb_set_error("%s: %s", name, hipGetErrorString(e)); return AGB_ELAUNCH; }
     }
-    const int lds = plan.wide ? NS_LDS(128) : NS_LDS(64), lds_p = plan.wide_p ? NS_LDS(128) : NS_LDS(64);
+#define NS_PRODUCT(kernel, which, wide, ...)                                                                                \
+    do {                                                                                                                    \
+        if (wide) hipLaunchKernelGGL(kernel<true>, dim3(grid[which]), dim3(NS_WIDE), NS_LDS(128), st, tab, count, __VA_ARGS__); \
+        else hipLaunchKernelGGL(kernel<false>, dim3(grid[which]), dim3(NS_WIDE), NS_LDS(64), st, tab, count, __VA_ARGS__);      \
+    } while (0)
     hipLaunchKernelGGL(k_ns_squares, dim3(grid[NS_SQUARES]), dim3(NS_THREADS), 0, st, tab, count, up);
     hipLaunchKernelGGL(k_ns_planes, dim3(grid[NS_PLANES]), dim3(NS_THREADS), 0, st, tab, count, up, eps);
     for (int i = 0; i < steps; ++i) {
         const float* c = coef + 3 * i;
-        hipLaunchKernelGGL(k_ns_gram, dim3(grid[NS_GRAM]), dim3(NS_WIDE), lds, st, tab, count, i & 1);
+        NS_PRODUCT(k_ns_gram, NS_GRAM, plan.wide, i & 1);
         if (grid[NS_FOLD]) hipLaunchKernelGGL(k_ns_fold, dim3(grid[NS_FOLD]), dim3(NS_THREADS), 0, st, tab, count);
-        hipLaunchKernelGGL(k_ns_poly, dim3(grid[NS_POLY]), dim3(NS_WIDE), lds_p, st, tab, count, c[1], c[2]);
-        hipLaunchKernelGGL(k_ns_apply, dim3(grid[NS_APPLY]), dim3(NS_WIDE), lds, st, tab, count, i & 1, c[0], i == steps - 1, up);
+        NS_PRODUCT(k_ns_poly, NS_POLY, plan.wide_p, c[1], c[2]);
+        if (i < steps - 1 || !grid[NS_RESIDENT]) {
+            NS_PRODUCT(k_ns_apply, NS_APPLY, plan.wide_x, i & 1, c[0], i == steps - 1, up);
+            continue;
+        }
+        const int whole = grid[NS_RESIDENT], lds = plan.wide_x ? NS_LDS(128) : NS_LDS(64);
+        const dim3 both(whole + grid[NS_APPLY]);
+        if (plan.wide_x)
+            hipLaunchKernelGGL(k_ns_last<true>, both, dim3(NS_WIDE), lds > plan.lds ? lds : plan.lds, st, tab, count, i & 1, c[0], up,
+                               whole, eps, all, steps);
+        else
+            hipLaunchKernelGGL(k_ns_last<false>, both, dim3(NS_WIDE), lds > plan.lds ? lds : plan.lds, st, tab, count, i & 1, c[0], up,
+                               whole, eps, all, steps);
     }
+#undef NS_PRODUCT
     AGB_CHECK_LAUNCH(name);
     return AGB_OK;
 }

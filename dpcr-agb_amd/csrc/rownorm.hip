@@ -98,33 +98,38 @@ struct RnPiece<T, 1> {
     static __device__ __forceinline__ void put(T* p, const float* v) { st1(p, *v); }
 };
 
-// a row's pieces: zeros behind the last channel, where there is no matrix and where `on` is false
+// This lane's piece 0 of a group's row of a matrix, and a walk down the rows a turn apart; pieces behind the last channel, rows
+// that are not there (`on` false) and absent matrices read as zeros and are not written.
 template <typename T, int W, int G, int V>
 struct RnRow {
-    RnPiece<T, W> piece[V];
-    __device__ __forceinline__ void load(const void* base, long long ld, long long row, int lane, int C, bool on) {
-        const T* p = (const T*)base + row * ld;
+    T* at;
+    long long step;
+    RnPiece<T, W> piece[V ? V : 1];
+    __device__ __forceinline__ void start(const void* base, long long ld, int row, int lane, int groups) {
+        at = base ? (T*)base + row * ld + lane * W : nullptr;
+        step = groups * ld;
+    }
+    __device__ __forceinline__ void load(int lane, int C, bool on) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const int c = (j * G + lane) * W;
-            if (on && base && c < C) piece[j].load(p + c);
+            if (on && at && (j * G + lane) * W < C) piece[j].load(at + j * G * W);
             else piece[j].clear();
         }
+        at += at ? step : 0;
     }
     __device__ __forceinline__ void get(float* v) const {
 #pragma unroll
         for (int j = 0; j < V; ++j) piece[j].get(v + j * W);
     }
-};
-template <typename T, int W, int G, int V>
-__device__ __forceinline__ void rn_put(void* base, long long ld, long long row, int lane, int C, bool on, const float* v) {
-    T* p = (T*)base + row * ld;
+    template <int VP>
+    __device__ __forceinline__ void put(int lane, int C, bool on, const float* v) {
+        if (!at) return;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int c = (j * G + lane) * W;
-        if (on && c < C) RnPiece<T, W>::put(p + c, v + j * W);
+        for (int j = 0; j < VP; ++j)
+            if (on && (j * G + lane) * W < C) RnPiece<T, W>::put(at + j * G * W, v + j * W);
+        at += step;
     }
-}
+};
 // a parameter vector's values: `other` where there is none, 0 behind the last channel.  No branch between the loads: all are in
 // flight together (a load, a branch and a use at a time they were most of a short call's time).
 struct __attribute__((packed, aligned(4))) RnFour {
@@ -263,18 +268,25 @@ __global__ __launch_bounds__(RN_THREADS) void k_rownorm(const RnArgs a) {
                 for (int i = 0; i < N; ++i) sums[s][i] = 0.f;
         }
         Row z, r, dy, dh;
+        RnRow<T, W, G, 0> to1, to2;      // y and h, or dr and dz
+        z.start(a.z, a.ldz, row0 + group, lane, GROUPS);
+        r.start(a.r, a.ldr, row0 + group, lane, GROUPS);
+        if constexpr (BWD) {
+            dy.start(a.dy, a.lddy, row0 + group, lane, GROUPS);
+            dh.start(a.dh, a.lddh, row0 + group, lane, GROUPS);
+        }
+        to1.start(BWD ? a.dr : a.y, BWD ? a.lddr : a.ldy, row0 + group, lane, GROUPS);
+        to2.start(BWD ? a.dz : a.h, BWD ? a.lddz : a.ldh, row0 + group, lane, GROUPS);
         auto fetch = [&](int at) {
-            const long long row = at + group;
-            const bool on = row < end;
-            z.load(a.z, a.ldz, row, lane, a.C, on);
-            r.load(a.r, a.ldr, row, lane, a.C, on);
-            if constexpr (BWD) dy.load(a.dy, a.lddy, row, lane, a.C, on);
-            if constexpr (BWD && NEXT) dh.load(a.dh, a.lddh, row, lane, a.C, on);
+            const bool on = at + group < end;
+            z.load(lane, a.C, on);
+            r.load(lane, a.C, on);
+            if constexpr (BWD) dy.load(lane, a.C, on);
+            if constexpr (BWD && NEXT) dh.load(lane, a.C, on);
         };
         fetch(row0);
         for (int at = row0; at < end; at += GROUPS) {      // (every lane takes every turn: the sums need whole groups)
-            const long long row = at + group;
-            const bool on = row < end;
+            const bool on = at + group < end;
             float x[N], u[N], g[BWD ? N : 1], h[(BWD && NEXT) ? N : 1];
             z.get(x);
             r.get(u);
@@ -299,12 +311,12 @@ __global__ __launch_bounds__(RN_THREADS) void k_rownorm(const RnArgs a) {
 #pragma unroll
                     for (int i = 0; i < N; ++i) u[i] = act_fwd(u[i], ACT_RELU);
                 }
-                if (a.y) rn_put<T, W, G, V>(a.y, a.ldy, row, lane, a.C, on, u);
+                to1.template put<V>(lane, a.C, on, u);
                 if constexpr (NEXT) {
                     rn_normalise<W, G, V>(u, there, inv, a.rms, a.eps2, on, red, turn);
 #pragma unroll
                     for (int i = 0; i < N; ++i) u[i] = __builtin_fmaf(u[i], w2[i], b2[i]);
-                    rn_put<T, W, G, V>(a.h, a.ldh, row, lane, a.C, on, u);
+                    to2.template put<V>(lane, a.C, on, u);
                 }
             } else {
                 float slope[N];
@@ -337,12 +349,12 @@ __global__ __launch_bounds__(RN_THREADS) void k_rownorm(const RnArgs a) {
                     sums[0][i] += g[i];
                     sums[1][i] = __builtin_fmaf(g[i], x[i], sums[1][i]);
                 }
-                if (a.dr) rn_put<T, W, G, V>(a.dr, a.lddr, row, lane, a.C, on, g);
+                to1.template put<V>(lane, a.C, on, g);
                 if (a.dz) {
 #pragma unroll
                     for (int i = 0; i < N; ++i) g[i] *= fw[i];
                     rn_norm_grad<W, G, V>(g, x, live ? rstd : 0.f, inv, a.rms, red, turn);
-                    rn_put<T, W, G, V>(a.dz, a.lddz, row, lane, a.C, on, g);
+                    to2.template put<V>(lane, a.C, on, g);
                 }
             }
         }
@@ -400,8 +412,10 @@ __device__ __forceinline__ float rn_fold32(float v, float (*t)[33]) {
     t[k][c] = v;
     __syncthreads();
     float s = 0.f;
-    if (k == 0)
+    if (k == 0) {
+#pragma unroll
         for (int i = 0; i < 32; ++i) s += t[i][c];
+    }
     return s;          // (lane k == 0)
 }
 
@@ -427,8 +441,11 @@ __global__ __launch_bounds__(1024) void k_rownorm_fold_slots(const RnFold a) {
         p += __popcll(__ballot(i <= a.B && s1 <= first));
     }
     p = __builtin_amdgcn_readfirstlane(p);
-    for (; p <= a.B; ++p) {
-        rn_slots(a, p, s0, s1);
+    int look0 = 0, look1 = 0;      // lane i: the slots of plot p + i (of every 64 plots, one look)
+    for (int i = 0; p <= a.B; ++p, i = (i + 1) & 63) {
+        if (i == 0) rn_slots(a, min(p + (int)(threadIdx.x & 63), a.B), look0, look1);
+        s0 = __builtin_amdgcn_readlane(look0, i);
+        s1 = __builtin_amdgcn_readlane(look1, i);
         if (s0 >= first + 64) return;
         s0 = max(s0, first);
         s1 = min(s1, first + 64);

@@ -394,140 +394,136 @@ ROW_NORM_KINDS = {"layer": 0, "rms": 1}
 ROW_NORM_MAX_C = 4096
 
 
+_ROW_TYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
 def _as_rows(t):
     """A row matrix the kernels can walk: channels adjacent, rows apart by at least their width."""
+    if t.is_contiguous():
+        return t
     n, c = t.shape
     return t if (c == 1 or t.stride(1) == 1) and (n == 1 or t.stride(0) >= c) else t.contiguous()
 
 
 def _ld(t):
     """Row stride (of a single row: its width; the stride of an axis of length one says nothing)."""
-    return 0 if t is None else max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 def _row_norm_forward(z, r, w, b, gate, scale, w2, b2, keep, ptr, cfg):
-    eps, rms, act, eps2, want_h = cfg
+    """One launch.  (Everything has been checked: addresses are taken as they are.)"""
+    eps, rms, act, eps2, want_h, bf16 = cfg
     n, c = z.shape
     y = torch.empty((n, c), dtype=z.dtype, device=z.device)
     h = torch.empty_like(y) if want_h else None
-    _lib.call("agb_rownorm_fwd", _R(z), _ld(z), _R(r), _ld(r), n, c, _P(w), _P(b), eps, rms, act, _P(gate), _P(keep), _P(ptr),
-              0 if ptr is None else ptr.shape[0] - 1, _P(scale), _P(w2), _P(b2), eps2, _R(y), c, _R(h), c,
-              int(z.dtype == torch.bfloat16), _lib.stream())
+    _lib.call("agb_rownorm_fwd", z.data_ptr(), _ld(z), _at(r), 0 if r is None else _ld(r), n, c, _at(w), _at(b), eps, rms, act,
+              _at(gate), _at(keep), _at(ptr), 0 if ptr is None else ptr.shape[0] - 1, _at(scale), _at(w2), _at(b2), eps2,
+              y.data_ptr(), c, _at(h), c, bf16, _lib.stream())
     return y, h
 
 
-class RowNormFunction(torch.autograd.Function):
-    """y = act(r + keep[p] gate[p] scale norm(z)) and, on request, h = norm(y): csrc/rownorm.hip, one launch forward; one launch
-    and its folds backward.  Keeps z and r; everything else is recomputed in registers."""
+def _row_norm_backward(z, r, w, b, gate, scale, w2, b2, keep, ptr, cfg, dy, dh, need):
+    """Gradients of (z, r, w, b, gate, scale, w2, b2) where `need` asks for them."""
+    if torch.is_grad_enabled():
+        raise _lib.AgbError("row norms have first derivatives only (a backward pass that is itself differentiated)")
+    if dy is None and dh is None:
+        return (None,) * 8
+    eps, rms, act, eps2, _, bf16 = cfg
+    n, c = z.shape
+    dev = z.device
+    dy = None if dy is None else _as_rows(dy)
+    dh = None if dh is None else _as_rows(dh)
+    plots = 0 if ptr is None else ptr.shape[0] - 1
+    has_h = dh is not None
+    dz = torch.empty((n, c), dtype=z.dtype, device=dev) if need[0] else None
+    through = need[1] and act == 0 and not has_h           # dr = dy
+    dr = torch.empty((n, c), dtype=z.dtype, device=dev) if need[1] and not through else None
+    dw, db, dscale, dw2, db2 = (torch.empty(c, dtype=torch.float32, device=dev) if k else None
+                                for k in (need[2], need[3], need[5], need[6] and has_h, need[7] and has_h))
+    dgate = torch.empty((plots, c), dtype=torch.float32, device=dev) if need[4] else None
+    size = _lib.size_call("agb_rownorm_bwd_workspace_bytes", n, c, plots, int(has_h))
+    work = torch.empty(size, dtype=torch.uint8, device=dev)
+    _lib.call("agb_rownorm_bwd", z.data_ptr(), _ld(z), _at(r), 0 if r is None else _ld(r), _at(dy), 0 if dy is None else _ld(dy),
+              _at(dh), _ld(dh) if has_h else 0, n, c, _at(w), _at(b), eps, rms, act, _at(gate), _at(keep), _at(ptr), plots,
+              _at(scale), _at(w2), _at(b2), eps2, _at(dz), c, _at(dr), c, _at(dw), _at(db), _at(dgate), _at(dscale), _at(dw2),
+              _at(db2), work.data_ptr(), size, bf16, _lib.stream())
+    return dz, (dy if through else dr), dw, db, dgate, dscale, dw2, db2
+
+
+class RowNormActFunction(torch.autograd.Function):
+    """y = act(norm(x)): csrc/rownorm.hip, one launch forward; one launch and its folds backward.  Keeps x; everything else is
+    recomputed in registers."""
 
     @staticmethod
-    def forward(ctx, z, r, w, b, gate, scale, w2, b2, keep, ptr, cfg):
-        y, h = _row_norm_forward(z, r, w, b, gate, scale, w2, b2, keep, ptr, cfg)
-        ctx.save_for_backward(z, r, w, b, gate, scale, w2, b2, keep, ptr)
+    def forward(ctx, x, w, b, cfg):
+        ctx.save_for_backward(x, w, b)
+        ctx.cfg = cfg
+        return _row_norm_forward(x, None, w, b, None, None, None, None, None, None, cfg)[0]
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, w, b = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        g = _row_norm_backward(x, None, w, b, None, None, None, None, None, None, ctx.cfg, dy, None,
+                               (need[0], False, need[1], need[2], False, False, False, False))
+        return g[0], g[2], g[3], None
+
+
+class RowNormJoinFunction(torch.autograd.Function):
+    """y = act(r + keep[p] gate[p] scale norm(z)) and, on request, h = norm(y), as RowNormActFunction; keeps z and r."""
+
+    @staticmethod
+    def forward(ctx, z, r, w, b, gate, scale, w2, b2, plots, cfg):
+        ctx.save_for_backward(z, r, w, b, gate, scale, w2, b2, *plots)
         ctx.cfg = cfg
         ctx.set_materialize_grads(False)
+        y, h = _row_norm_forward(z, r, w, b, gate, scale, w2, b2, *plots, cfg)
         return (y, h) if cfg[4] else y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dh=None):
-        z, r, w, b, gate, scale, w2, b2, keep, ptr = ctx.saved_tensors
-        eps, rms, act, eps2, _ = ctx.cfg
-        if dy is None and dh is None:
-            return (None,) * 11
-        need = ctx.needs_input_grad
-        n, c = z.shape
-        dev, bf16 = z.device, int(z.dtype == torch.bfloat16)
-        dy = None if dy is None else _as_rows(dy)
-        dh = None if dh is None else _as_rows(dh)
-        plots = 0 if ptr is None else ptr.shape[0] - 1
-
-        def grad(wanted, *shape, dtype=torch.float32):
-            return torch.empty(shape, dtype=dtype, device=dev) if wanted else None
-
-        dz = grad(need[0], n, c, dtype=z.dtype)
-        through = need[1] and act == 0 and dh is None           # dr = dy
-        dr = grad(need[1] and not through, n, c, dtype=z.dtype)
-        dw, db, dscale = grad(need[2], c), grad(need[3], c), grad(need[5], c)
-        dgate = grad(need[4], plots, c)
-        dw2, db2 = grad(need[6] and dh is not None, c), grad(need[7] and dh is not None, c)
-        size = _lib.size_call("agb_rownorm_bwd_workspace_bytes", n, c, plots, int(dh is not None))
-        work = torch.empty(size, dtype=torch.uint8, device=dev)
-        _lib.call("agb_rownorm_bwd", _R(z), _ld(z), _R(r), _ld(r), _R(dy), _ld(dy), _R(dh), _ld(dh), n, c, _P(w), _P(b), eps,
-                  rms, act, _P(gate), _P(keep), _P(ptr), plots, _P(scale), _P(w2), _P(b2), eps2, _R(dz), c, _R(dr), c, _P(dw),
-                  _P(db), _P(dgate), _P(dscale), _P(dw2), _P(db2), work.data_ptr(), size, bf16, _lib.stream())
-        return dz, (dy if through else dr), dw, db, dgate, dscale, dw2, db2, None, None, None
+        return (*_row_norm_backward(*ctx.saved_tensors, ctx.cfg, dy, dh, ctx.needs_input_grad), None, None)
 
 
-def _vector(name, v, n, device):
-    if v is None:
-        return None
-    if v.dim() != 1 or v.shape[0] != n:
-        raise ValueError(f"{name}: expected [{n}], got {list(v.shape)}")
-    return _param(name, v, device)
-
-
-def _param(name, v, device):
-    if v.dtype != torch.float32:
-        raise _lib.AgbError(f"{name}: parameters and per-plot factors are fp32 (got {v.dtype})")
-    if v.device != device:
-        raise _lib.AgbError(f"{name}: on {v.device}, the rows are on {device}")
-    return v.contiguous()
-
-
-def _row_norm(what, z, r, weight, bias, eps, kind, act, gate, keep, ptr, scale, next_norm):
+def _check_rows(what, z, kind, act):
     if kind not in ROW_NORM_KINDS:
         raise ValueError(f"{what}: kind '{kind}': choose layer or rms")
     if act not in ACT_IDS:
         raise ValueError(f"{what}: act '{act}': choose none, relu or gelu")
-    if z.dim() != 2 or z.shape[1] < 1 or z.shape[1] > ROW_NORM_MAX_C:
+    if z.dim() != 2 or not 1 <= z.shape[1] <= ROW_NORM_MAX_C:
         raise ValueError(f"{what}: rows [N, C] with 1 <= C <= {ROW_NORM_MAX_C} are normalised, got {list(z.shape)}")
-    if z.dtype not in (torch.float32, torch.bfloat16):
+    if z.dtype not in _ROW_TYPES:
         raise _lib.AgbError(f"{what}: rows are fp32 or bf16 (got {z.dtype})")
-    if r is not None:
-        if r.shape != z.shape:
-            raise ValueError(f"{what}: z {list(z.shape)} and r {list(r.shape)} differ")
-        if r.dtype != z.dtype or r.device != z.device:
-            raise _lib.AgbError(f"{what}: z ({z.dtype}, {z.device}) and r ({r.dtype}, {r.device}) differ")
-        r = _as_rows(r)
-    c, dev = z.shape[1], z.device
-    w, b, scale = (_vector(f"{what}: {k}", v, c, dev) for k, v in (("weight", weight), ("bias", bias), ("scale", scale)))
-    w2 = b2 = None
-    eps2 = eps
-    if next_norm is not None:
-        w2, b2 = (_vector(f"{what}: next_norm {k}", v, c, dev) for k, v in zip(("weight", "bias"), next_norm))
-        eps2 = next_norm[2] if len(next_norm) > 2 else eps
-    if gate is None and keep is None:
-        ptr = None
-    else:
-        if ptr is None:
-            raise ValueError(f"{what}: a gate or a keep factor needs ptr, the plots' row ranges")
-        if ptr.dim() != 1 or ptr.shape[0] < 2 or ptr.dtype != torch.int32 or ptr.device != dev:
-            raise ValueError(f"{what}: ptr is int32 [B + 1] on {dev}, got {ptr.dtype} {list(ptr.shape)} on {ptr.device}")
-        ptr = ptr.contiguous()
-        plots = ptr.shape[0] - 1
-        keep = _vector(f"{what}: keep", keep, plots, dev)
-        if keep is not None and keep.requires_grad:
-            raise ValueError(f"{what}: keep factors are drawn, they have no gradient: pass a learned factor as gate")
-        if gate is not None:
-            if gate.shape != (plots, c):
-                raise ValueError(f"{what}: gate: expected [{plots}, {c}], got {list(gate.shape)}")
-            gate = _param(f"{what}: gate", gate, dev)
-    cfg = (float(eps), ROW_NORM_KINDS[kind], ACT_IDS[act], float(eps2), next_norm is not None)
-    args = (_as_rows(z), r, w, b, gate, scale, w2, b2, keep, ptr, cfg)
+    return ROW_NORM_KINDS[kind], ACT_IDS[act], _ROW_TYPES[z.dtype]
+
+
+def _vector(what, name, v, n, device):
+    if v is None:
+        return None
+    if v.dim() != 1 or v.shape[0] != n:
+        raise ValueError(f"{what}: {name}: expected [{n}], got {list(v.shape)}")
+    return _param(what, name, v, device)
+
+
+def _param(what, name, v, device):
+    if v.dtype != torch.float32:
+        raise _lib.AgbError(f"{what}: {name}: parameters and per-plot factors are fp32 (got {v.dtype})")
+    if v.device != device:
+        raise _lib.AgbError(f"{what}: {name}: on {v.device}, the rows are on {device}")
+    return v if v.is_contiguous() else v.contiguous()
+
+
+def _on_device(z, run):
+    """Launches go to the current stream of the current device: rows of another device bring theirs."""
     _R(z)       # (refuses host tensors)
-    # (launches go to the current stream of the current device: rows of another device bring theirs)
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            return _row_norm_apply(args)
-    return _row_norm_apply(args)
-
-
-def _row_norm_apply(args):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:8]):
-        return RowNormFunction.apply(*args)
-    y, h = _row_norm_forward(*args)
-    return (y, h) if args[-1][4] else y
+    if z.device.index == _lib.current_device():
+        return run()
+    with torch.cuda.device(z.device):
+        return run()
 
 
 def row_norm_act(x, weight=None, bias=None, eps=1e-6, kind="layer", act=None):
@@ -536,8 +532,17 @@ def row_norm_act(x, weight=None, bias=None, eps=1e-6, kind="layer", act=None):
     x [N, C], fp32 or bf16 rows (C <= 4096; row strides above C are walked in place); kind "layer": each row less its mean, over
     its standard deviation; "rms": over its root mean square; eps is added to the variance / mean square.  weight, bias: fp32
     [C] or None.  act: None / "none", "relu", "gelu" (erf).  Statistics and sums are fp32; the result is rounded once.
-    Differentiable in x, weight and bias."""
-    return _row_norm("row_norm_act", x, None, weight, bias, eps, kind, act, None, None, None, None, None)
+    Differentiable (once) in x, weight and bias."""
+    rms, act_id, bf16 = _check_rows("row_norm_act", x, kind, act)
+    c, dev = x.shape[1], x.device
+    weight = _vector("row_norm_act", "weight", weight, c, dev)
+    bias = _vector("row_norm_act", "bias", bias, c, dev)
+    x = _as_rows(x)
+    cfg = (float(eps), rms, act_id, float(eps), False, bf16)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        return _on_device(x, lambda: RowNormActFunction.apply(x, weight, bias, cfg))
+    return _on_device(x, lambda: _row_norm_forward(x, None, weight, bias, None, None, None, None, None, None, cfg)[0])
 
 
 def row_norm_join(z, r, weight=None, bias=None, eps=1e-6, kind="layer", act=None, gate=None, keep=None, ptr=None, scale=None,
@@ -549,7 +554,41 @@ def row_norm_join(z, r, weight=None, bias=None, eps=1e-6, kind="layer", act=None
     gate and keep need ptr int32 [B + 1], the plots' row ranges (``coordinate_manager.batch_ptr``): ascending, ptr[0] = 0; plots
     may be empty; rows behind ptr[B] belong to no plot and come out as act(r).
     next_norm=(weight2, bias2[, eps2]): also returns h = norm(y), of the same kind, from the unrounded y: (y, h).
-    Differentiable in z, r, weight, bias, gate, scale and next_norm's vectors; sums over rows are folded in a fixed order."""
+    Differentiable (once) in z, r, weight, bias, gate, scale and next_norm's vectors; sums over rows are folded in a fixed order."""
+    what = "row_norm_join"
     if r is None:
         raise ValueError("row_norm_join: r is the shortcut's rows; without one use row_norm_act")
-    return _row_norm("row_norm_join", z, r, weight, bias, eps, kind, act, gate, keep, ptr, scale, next_norm)
+    rms, act_id, bf16 = _check_rows(what, z, kind, act)
+    c, dev = z.shape[1], z.device
+    if r.shape != z.shape:
+        raise ValueError(f"{what}: z {list(z.shape)} and r {list(r.shape)} differ")
+    if r.dtype != z.dtype or r.device != dev:
+        raise _lib.AgbError(f"{what}: z ({z.dtype}, {dev}) and r ({r.dtype}, {r.device}) differ")
+    weight, bias, scale = (_vector(what, k, v, c, dev) for k, v in (("weight", weight), ("bias", bias), ("scale", scale)))
+    w2 = b2 = None
+    eps2 = eps
+    if next_norm is not None:
+        w2, b2 = (_vector(what, "next_norm " + k, v, c, dev) for k, v in zip(("weight", "bias"), next_norm))
+        eps2 = next_norm[2] if len(next_norm) > 2 else eps
+    if gate is None and keep is None:
+        ptr = None
+    else:
+        if ptr is None:
+            raise ValueError(f"{what}: a gate or a keep factor needs ptr, the plots' row ranges")
+        if ptr.dim() != 1 or ptr.shape[0] < 2 or ptr.dtype != torch.int32 or ptr.device != dev:
+            raise ValueError(f"{what}: ptr is int32 [B + 1] on {dev}, got {ptr.dtype} {list(ptr.shape)} on {ptr.device}")
+        ptr = ptr.contiguous()
+        plots = ptr.shape[0] - 1
+        keep = _vector(what, "keep", keep, plots, dev)
+        if keep is not None and keep.requires_grad:
+            raise ValueError(f"{what}: keep factors are drawn, they have no gradient: pass a learned factor as gate")
+        if gate is not None:
+            if gate.shape != (plots, c):
+                raise ValueError(f"{what}: gate: expected [{plots}, {c}], got {list(gate.shape)}")
+            gate = _param(what, "gate", gate, dev)
+    cfg = (float(eps), rms, act_id, float(eps2), next_norm is not None, bf16)
+    args = (_as_rows(z), _as_rows(r), weight, bias, gate, scale, w2, b2)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+        return _on_device(z, lambda: RowNormJoinFunction.apply(*args, (keep, ptr), cfg))
+    y, h = _on_device(z, lambda: _row_norm_forward(*args, keep, ptr, cfg))
+    return (y, h) if cfg[4] else y
