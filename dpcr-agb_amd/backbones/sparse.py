@@ -14,7 +14,8 @@ import torch
 import torch.nn as nn
 
 from .. import me_compat as ME
-from ..se_ops import MAX_HIDDEN as MAX_SE_HIDDEN, se_layer
+from ..norm_ops import ROW_NORM_MAX_C, row_norm_act
+from ..se_ops import MAX_HIDDEN as MAX_SE_HIDDEN, se_excite, se_layer
 from ..sparse_ops import current as current_options, model_scope
 
 ACTIVATIONS = {
@@ -116,17 +117,53 @@ class MinkowskiDropPath(nn.Module):
 
 class MinkowskiLayerNorm(nn.Module):
     """Channel-wise layer normalisation of a sparse tensor's rows (common.py:369-386: nn.LayerNorm(C, eps=1e-6) on .F;
-    state_dict keys ``ln.weight`` / ``ln.bias``), on csrc/layernorm.hip."""
+    state_dict keys ``ln.weight`` / ``ln.bias``), on csrc/layernorm.hip, or under KernelOptions.fused_row_norm on
+    csrc/rownorm.hip together with what follows it."""
 
     def __init__(self, normalized_shape, eps=1e-6):
         super().__init__()
         self.ln = nn.LayerNorm(normalized_shape, eps=eps)
 
+    def row_norm_form(self):
+        if not current_options().fused_row_norm or self.ln.normalized_shape[0] > ROW_NORM_MAX_C:
+            return None
+        return dict(weight=self.ln.weight, bias=self.ln.bias, eps=self.ln.eps, kind="layer")
+
     def forward(self, input):
+        form = self.row_norm_form()
+        if form is not None:
+            return input._like(row_norm_act(input.F, **form))
         from ..norm_ops import layer_norm
         if input.F.dtype == torch.bfloat16:     # bf16 row storage: csrc/layernorm.hip takes fp32 rows
             return input._like(layer_norm(input.F.float(), self.ln).to(torch.bfloat16))
         return input._like(layer_norm(input.F, self.ln))
+
+
+class MinkowskiRMSNorm(nn.Module):
+    """Channel-wise root-mean-square normalisation of a sparse tensor's rows, weight only (state_dict key ``rms.weight``), on
+    csrc/rownorm.hip; an encoder's ``norm_type="rms"``."""
+
+    def __init__(self, normalized_shape, eps=1e-6):
+        super().__init__()
+        self.rms = nn.RMSNorm(normalized_shape, eps=eps)
+
+    def row_norm_form(self):
+        return dict(weight=self.rms.weight, eps=self.rms.eps, kind="rms")
+
+    def forward(self, input):
+        return input._like(row_norm_act(input.F, **self.row_norm_form()))
+
+
+def _row_norm_tail(block, z, residual, last_norm, gate=None):
+    """act(drop_path(last_norm(z) * gate) + residual) as one kernel; None where a piece is not of the plain kind."""
+    dp = block.drop_path
+    if (ME.row_norm_form(last_norm) is None or getattr(block.relu, "act_name", None) is None
+            or not isinstance(dp, (MinkowskiDropPath, nn.Identity))):
+        return None
+    keep = dp.scale_vector(z) if isinstance(dp, MinkowskiDropPath) else None
+    if gate is not None:
+        gate = gate()
+    return ME.fused_norm_residual(last_norm, z, residual, block.relu, keep, gate)
 
 
 def _residual_tail(block, out, residual):
@@ -172,6 +209,11 @@ class BasicBlock(nn.Module):
         return self.norm2(self.conv2(out))
 
     def forward(self, x):
+        if ME.row_norm_form(self.norm2) is not None:
+            z = self.conv2(ME.fused_norm_act(self.norm1, self.relu, self.conv1(x)))
+            residual = self.downsample(x)
+            y = _row_norm_tail(self, z, residual, self.norm2)
+            return y if y is not None else _residual_tail(self, self.norm2(z), residual)
         out = self._main(x)
         residual = self.downsample(x)
         return _residual_tail(self, out, residual)
@@ -206,6 +248,10 @@ class Bottleneck(nn.Module):
         out, x = self.conv1.forward_join(x)
         out = ME.fused_norm_act(self.norm1, self.relu, out)
         out = ME.fused_norm_act(self.norm2, self.relu, self.conv2(out))
+        if ME.row_norm_form(self.norm3) is not None:
+            z, residual = self.conv3(out), self.downsample(x)
+            y = _row_norm_tail(self, z, residual, self.norm3)
+            return y if y is not None else _residual_tail(self, self.norm3(z), residual)
         out = self.norm3(self.conv3(out))
         residual = self.downsample(x)
         return _residual_tail(self, out, residual)
@@ -238,6 +284,16 @@ class SELayer(nn.Module):
         pooled = self.pooling(x)
         return self.broadcast_mul(x, self.fc(pooled))
 
+    def excitation(self, x):
+        """The factors alone, fp32 [B, C]: sigmoid(fc(pool(x)))."""
+        lin1, act, lin2, gate = self.fc[0], self.fc[1], self.fc[2], self.fc[3]
+        name = getattr(act, "act_name", None)
+        pooled = self.pooling(x)
+        if (name in ("relu", "gelu") and isinstance(gate, ME.MinkowskiSigmoid)
+                and lin1.linear.out_features <= MAX_SE_HIDDEN):
+            return se_excite(pooled.F, lin1.linear, name, lin2.linear)
+        return self.fc(pooled).F
+
 
 def _se_block_forward(block, x, z, last_norm):
     """Everything behind the last convolution of an SE block (its output z before `last_norm`): the one-node fused tail
@@ -256,6 +312,11 @@ def _se_block_forward(block, x, z, last_norm):
         keep = dp.scale_vector(z) if isinstance(dp, MinkowskiDropPath) else None
         return z._like(se_ops.se_block_tail(z.F, residual.F, last_norm.bn, cm.level(ts).coords, cm.batch_ptr(ts),
                                             cm.batch_size, lin1.linear, se_name, lin2.linear, keep, act_name))
+    if current_options().fused_tail and ME.row_norm_form(last_norm) is not None and z._ts != 0:
+        # (the excitation reads the normalised rows once, for its pool; the join normalises again from z, in registers)
+        y = _row_norm_tail(block, z, residual, last_norm, gate=lambda: se.excitation(last_norm(z)))
+        if y is not None:
+            return y
     return _residual_tail(block, se(last_norm(z)), residual)
 
 
@@ -313,8 +374,10 @@ class ResNetBase(nn.Module):
             self.norm_layer = ME.MinkowskiInstanceNorm
         elif norm_type == "ln":
             self.norm_layer = MinkowskiLayerNorm
+        elif norm_type == "rms":
+            self.norm_layer = MinkowskiRMSNorm
         else:
-            raise NotImplementedError(f"Choose either 'bn', 'in', or 'ln'. Given: {norm_type}")
+            raise NotImplementedError(f"Choose either 'bn', 'in', 'ln' or 'rms'. Given: {norm_type}")
 
         # tensor strides the forward pass will visit (lets set_input build the whole coordinate pyramid at once)
         ts, self.tensor_strides = first_stride * 2, [first_stride, first_stride * 2]
@@ -471,5 +534,5 @@ SENet17_5deep = _variant("SENet17_5deep", SEBasicBlock, (1, 1, 1, 2, 2), (1, 2, 
 __all__ = ["ResNetBase", "ResNet14_", "ResNet18_", "ResNet34_", "ResNet50_", "ResNet101_", "SENet14", "SENet18",
            "SENet34", "SENet50", "SENet101", "SENet17_6deep", "SENet17_5deep", "BasicBlock", "Bottleneck",
            "SEBasicBlock", "SEBottleneck", "SELayer", "ConvNormActivation", "MinkowskiDropPath", "MinkowskiLayerNorm",
-           "ACTIVATIONS",
+           "MinkowskiRMSNorm", "ACTIVATIONS",
            "GLOBAL_POOL"]

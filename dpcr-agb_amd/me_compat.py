@@ -20,7 +20,7 @@ import torch.nn as nn
 
 from . import _lib
 from .coords import CoordinateManager, CoordinateMapKey, _as_int
-from .norm_ops import ACT_IDS, AddActFunction, batch_norm_act
+from .norm_ops import ACT_IDS, AddActFunction, batch_norm_act, row_norm_act, row_norm_join
 from .sparse_ops import (BroadcastMulFunction, DenseConvFunction, take_bn_hint, GlobalPoolFunction, MaxPoolFunction,
                          SparseConvFunction, dense_conv_join, dense_linear)
 
@@ -418,12 +418,31 @@ MinkowskiAvgUnpooling = _unsupported("MinkowskiAvgUnpooling")
 
 def fused_norm_act(norm, act, x: SparseTensor) -> SparseTensor:
     """act(norm(x)) in one fused BatchNorm+activation kernel pair when norm is a MinkowskiBatchNorm and act a plain
-    ReLU/GELU (the reference's ConvNormActivation / block wiring); otherwise the modules are applied one by one."""
+    ReLU/GELU (the reference's ConvNormActivation / block wiring), in one row-norm kernel when norm has that form
+    (``row_norm_form``); otherwise the modules are applied one by one."""
     name = getattr(act, "act_name", None) if act is not None else "none"
     if isinstance(norm, MinkowskiBatchNorm) and name is not None and x.F.shape[1] % 4 == 0:
         return x._like(batch_norm_act(x.F, norm.bn, name))
+    form = row_norm_form(norm)
+    if form is not None and name is not None:
+        return x._like(row_norm_act(x.F, act=name, **form))
     x = norm(x)
     return act(x) if act is not None else x
+
+
+def row_norm_form(norm):
+    """The arguments of norm_ops.row_norm_act / row_norm_join for a norm module whose rows these kernels take; None for others."""
+    form = getattr(norm, "row_norm_form", None)
+    return form() if form is not None else None
+
+
+def fused_norm_residual(norm, out: SparseTensor, residual: SparseTensor, act, drop_scale=None, gate=None) -> SparseTensor:
+    """act(norm(out) * gate[batch] * drop_scale[batch] + residual) in one row-norm kernel: `norm` has a ``row_norm_form`` and
+    `act` is a plain one."""
+    out._check_same_map(residual)
+    ptr = None if gate is None and drop_scale is None else out.coordinate_manager.batch_ptr(out._ts)
+    return out._like(row_norm_join(out.F, residual.F, act=act.act_name, gate=gate, keep=drop_scale, ptr=ptr,
+                                   **row_norm_form(norm)))
 
 
 def fused_residual(out: SparseTensor, residual: SparseTensor, act, drop_scale=None) -> SparseTensor:
@@ -455,4 +474,4 @@ for _n in ("ReLU", "GELU", "CELU", "SiLU", "ELU", "Sigmoid", "Tanh", "LeakyReLU"
 
 __all__ = [n for n in dir() if n.startswith("Minkowski")] + ["SparseTensor", "CoordinateManager", "CoordinateMapKey",
                                                               "RegionType", "KernelGenerator", "fused_norm_act",
-                                                              "fused_residual"]
+                                                              "fused_residual", "fused_norm_residual"]

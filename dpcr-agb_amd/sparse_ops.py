@@ -66,19 +66,22 @@ class KernelOptions:
       join_dgrad           a KPConv bottleneck block's input feeds its first Linear AND its shortcut: the shortcut's gradient
                            rides in the final store of that Linear's data gradient (DenseLinearFunction join form,
                            agb_spconv_bwd_data's addend) instead of a separate addition pass per block.  Default on (fp32).
+      fused_row_norm       norm_type "ln" on the row-norm kernels (csrc/rownorm.hip): each norm in one pass with its activation,
+                           the last one of a block with gate, drop path and shortcut, bf16 rows read and written as they are.
+                           Its own summation order (1e-6 of csrc/layernorm.hip's).  Default off; norm_type "rms" always.
 
     Use: ``model.kernel_options = KernelOptions(precision="bf16")`` (the backbones run their forward pass inside it), or
     ``with KernelOptions(cmp_mode=128): ...`` around direct calls.  Autograd nodes keep the options they were created
     under for their backward pass.  ``DEFAULTS`` (environment-initialised) applies where nothing else is set."""
     __slots__ = ("precision", "cmp_mode", "cmp_interleave", "balanced_tiles", "bn_stats_in_epilogue", "fused_tail",
                  "deterministic_wgrad", "dw_variant", "bf16_storage", "bf16_activations", "closed_form_bias_grad",
-                 "fused_blocks", "fused_head", "fused_kpconv", "join_dgrad")
+                 "fused_blocks", "fused_head", "fused_kpconv", "join_dgrad", "fused_row_norm")
     PRECISIONS = ("fp32", "bf16", "bf16x3")
 
     def __init__(self, precision=None, cmp_mode=None, cmp_interleave=None, balanced_tiles=None,
                  bn_stats_in_epilogue=None, fused_tail=None, deterministic_wgrad=None, dw_variant=None,
                  bf16_storage=None, bf16_activations=None, closed_form_bias_grad=None, fused_blocks=None, fused_head=None,
-                 fused_kpconv=None, join_dgrad=None, base=None):
+                 fused_kpconv=None, join_dgrad=None, fused_row_norm=None, base=None):
         base = base if base is not None else (current() if "DEFAULTS" in globals() else None)
         pick = lambda v, name, dflt: v if v is not None else (getattr(base, name) if base is not None else dflt)  # noqa: E731
         self.precision = pick(precision, "precision", "fp32")
@@ -98,6 +101,7 @@ class KernelOptions:
         self.fused_head = bool(pick(fused_head, "fused_head", True))
         self.fused_kpconv = bool(pick(fused_kpconv, "fused_kpconv", True))
         self.join_dgrad = bool(pick(join_dgrad, "join_dgrad", True))
+        self.fused_row_norm = bool(pick(fused_row_norm, "fused_row_norm", False))
 
     def replace(self, **kw):
         return KernelOptions(base=self, **kw)
@@ -153,7 +157,8 @@ DEFAULTS = KernelOptions(precision=os.environ.get("AGB_CONV_PRECISION", "fp32"),
                          fused_blocks=os.environ.get("AGB_FUSED_BLOCKS", "1") != "0",
                          fused_head=os.environ.get("AGB_FUSED_HEAD", "1") != "0",
                          fused_kpconv=os.environ.get("AGB_FUSED_KPCONV", "1") != "0",
-                         join_dgrad=os.environ.get("AGB_JOIN_DGRAD", "1") != "0")
+                         join_dgrad=os.environ.get("AGB_JOIN_DGRAD", "1") != "0",
+                         fused_row_norm=os.environ.get("AGB_FUSED_ROW_NORM", "0") != "0")
 
 
 def set_conv_precision(name):
