@@ -1169,30 +1169,35 @@ static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
     if (m.k > 16384) return false;
     m.kp = agb_cdiv(m.k, 64) * 64;
     m.np = agb_cdiv(m.n, 64) * 64;
-    // Products: a workgroup of T = 128 (one a CU) takes about 6 us and 0.65 us for each 32 of the sum, one of T = 64 (two a CU)
-    // 5 and 0.25 (measured).  T = 128 where its tiles fill half of the device.
+    // Products, measured: a workgroup of T = 128 has a CU to itself, for about 6 us and 0.65 for each 32 of the sum; of T = 64 a CU
+    // holds two, which share what one alone reaches: 6 us and 0.22 for each 32 (a quarter of the work).  So 64 x 64 where the
+    // tiles are few and 128 x 128 where they are many.
     auto tiles_of = [](long long down, long long across, int T, int batch) { return agb_cdiv(down, T) * (long long)agb_cdiv(across, T) * batch; };
     m.tile_x = m.kp >= 256 && tiles_of(m.np, m.kp, 128, m.batch) >= NS_HALF_DEVICE ? 128 : 64;
     m.kt_x = agb_cdiv(m.kp, m.tile_x);
     m.nt_x = agb_cdiv(m.np, m.tile_x);
-    m.tile = m.kp >= 256 ? 128 : 64;
+    // G: the tile and the number of chunks of n (none shorter than 256) that take least by those figures and the fold's, which
+    // more than one chunk needs: 3 us and what the chunks' sums take through memory.  (By the matrix alone: what else is in the
+    // list does not change a result.  3 x 515 x 1029: 135 tiles of 64 x 64 take 200 us in all; 45 of 128 x 128 in three chunks
+    // each 231.  2048 x 2048: 136 of 128 x 128 698, 528 of 64 x 64 736.)
+    double best = 1e30;
+    for (int T = 64; T <= (m.kp >= 256 ? 128 : 64); T *= 2) {
+        const long long kt = agb_cdiv(m.kp, T), tiles = kt * (kt + 1) / 2 * m.batch;
+        for (int splits = 1; splits <= 64 && (splits == 1 || m.np / splits >= 256); ++splits) {
+            const int chunk = agb_cdiv(agb_cdiv(m.np, splits), 64) * 64, real = agb_cdiv(m.np, chunk);
+            const double rounds = (double)((tiles * real + 255) / 256), sum = chunk / 32;
+            const double us = (T == 128 ? rounds * (6 + 0.65 * sum) : 5 + rounds * (1 + 0.22 * sum)) +
+                              (real > 1 ? 3 + (double)tiles * real * (T == 128 ? 0.04 : 0.02) : 0);
+            if (us < best) {
+                best = us;
+                m.tile = T;
+                m.chunk = chunk;
+            }
+        }
+    }
     m.kt = agb_cdiv(m.kp, m.tile);
     m.tri = m.kt * (m.kt + 1) / 2;
     const long long tiles = (long long)m.tri * m.batch;
-    // G: the number of chunks of n that takes least by those figures, with 6 us for the fold that more than one needs; none
-    // shorter than 512.  (By the matrix alone: what else is in the list does not change a result.)
-    double best = 1e30;
-    m.chunk = m.np;
-    for (int splits = 1; splits <= 64 && (splits == 1 || m.np / splits >= 512); ++splits) {
-        const int chunk = agb_cdiv(agb_cdiv(m.np, splits), 64) * 64, real = agb_cdiv(m.np, chunk);
-        const double wgs = (double)tiles * real, slots = m.tile == 128 ? 256 : 512;
-        const double rounds = wgs <= slots ? 1 : (double)agb_cdiv((long long)wgs, (long long)slots);
-        const double us = rounds * (m.tile == 128 ? 6 + chunk * (0.65 / 32) : 5 + chunk * (0.25 / 32)) + (real > 1 ? 6 + wgs * 0.01 : 0);
-        if (us < best) {
-            best = us;
-            m.chunk = chunk;
-        }
-    }
     m.splits = agb_cdiv(m.np, m.chunk);
     // P: k products a sum and few tiles: 64 x 64 as long as those fit the device twice
     const int k64 = m.kp / 64;
@@ -1200,7 +1205,7 @@ static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
     m.kt_p = agb_cdiv(m.kp, m.tile_p);
     m.tri_p = m.kt_p * (m.kt_p + 1) / 2;
     m.sums = agb_cdiv((long long)rows * cols, NS_CHUNK);
-    // (measured, 64 x 64: 21 us whole, 111 us in tiles; the limits: LDS, and what a thread holds of X)
+    // (measured: 64 x 64 18 us whole, 64 x 1728 in tiles 110; the limits: LDS, and what a thread holds of X)
     const bool whole = (m.kp == 64 && m.np <= NS_RES_ROWS) || (m.kp == 128 && m.np == 128);
     if (whole) {
         const int lds = m.np * m.kp * 4 + m.kp * m.kp * 4;
