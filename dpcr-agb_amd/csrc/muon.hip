@@ -946,10 +946,23 @@ __device__ __forceinline__ void ns_resident(const NsMat& m, int b, const NsUpdat
     }
     __syncthreads();
     const int ia0 = (wave >> 1) * TA, ib0 = (wave & 1) * TB, pair = wave & (PAIRS - 1);
-    f32x4 x[UNITS][2];
+    f32x4 x[UNITS][2];      // this wave's blocks of X, as the last step left them
+#pragma unroll
+    for (int l = 0; l < UNITS; ++l) {
+        const int n = (l * 8 + wave) / PAIRS;
+        if (n < NP / 16) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float v[4];
+                ns_quad_get(X, NP, pair * 2 + i, n, v);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[l][i][e] = v[e];
+            }
+        }
+    }
     for (int step = 0; step < steps; ++step) {
         const float ca = abc[3 * step], cb = abc[3 * step + 1], cc = abc[3 * step + 2] * NS_UNSCALE;
-        f32x4 acc[TA][TB];
+        f32x4 acc[TA][TB], g[TA][TB];
         auto clear = [&]() {
 #pragma unroll
             for (int i = 0; i < TA; ++i)
@@ -986,7 +999,7 @@ __device__ __forceinline__ void ns_resident(const NsMat& m, int b, const NsUpdat
             for (int j = 0; j < TB; ++j) {
                 float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * NS_UNSCALE;
+                for (int e = 0; e < 4; ++e) g[i][j][e] = v[e] = acc[i][j][e] * NS_UNSCALE;
                 ns_quad_put(G, KP, ia0 + i, ib0 + j, v);
             }
         __syncthreads();
@@ -1014,13 +1027,12 @@ __device__ __forceinline__ void ns_resident(const NsMat& m, int b, const NsUpdat
 #pragma unroll
             for (int j = 0; j < TB; ++j) {
                 float v[4];
-                ns_quad_get(G, KP, ia0 + i, ib0 + j, v);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(cc, acc[i][j][e], cb * v[e]);
+                for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(cc, acc[i][j][e], cb * g[i][j][e]);
                 ns_quad_put(G, KP, ia0 + i, ib0 + j, v);
             }
         __syncthreads();
-        // X <- a X + X P: every product first, then every block in its place
+        // X <- a X + X P: every product first, then every block in its place (behind the last step nobody reads it)
         {
             half8 ph[2][SUM], pl[2][SUM];
 #pragma unroll
@@ -1031,18 +1043,23 @@ __device__ __forceinline__ void ns_resident(const NsMat& m, int b, const NsUpdat
             for (int l = 0; l < UNITS; ++l) {
                 const int n = (l * 8 + wave) / PAIRS;
                 if (n < NP / 16) {
-                    x[l][0] = x[l][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    f32x4 xp[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
                     const int at = ns_row_at(NP, n);
 #pragma unroll
                     for (int s = 0; s < SUM; ++s) {
                         half8 xh, xl;
                         ns_row16(X, at, s * NP * 128, xh, xl);
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) ns_mfma<LOLO>(x[l][i], ph[i][s], pl[i][s], xh, xl);
+                        for (int i = 0; i < 2; ++i) ns_mfma<LOLO>(xp[i], ph[i][s], pl[i][s], xh, xl);
                     }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[l][i][e] = __builtin_fmaf(xp[i][e], NS_UNSCALE, ca * x[l][i][e]);
                 }
             }
         }
+        if (step == steps - 1) break;
         __syncthreads();
 #pragma unroll
         for (int l = 0; l < UNITS; ++l) {
@@ -1051,9 +1068,8 @@ __device__ __forceinline__ void ns_resident(const NsMat& m, int b, const NsUpdat
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     float v[4];
-                    ns_quad_get(X, NP, pair * 2 + i, n, v);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[l][i][e] = v[e] = __builtin_fmaf(x[l][i][e], NS_UNSCALE, ca * v[e]);
+                    for (int e = 0; e < 4; ++e) v[e] = x[l][i][e];
                     ns_quad_put(X, NP, pair * 2 + i, n, v);
                 }
             }
