@@ -20,6 +20,7 @@
 // symmetric: only tiles on and above the diagonal are computed.  G has few tiles and a long sum: it is split over n into chunks,
 // folded in order.
 #include "agb_common.h"
+#include <type_traits>
 
 typedef _Float16 half_t;
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -56,7 +57,8 @@ struct __attribute__((aligned(16))) NsMat {
     long long in_ld, in_bs, out_ld, out_bs;
     int rows, cols, batch, type;      // type of `in` (and of `out` where nothing is updated): 0 fp32, 1 bf16, 2 fp16
     int k, n, kp, np, tall;
-    int vec, out_vec;                 // input contiguous and aligned: four elements at a time; output rows aligned: eight
+    int vec, out_vec;                 // bits: input contiguous and aligned, four elements at a time; tall, and eight elements along
+                                      // k at a time; output rows aligned: eight elements
     int tile, kt, tri, splits, chunk;          // tile of G: along k, on and above the diagonal; chunks of n
     int tile_p, kt_p, tri_p;                   // tile of P
     int tile_x, kt_x, nt_x;                    // tile of X
@@ -163,7 +165,7 @@ __global__ __launch_bounds__(NS_THREADS) void k_ns_squares(const NsMat* tab, int
 #pragma unroll
     for (int l = 0; l < TURNS; ++l) {
         const long long i0 = first + (l * NS_THREADS + threadIdx.x) * 4;
-        if (m.vec && i0 + 4 <= last) {
+        if ((m.vec & 1) && i0 + 4 <= last) {
             ns_in4(m, base + i0, v[l]);
             if (up.on) {
                 const f32x4 q = *(const gfloat4*)(m.mom + i0);
@@ -192,7 +194,7 @@ __global__ __launch_bounds__(NS_THREADS) void k_ns_squares(const NsMat* tab, int
                 mom[l][e] = mom[l][e] * up.mu + v[l][e] * up.omu;
                 v[l][e] = up.nesterov ? v[l][e] * up.omu + mom[l][e] * up.mu : mom[l][e];
             }
-            if (m.vec && i0 + 4 <= last) {
+            if ((m.vec & 1) && i0 + 4 <= last) {
                 *(gfloat4*)(m.mom + i0) = f32x4{mom[l][0], mom[l][1], mom[l][2], mom[l][3]};
             } else {
 #pragma unroll
@@ -876,7 +878,29 @@ __device__ __forceinline__ void ns_resident(const NsMat& m, int b, const NsUpdat
     const int groups = NP / 64 * GROUPS8;      // of a matrix; this wave's: wave, wave + 8, ...
     auto first_of = [&](int group, long long ld) { return min(group / GROUPS8 * 64 + lane, m.n - 1) * (m.tall ? ld : 1); };
     auto column_of = [&](int group, int e, long long ld) { return min(group % GROUPS8 * 8 + e, m.k - 1) * (m.tall ? 1 : ld); };
-    if (m.type == 0) {
+    const bool eights = m.vec & 2;      // (rows of M are rows n, and their ends are groups' ends)
+    auto eight_at = [&](int group, long long ld) { return first_of(group, ld) + min(group % GROUPS8 * 8, m.k - 8); };
+    if (eights && m.type == 0) {
+        const gfloat* in = (const gfloat*)m.in + b * m.in_bs;
+#pragma unroll
+        for (int l = 0; l < GROUPS; ++l)
+            if (l * 8 + wave < groups) {
+                const gfloat4* p = (const gfloat4*)(in + eight_at(l * 8 + wave, m.in_ld));
+                const f32x4 q = p[0], r = p[1];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { u[l][e] = q[e]; u[l][4 + e] = r[e]; }
+            }
+    } else if (eights) {
+        const gshort* in = (const gshort*)m.in + b * m.in_bs;
+        u32x4 raw[GROUPS];
+#pragma unroll
+        for (int l = 0; l < GROUPS; ++l)
+            if (l * 8 + wave < groups) raw[l] = *(const guint4*)(in + eight_at(l * 8 + wave, m.in_ld));
+#pragma unroll
+        for (int l = 0; l < GROUPS; ++l)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) u[l][e] = ns_value((unsigned short)(raw[l][e / 2] >> 16 * (e & 1)), m.type);
+    } else if (m.type == 0) {
         const gfloat* in = (const gfloat*)m.in + b * m.in_bs;
 #pragma unroll
         for (int l = 0; l < GROUPS; ++l)
@@ -908,7 +932,12 @@ __device__ __forceinline__ void ns_resident(const NsMat& m, int b, const NsUpdat
         if (group >= groups) continue;
         float mom[8];
         gfloat* pm = m.mom + first_of(group, m.cols);
-        if (up.on) {
+        gfloat4* pm8 = (gfloat4*)(m.mom + eight_at(group, m.cols));
+        if (up.on && eights) {
+            const f32x4 q = pm8[0], r = pm8[1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { mom[e] = q[e]; mom[4 + e] = r[e]; }
+        } else if (up.on) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) mom[e] = pm[column_of(group, e, m.cols)];
         }
@@ -919,11 +948,15 @@ __device__ __forceinline__ void ns_resident(const NsMat& m, int b, const NsUpdat
             if (up.on) {
                 v = ns_clip(v, up.clip);
                 mom[e] = mom[e] * up.mu + v * up.omu;
-                if (there) pm[column_of(group, e, m.cols)] = mom[e];
+                if (there && !eights) pm[column_of(group, e, m.cols)] = mom[e];
                 v = up.nesterov ? v * up.omu + mom[e] * up.mu : mom[e];
             }
             u[l][e] = there ? v : 0.f;
             s += (double)u[l][e] * u[l][e];
+        }
+        if (up.on && eights && n < m.n && k < m.k) {
+            pm8[0] = f32x4{mom[0], mom[1], mom[2], mom[3]};
+            pm8[1] = f32x4{mom[4], mom[5], mom[6], mom[7]};
         }
     }
 #pragma unroll
@@ -969,11 +1002,29 @@ __device__ __forceinline__ void ns_resident(const NsMat& m, int b, const NsUpdat
 #pragma unroll
                 for (int j = 0; j < TB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         };
-        auto multiply = [&](const half8* ah, const half8* al, const half8* bh, const half8* bl) {
+        // Operands are read one block of B ahead of the products that take them (all of a step ahead: too many registers).
+        auto product = [&](auto count, auto read_a, auto read_b) {
+            half8 ah[2][TA], al[2][TA], bh[2], bl[2];
 #pragma unroll
-            for (int i = 0; i < TA; ++i)
+            for (int i = 0; i < TA; ++i) read_a(0, i, ah[0][i], al[0][i]);
+            read_b(0, 0, bh[0], bl[0]);
 #pragma unroll
-                for (int j = 0; j < TB; ++j) ns_mfma<LOLO>(acc[i][j], ah[i], al[i], bh[j], bl[j]);
+            for (int l = 0; l < count * TB; ++l) {
+                const int s = l / TB, j = l % TB, n = l + 1;
+                if (n < count * TB) read_b(n / TB, n % TB, bh[n & 1], bl[n & 1]);
+                if (s + 1 < count) {
+#pragma unroll
+                    for (int i = j * TA / TB; i < (j + 1) * TA / TB; ++i) read_a(s + 1, i, ah[(s + 1) & 1][i], al[(s + 1) & 1][i]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int k = LOLO ? 0 : 1; k < 4; ++k)
+#pragma unroll
+                    for (int i = 0; i < TA; ++i)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k < 2 ? al[s & 1][i] : ah[s & 1][i],
+                                                                           k == 0 || k == 2 ? bl[l & 1] : bh[l & 1], acc[i][j], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         };
         // G = X^T X
         {
@@ -983,15 +1034,9 @@ __device__ __forceinline__ void ns_resident(const NsMat& m, int b, const NsUpdat
 #pragma unroll
             for (int j = 0; j < TB; ++j) { b1[j] = ns_column_at(NP, ib0 + j, 0); b2[j] = ns_column_at(NP, ib0 + j, 1); }
             clear();
-#pragma unroll 2
-            for (int s = 0; s < NP / 32; ++s) {
-                half8 ah[TA], al[TA], bh[TB], bl[TB];
-#pragma unroll
-                for (int i = 0; i < TA; ++i) ns_column16(X, a1[i], a2[i], s * 4096, ah[i], al[i]);
-#pragma unroll
-                for (int j = 0; j < TB; ++j) ns_column16(X, b1[j], b2[j], s * 4096, bh[j], bl[j]);
-                multiply(ah, al, bh, bl);
-            }
+            product(std::integral_constant<int, NP / 32>(),
+                    [&](int s, int i, half8& hi, half8& lo) { ns_column16(X, a1[i], a2[i], s * 4096, hi, lo); },
+                    [&](int s, int j, half8& hi, half8& lo) { ns_column16(X, b1[j], b2[j], s * 4096, hi, lo); });
         }
 #pragma unroll
         for (int i = 0; i < TA; ++i)
@@ -1011,15 +1056,9 @@ __device__ __forceinline__ void ns_resident(const NsMat& m, int b, const NsUpdat
             for (int i = 0; i < TA; ++i) a1[i] = ns_row_at(KP, ia0 + i);
 #pragma unroll
             for (int j = 0; j < TB; ++j) b1[j] = ns_row_at(KP, ib0 + j);
-#pragma unroll
-            for (int s = 0; s < SUM; ++s) {
-                half8 ah[TA], al[TA], bh[TB], bl[TB];
-#pragma unroll
-                for (int i = 0; i < TA; ++i) ns_row16(G, a1[i], s * KP * 128, ah[i], al[i]);
-#pragma unroll
-                for (int j = 0; j < TB; ++j) ns_row16(G, b1[j], s * KP * 128, bh[j], bl[j]);
-                multiply(ah, al, bh, bl);
-            }
+            product(std::integral_constant<int, SUM>(),
+                    [&](int s, int i, half8& hi, half8& lo) { ns_row16(G, a1[i], s * KP * 128, hi, lo); },
+                    [&](int s, int j, half8& hi, half8& lo) { ns_row16(G, b1[j], s * KP * 128, hi, lo); });
         }
         __syncthreads();
 #pragma unroll
@@ -1088,7 +1127,17 @@ __device__ __forceinline__ void ns_resident(const NsMat& m, int b, const NsUpdat
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int k0 = (pair * 2 + i) * 16 + 4 * (lane >> 4);
-            if (up.on || m.type == 0) {
+            if (m.tall && m.out_vec && k0 + 4 <= m.k) {
+                if (n >= m.n) continue;
+                if (up.on || m.type == 0) {
+                    gfloat4* p = (gfloat4*)((gfloat*)m.out + base + k0);
+                    *p = up.on ? *p * up.decay - m.step * x[l][i] : x[l][i];
+                } else {
+                    const unsigned long long w = ns_pack(x[l][i][0], x[l][i][1], m.type) |
+                                                 (unsigned long long)ns_pack(x[l][i][2], x[l][i][3], m.type) << 32;
+                    *(NS_GLOBAL unsigned long long*)((gshort*)m.out + base + k0) = w;
+                }
+            } else if (up.on || m.type == 0) {
                 gfloat* p = (gfloat*)m.out + base;
                 float old[4];
                 if (up.on) {
@@ -1177,8 +1226,10 @@ static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
     m.in_ld = f[NS_IN_LD]; m.in_bs = f[NS_IN_BS]; m.out_ld = f[NS_OUT_LD]; m.out_bs = f[NS_OUT_BS];
     m.rows = (int)rows; m.cols = (int)cols; m.batch = (int)batch; m.type = (int)f[NS_TYPE];
     m.tall = rows >= cols;
-    m.vec = m.in_ld == cols && m.in_bs % 4 == 0 && f[NS_IN] % 16 == 0 && f[NS_MOM] % 16 == 0;
     const int esize = m.type == 0 ? 4 : 2;
+    const bool aligned = f[NS_IN] % 16 == 0 && f[NS_MOM] % 16 == 0;
+    m.vec = (m.in_ld == cols && m.in_bs % 4 == 0 && aligned ? 1 : 0) |
+            (m.tall && cols % 8 == 0 && m.in_ld * esize % 16 == 0 && m.in_bs * esize % 16 == 0 && aligned ? 2 : 0);
     m.out_vec = m.out_ld * esize % 16 == 0 && m.out_bs * esize % 16 == 0 && f[NS_OUT] % 16 == 0;
     m.k = m.tall ? m.cols : m.rows;
     m.n = m.tall ? m.rows : m.cols;

@@ -205,6 +205,31 @@ def test_update(device, nesterov, gdtype):
             assert float((p.double() - rp).norm()) <= 2 * bound + 4 * 2.0 ** -24 * float(rp.norm())
 
 
+# tall ones whose rows are read eight elements at a time, and those that just miss it: widths, ends, types, strides
+WHOLE = [(200, 40), (100, 8), (129, 64), (250, 24), (97, 96), (128, 120), (128, 104), (64, 8), (256, 56), (8, 8), (200, 36), (130, 7),
+         (128, 100), (40, 200), (104, 128), (9, 256)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", WHOLE)
+def test_matrices_taken_whole(device, shape, dtype):
+    from dpcr_agb_amd.muon_ops import muon_update, orthogonalize
+    x = matrix(3, *shape, dtype=dtype, device=device)
+    for got, want in zip(orthogonalize(x), x):
+        close(got, want)
+    wide = torch.full((3, shape[0] + 1, shape[1] + 24), float("nan"), dtype=dtype, device=device)
+    for first in (8, 1):           # aligned rows further apart, and rows off the grid
+        v = wide[:, :shape[0], first:first + shape[1]]
+        v.copy_(x)
+        assert torch.equal(orthogonalize(v), orthogonalize(x))
+    p, m = matrix(*shape, device=device, seed=1), matrix(*shape, device=device, seed=2)
+    rp, rm, bound = update64(p, x[0], m, 0.02, 0.9, True, 0.1)
+    muon_update([p], [x[0]], [m], lr=0.02, momentum=0.9, weight_decay=0.1)
+    assert float((m.double() - rm).abs().max()) <= 4 * 2.0 ** -24 * float(rm.abs().max() + 1e-3)
+    assert float((p.double() - rp).norm()) <= 2 * bound + 4 * 2.0 ** -24 * float(rp.norm())
+
+
 @pytest.mark.gpu
 def test_optimiser_splits_matrices_and_vectors(device):
     """optim.Muon: matrices by the update above, vectors and groups with muon=False exactly as AdaBelief alone."""
