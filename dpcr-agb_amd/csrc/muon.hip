@@ -794,11 +794,11 @@ __device__ __forceinline__ void ns_apply(const NsMat& m, int wg, int from, float
     }
 }
 // ---- small matrices: everything in one workgroup, X, G and P in LDS (one launch instead of 17)
-// kp = 64 with np <= 256, or kp = np = 128.  Products by 16 x 16 blocks of the result spread over eight waves: what an iteration
+// kp = 64 with np <= 512 (one matrix alone: 256), or kp = np = 128.  Products by 16 x 16 blocks of the result spread over eight waves: what an iteration
 // takes is latency — the products' chains, the splitting of what they leave, five meetings — and small blocks shorten each.
 // kp = 64 adds lo lo: its short sums round so little that the dropped term would show.
 // LDS: X [block of 32 columns][n][128 bytes], then G / P [block][k][128 bytes], piece q of row r at place q ^ (r / 2 % 8).
-#define NS_RES_ROWS 256
+#define NS_RES_ROWS 512
 struct NsCoef {
     float v[3 * NS_MAX_STEPS];
 };
@@ -1165,7 +1165,8 @@ __device__ __forceinline__ void ns_resident_any(const NsMat& m, int b, const NsU
     else if (m.np == 64) ns_resident<64, 64>(m, b, up, eps, abc, steps, lds, red);
     else if (m.np == 128) ns_resident<64, 128>(m, b, up, eps, abc, steps, lds, red);
     else if (m.np == 192) ns_resident<64, 192>(m, b, up, eps, abc, steps, lds, red);
-    else ns_resident<64, 256>(m, b, up, eps, abc, steps, lds, red);
+    else if (m.np == 256) ns_resident<64, 256>(m, b, up, eps, abc, steps, lds, red);
+    else ns_resident<64, 512>(m, b, up, eps, abc, steps, lds, red);
 }
 __global__ __launch_bounds__(NS_WIDE) void k_ns_resident(const NsTable args, const NsMat* tab, int count, const NsUpdate up, double eps,
                                                          const NsCoef coef, int steps) {
@@ -1236,6 +1237,10 @@ static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
     if (m.k > 16384) return false;
     m.kp = agb_cdiv(m.k, 64) * 64;
     m.np = agb_cdiv(m.n, 64) * 64;
+    // (measured: 64 x 64 13 us whole, 64 x 1728 in tiles 110; the limits: LDS, and what a thread holds of X)
+    // (a single 64 x 512 takes 52 us whole and 75 in tiles, but in a list those come with the others' launches, and of the last
+    // launch alone it would be the longest; a stack of 27 takes 74 whole, 102 in tiles)
+    const bool whole = (m.kp == 64 && m.np <= (m.batch > 1 ? NS_RES_ROWS : NS_RES_ROWS / 2)) || (m.kp == 128 && m.np == 128);
     // Products, measured: a workgroup of T = 128 has a CU to itself, for about 6 us and 0.65 for each 32 of the sum; of T = 64 a CU
     // holds two, which share what one alone reaches: 6 us and 0.22 for each 32 (a quarter of the work).  So 64 x 64 where the
     // tiles are few and 128 x 128 where they are many.
@@ -1248,7 +1253,9 @@ static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
     // list does not change a result.  3 x 515 x 1029: 135 tiles of 64 x 64 take 200 us in all; 45 of 128 x 128 in three chunks
     // each 231.  2048 x 2048: 136 of 128 x 128 698, 528 of 64 x 64 736.)
     double best = 1e30;
-    for (int T = 64; T <= (m.kp >= 256 ? 128 : 64); T *= 2) {
+    m.tile = 64;
+    m.chunk = m.np;
+    for (int T = 64; !whole && T <= (m.kp >= 256 ? 128 : 64); T *= 2) {
         const long long kt = agb_cdiv(m.kp, T), tiles = kt * (kt + 1) / 2 * m.batch;
         for (int splits = 1; splits <= 64 && (splits == 1 || m.np / splits >= 256); ++splits) {
             const int chunk = agb_cdiv(agb_cdiv(m.np, splits), 64) * 64, real = agb_cdiv(m.np, chunk);
@@ -1272,10 +1279,8 @@ static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
     m.kt_p = agb_cdiv(m.kp, m.tile_p);
     m.tri_p = m.kt_p * (m.kt_p + 1) / 2;
     m.sums = agb_cdiv((long long)rows * cols, NS_CHUNK);
-    // (measured: 64 x 64 18 us whole, 64 x 1728 in tiles 110; the limits: LDS, and what a thread holds of X)
-    const bool whole = (m.kp == 64 && m.np <= NS_RES_ROWS) || (m.kp == 128 && m.np == 128);
     if (whole) {
-        const int lds = m.np * m.kp * 4 + m.kp * m.kp * 4;
+        const int lds = (m.np > 256 ? NS_RES_ROWS : m.np) * m.kp * 4 + m.kp * m.kp * 4;
         if (lds > plan.lds) plan.lds = lds;
     } else {
         plan.wide |= m.tile == 128;
@@ -1308,20 +1313,29 @@ static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
 }
 
 // Largest |sigma| along the iterations from [0, 1], and largest |b s^2 + c s^4|: both are entries' bounds of what is held as
-// fp16 pairs.
+// fp16 pairs.  In t = s^2: the former is largest at an end or where a + 3 b t + 5 c t^2 = 0, the latter at an end or at -b / 2 c.
 static bool ns_bounded(const float* coef, int steps) {
     double hi = 1.0;
     for (int i = 0; i < steps; ++i) {
-        const double a = coef[3 * i], b = coef[3 * i + 1], c = coef[3 * i + 2];
-        double next = 0;
-        if (!(hi * hi < 7)) return false;
-        for (int s = 0; s <= 256; ++s) {
-            const double x = hi * s / 256, q = b * x * x + c * x * x * x * x, v = x * (a + q);
-            if (!(q < 7 && q > -7)) return false;
-            const double w = v < 0 ? -v : v;
-            if (!(w <= 7)) return false;
-            next = w > next ? w : next;
+        const double a = coef[3 * i], b = coef[3 * i + 1], c = coef[3 * i + 2], end = hi * hi;
+        if (!(end < 7)) return false;
+        double at[4] = {end, 0, 0, 0};
+        if (c != 0) {
+            at[1] = -b / (2 * c);
+            const double root = sqrt(9 * b * b - 20 * a * c);      // (NaN: there are none)
+            at[2] = (-3 * b + root) / (10 * c);
+            at[3] = (-3 * b - root) / (10 * c);
+        } else if (b != 0) {
+            at[1] = -a / (3 * b);
         }
+        double next = 0;
+        for (double t : at) {
+            if (!(t > 0 && t <= end)) continue;
+            const double q = t * (b + c * t), v = fabs(sqrt(t) * (a + q));
+            if (!(fabs(q) < 7 && v <= 7)) return false;
+            next = v > next ? v : next;
+        }
+        if (!(a == a && b == b && c == c)) return false;
         hi = next * 1.001 + 1e-3;
     }
     return true;

@@ -1,6 +1,7 @@
 """Bindings of csrc/muon.hip: orthogonalised matrices (Newton-Schulz iterations) and the update of weight matrices along an
 orthogonalised momentum.  ``optim.Muon`` is the optimiser on top of it."""
 import ctypes
+import functools
 import math
 
 import torch
@@ -15,7 +16,17 @@ MAX_SIDE, MAX_SHORT_SIDE, MAX_STEPS = 1 << 24, 16384, 64
 
 def _coefficients(coefficients, steps):
     """float[3 * steps]: one triple for every step, or a triple for each."""
-    steps = int(steps)
+    if type(coefficients) is tuple and len(coefficients) == 3 and all(type(v) is float for v in coefficients):
+        return _same_coefficients(coefficients, int(steps))
+    return _coefficient_array(coefficients, int(steps))
+
+
+@functools.lru_cache(maxsize=32)
+def _same_coefficients(coefficients, steps):
+    return _coefficient_array(coefficients, steps)
+
+
+def _coefficient_array(coefficients, steps):
     if not 1 <= steps <= MAX_STEPS:
         raise ValueError(f"steps: 1 to {MAX_STEPS}, got {steps}")
     rows = list(coefficients)
@@ -33,7 +44,7 @@ def _check_side(name, rows, cols):
 
 def _run(entry, table, count, device, *args):
     """One call over `count` matrix stacks; workspace from the current stream's pool of the tensors' device."""
-    if device.index != torch.cuda.current_device():
+    if device.index != _lib.current_device():
         with torch.cuda.device(device):
             return _run(entry, table, count, device, *args)
     fields = (ctypes.c_longlong * len(table))(*table)

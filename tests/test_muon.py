@@ -207,7 +207,7 @@ def test_update(device, nesterov, gdtype):
 
 # tall ones whose rows are read eight elements at a time, and those that just miss it: widths, ends, types, strides
 WHOLE = [(200, 40), (100, 8), (129, 64), (250, 24), (97, 96), (128, 120), (128, 104), (64, 8), (256, 56), (8, 8), (200, 36), (130, 7),
-         (128, 100), (40, 200), (104, 128), (9, 256)]
+         (128, 100), (40, 200), (104, 128), (9, 256), (512, 64), (300, 48), (321, 5), (60, 400), (257, 8)]
 
 
 @pytest.mark.gpu
