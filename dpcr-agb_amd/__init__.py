@@ -9,7 +9,9 @@ Layout:
   me_compat.py     the MinkowskiEngine API subset the reference's backbones use
   backbones/       SENet/ResNet (MSENet14/50), MinkowskiPointNet, KPCNN
   instance/        MinkowskiBaselineModel / KPConv model wrappers (set_input / optimize_parameters contract)
-  optim.py         AdaBelief;  dist.py  data-parallel gradient all-reduce (RCCL)
+  norm_ops.py      autograd bindings of the norms: BatchNorm, layer norm, row norms around a residual block
+  muon_ops.py      orthogonalised matrices and updates along them
+  optim.py         AdaBelief, Muon;  dist.py  data-parallel gradient all-reduce (RCCL)
   synthetic.py     seeded synthetic LiDAR plots + batch container
 
 The directory name carries a hyphen (it mirrors the reference's repository name); import it as

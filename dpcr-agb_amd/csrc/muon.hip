@@ -275,7 +275,7 @@ __global__ __launch_bounds__(NS_THREADS) void k_ns_planes(const NsMat* tab, int 
 // ---- a T x T tile of a product of plane pairs, by eight waves: two groups of four, a quarter of the tile each; a step takes 32
 // of the summed index, 16 a group, so that every SIMD has two waves whatever the number of tiles.  Operands go straight from
 // global memory to LDS, 16 bytes a lane, into four buffers in turn: transfers are issued four steps ahead (a step of 128 x 128
-// takes about 0.3 us, a transfer from the other XCDs' side of memory more than one), fragments are read one step ahead of their
+// takes 0.6 us, a transfer from the other XCDs' side of memory more than one), fragments are read one step ahead of their
 // products.  One barrier a step: behind it everybody's transfers of the next step have landed and everybody has read this one's.
 //   rows (TR = false): sum over columns [c0, c1) of A[a0 + i][.] B[b0 + j][.]; a block of 32 columns is T rows of 128 bytes, eight
 //     pieces of 16, piece q of row r at place q ^ (r / 2 % 8): the 16 lanes that read one piece of 16 rows meet each bank once.
@@ -283,8 +283,10 @@ __global__ __launch_bounds__(NS_THREADS) void k_ns_planes(const NsMat* tab, int 
 //   columns (TR = true): sum over rows [c0, c1) of A[.][a0 + i] B[.][b0 + j]; 32 rows of T columns, piece q of row r at place
 //     q ^ 4 (r % 4); ds_read_b64_tr_b16 hands a lane four rows of its column: the four rows that 16 lanes read lie in different
 //     quarters of the banks.  Column blocks behind the last are read as the last and never stored.
+// Measured: X P of 2048 x 2048 54 us (950 TFLOP/s of fp16), of 13824 x 512 35 us (432 tiles, two turns: 618); a step of 128 x 128
+// 0.63 us where its 24 MFMAs a SIMD alone take 0.51; before the first and behind the last together 6 us (descriptor 1.4, first
+// operands 0.7, adding the groups 0.9, the rest output).
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ half8 ns_read_tr(const char* p, int second) {
     const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
@@ -794,8 +796,10 @@ __device__ __forceinline__ void ns_apply(const NsMat& m, int wg, int from, float
     }
 }
 // ---- small matrices: everything in one workgroup, X, G and P in LDS (one launch instead of 17)
-// kp = 64 with np <= 512 (one matrix alone: 256), or kp = np = 128.  Products by 16 x 16 blocks of the result spread over eight waves: what an iteration
-// takes is latency — the products' chains, the splitting of what they leave, five meetings — and small blocks shorten each.
+// kp = 64 with np <= 512 (one matrix alone: 256), or kp = np = 128.  Products by 16 x 16 blocks of the result spread over eight
+// waves: what an iteration takes is latency — the products' chains, the splitting of what they leave, five meetings — and small
+// blocks shorten each.
+// X and G stay in registers beside their planes in LDS.  Measured: 64 x 64 13 us, 27 x 128 x 128 (27 CUs) 46: a step of 128 is 7.
 // kp = 64 adds lo lo: its short sums round so little that the dropped term would show.
 // LDS: X [block of 32 columns][n][128 bytes], then G / P [block][k][128 bytes], piece q of row r at place q ^ (r / 2 % 8).
 #define NS_RES_ROWS 512
@@ -1191,7 +1195,7 @@ __global__ __launch_bounds__(NS_WIDE) void k_ns_apply(const NsMat* tab, int coun
     ns_apply_any<WIDE>(m, blockIdx.x, from, ca, last, up, lds);
 }
 // The last step of a list that also has matrices that are taken whole: those, by the first workgroups, beside the others' tiles
-// (SENet14: seven such matrices take 60 us, on seven CUs).
+// (SENet14: seven of its matrices, on seven CUs, in the 80 us that its last products and the parameters take).
 template <bool WIDE>
 __global__ __launch_bounds__(NS_WIDE) void k_ns_last(const NsMat* tab, int count, int from, float ca, const NsUpdate up, int whole,
                                                      double eps, const NsCoef coef, int steps) {
@@ -1238,8 +1242,8 @@ static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
     m.kp = agb_cdiv(m.k, 64) * 64;
     m.np = agb_cdiv(m.n, 64) * 64;
     // (measured: 64 x 64 13 us whole, 64 x 1728 in tiles 110; the limits: LDS, and what a thread holds of X)
-    // (a single 64 x 512 takes 52 us whole and 75 in tiles, but in a list those come with the others' launches, and of the last
-    // launch alone it would be the longest; a stack of 27 takes 74 whole, 102 in tiles)
+    // (one 64 x 512 takes 70 us a call whole and 97 in tiles, but in a list those come with the others' launches, and of the last
+    // launch it would be the longest part; a stack of 27 takes 74 whole, 102 in tiles)
     const bool whole = (m.kp == 64 && m.np <= (m.batch > 1 ? NS_RES_ROWS : NS_RES_ROWS / 2)) || (m.kp == 128 && m.np == 128);
     // Products, measured: a workgroup of T = 128 has a CU to itself, for about 6 us and 0.65 for each 32 of the sum; of T = 64 a CU
     // holds two, which share what one alone reaches: 6 us and 0.22 for each 32 (a quarter of the work).  So 64 x 64 where the

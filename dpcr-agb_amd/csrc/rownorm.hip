@@ -14,6 +14,9 @@
 // contiguous run of rows and walks it plot segment by plot segment; each (run, plot) pair leaves ONE partial column sum in slot
 // run + plot — both only grow along the rows, so the slots are distinct and runs + plots + 1 of them are enough — folded in slot
 // order: no atomics, results repeat bit for bit.
+// Measured: norm + GELU of 211000 x 64 fp32 21 us forward, 31 backward (5.2 TB/s both); RMS norm + ReLU of 61007 x 512 bf16 23
+// and 36 (5.5, 5.3); join of 211000 x 256 bf16 78 and 111 (4.2, 4.9), folds 21; 50021 x 203 fp32, single channels, with the next
+// norm 32 and 57 (5.1, 4.3).
 // What a bf16 element may cost beside HBM is about 60 vector instructions (37 T lane-instructions/s against 1 T elements/s at 5
 // to 6 bytes): hence the fused parameters f w and f b, the one exponential that value and slope of the GELU share, no compares.
 #include "agb_common.h"
