@@ -47,7 +47,8 @@ typedef NS_GLOBAL u32x4 guint4;
 #define NS_WIDE 512           // threads of a product's workgroup
 #define NS_SCALE 8192.f
 #define NS_UNSCALE (1.f / 8192.f)
-#define NS_CHUNK 4096       // elements of one partial sum of squares
+#define NS_CHUNK 4096       // elements that a workgroup squares at once
+#define NS_SUMS 2048        // partial sums of squares at most (every workgroup of k_ns_planes adds them up)
 #define NS_MAX_STEPS 64
 
 struct __attribute__((aligned(16))) NsMat {
@@ -155,55 +156,57 @@ __device__ __forceinline__ float ns_clip(float g, float clip) {      // (NaN sta
 __global__ __launch_bounds__(NS_THREADS) void k_ns_squares(const NsMat* tab, int count, const NsUpdate up) {
     const NsMat m = ns_find<NS_SQUARES>((NsTab)tab, count, blockIdx.x);
     const int at = blockIdx.x - m.at[NS_SQUARES], b = at / m.sums, part = at % m.sums;
-    const long long total = (long long)m.rows * m.cols, first = (long long)part * NS_CHUNK;
-    const long long last = first + NS_CHUNK < total ? first + NS_CHUNK : total;
+    const long long total = (long long)m.rows * m.cols;
     const bool linear = m.in_ld == m.cols;
     const long long base = b * m.in_bs;
     // (all of a thread's loads first)
     constexpr int TURNS = NS_CHUNK / (4 * NS_THREADS);
-    float v[TURNS][4], mom[TURNS][4];
+    double s = 0;
+    for (long long first = (long long)part * NS_CHUNK; first < total; first += (long long)m.sums * NS_CHUNK) {
+        const long long last = first + NS_CHUNK < total ? first + NS_CHUNK : total;
+        float v[TURNS][4], mom[TURNS][4];
 #pragma unroll
-    for (int l = 0; l < TURNS; ++l) {
-        const long long i0 = first + (l * NS_THREADS + threadIdx.x) * 4;
-        if ((m.vec & 1) && i0 + 4 <= last) {
-            ns_in4(m, base + i0, v[l]);
-            if (up.on) {
-                const f32x4 q = *(const gfloat4*)(m.mom + i0);
-                mom[l][0] = q.x; mom[l][1] = q.y; mom[l][2] = q.z; mom[l][3] = q.w;
-            }
-        } else {
+        for (int l = 0; l < TURNS; ++l) {
+            const long long i0 = first + (l * NS_THREADS + threadIdx.x) * 4;
+            if ((m.vec & 1) && i0 + 4 <= last) {
+                ns_in4(m, base + i0, v[l]);
+                if (up.on) {
+                    const f32x4 q = *(const gfloat4*)(m.mom + i0);
+                    mom[l][0] = q.x; mom[l][1] = q.y; mom[l][2] = q.z; mom[l][3] = q.w;
+                }
+            } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const long long i = i0 + e;
-                v[l][e] = mom[l][e] = 0.f;
-                if (i < last) {
-                    v[l][e] = ns_in(m, linear ? base + i : base + i / m.cols * m.in_ld + i % m.cols);
-                    if (up.on) mom[l][e] = m.mom[i];
+                for (int e = 0; e < 4; ++e) {
+                    const long long i = i0 + e;
+                    v[l][e] = mom[l][e] = 0.f;
+                    if (i < last) {
+                        v[l][e] = ns_in(m, linear ? base + i : base + i / m.cols * m.in_ld + i % m.cols);
+                        if (up.on) mom[l][e] = m.mom[i];
+                    }
                 }
             }
         }
-    }
-    double s = 0;
 #pragma unroll
-    for (int l = 0; l < TURNS; ++l) {
-        const long long i0 = first + (l * NS_THREADS + threadIdx.x) * 4;
-        if (up.on) {
+        for (int l = 0; l < TURNS; ++l) {
+            const long long i0 = first + (l * NS_THREADS + threadIdx.x) * 4;
+            if (up.on) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[l][e] = ns_clip(v[l][e], up.clip);
-                mom[l][e] = mom[l][e] * up.mu + v[l][e] * up.omu;
-                v[l][e] = up.nesterov ? v[l][e] * up.omu + mom[l][e] * up.mu : mom[l][e];
+                for (int e = 0; e < 4; ++e) {
+                    v[l][e] = ns_clip(v[l][e], up.clip);
+                    mom[l][e] = mom[l][e] * up.mu + v[l][e] * up.omu;
+                    v[l][e] = up.nesterov ? v[l][e] * up.omu + mom[l][e] * up.mu : mom[l][e];
+                }
+                if ((m.vec & 1) && i0 + 4 <= last) {
+                    *(gfloat4*)(m.mom + i0) = f32x4{mom[l][0], mom[l][1], mom[l][2], mom[l][3]};
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (i0 + e < last) m.mom[i0 + e] = mom[l][e];
+                }
             }
-            if ((m.vec & 1) && i0 + 4 <= last) {
-                *(gfloat4*)(m.mom + i0) = f32x4{mom[l][0], mom[l][1], mom[l][2], mom[l][3]};
-            } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (i0 + e < last) m.mom[i0 + e] = mom[l][e];
-            }
+            for (int e = 0; e < 4; ++e) s += (double)v[l][e] * v[l][e];
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s += (double)v[l][e] * v[l][e];
     }
     __shared__ double red[NS_THREADS];
     red[threadIdx.x] = s;
@@ -1283,6 +1286,7 @@ static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
     m.kt_p = agb_cdiv(m.kp, m.tile_p);
     m.tri_p = m.kt_p * (m.kt_p + 1) / 2;
     m.sums = agb_cdiv((long long)rows * cols, NS_CHUNK);
+    m.sums = m.sums < NS_SUMS ? m.sums : NS_SUMS;
     if (whole) {
         const int lds = (m.np > 256 ? NS_RES_ROWS : m.np) * m.kp * 4 + m.kp * m.kp * 4;
         if (lds > plan.lds) plan.lds = lds;

@@ -23,6 +23,8 @@
 
 #define RN_THREADS 256
 #define RN_MAX_C 4096
+#define RN_MAX_N 2000000000      // (a row number and a turn further still fit)
+#define RN_MAX_B 10000000
 
 struct RnArgs {
     const void *z, *r, *dy, *dh;
@@ -433,10 +435,10 @@ __device__ __forceinline__ void rn_finish(const RnFold& a, int c, const float* s
     }
 }
 
-// slots [64 y, 64 y + 64), plot by plot
+// slots [64 x, 64 x + 64), plot by plot; 32 columns of blockIdx.y
 __global__ __launch_bounds__(1024) void k_rownorm_fold_slots(const RnFold a) {
     __shared__ float t[32][33];
-    const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5, first = blockIdx.y * 64;
+    const int c = blockIdx.y * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5, first = blockIdx.x * 64;
     int p = 0, s0, s1;
     for (int base = 0; a.ptr && base <= a.B; base += 64) {      // the first plot that ends behind `first`, 64 looks at once
         const int i = base + (threadIdx.x & 63);
@@ -458,16 +460,16 @@ __global__ __launch_bounds__(1024) void k_rownorm_fold_slots(const RnFold a) {
             if (c < a.C)
                 for (int s = s0 + k; s < s1; s += 32) v += a.part[((size_t)s * a.sums + i) * a.C + c];
             v = rn_fold32(v, t);
-            if (k == 0 && c < a.C) a.blocks[((size_t)(blockIdx.y + p) * a.sums + i) * a.C + c] = v;
+            if (k == 0 && c < a.C) a.blocks[((size_t)(blockIdx.x + p) * a.sums + i) * a.C + c] = v;
         }
     }
 }
 
-// per plot (blockIdx.y): the sum of its blocks, or slots -> plots[p][sums][C] and the gate's gradient; without plots straight to
+// per plot (blockIdx.x; there may be more than the other grid axes take): the sum of its blocks, or slots -> plots[p][sums][C] and the gate's gradient; without plots straight to
 // the parameter gradients
 __global__ __launch_bounds__(1024) void k_rownorm_fold_plots(const RnFold a) {
     __shared__ float t[32][33];
-    const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5, p = blockIdx.y;
+    const int c = blockIdx.y * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5, p = blockIdx.x;
     int s0, s1;
     rn_slots(a, p, s0, s1);
     const float* from = a.part;
@@ -588,7 +590,9 @@ static int rn_run(const RnArgs& a, bool bwd, hipStream_t st) {
 
 static int rn_check(const char* name, int n, int C, int B, const int32_t* ptr, const float* gate, const float* keep, int rms,
                     int act, int bf16) {
-    AGB_CHECK_ARG(n >= 0 && C >= 1 && C <= RN_MAX_C, "%s: bad shape n=%d C=%d (C <= %d)", name, n, C, RN_MAX_C);
+    AGB_CHECK_ARG(n >= 0 && n <= RN_MAX_N && C >= 1 && C <= RN_MAX_C, "%s: bad shape n=%d C=%d (n <= %d, C <= %d)", name, n, C,
+                  RN_MAX_N, RN_MAX_C);
+    AGB_CHECK_ARG(!ptr || B <= RN_MAX_B, "%s: %d plots (up to %d)", name, B, RN_MAX_B);
     AGB_CHECK_ARG(act >= ACT_NONE && act <= ACT_GELU, "%s: act %d", name, act);
     AGB_CHECK_ARG((rms == 0 || rms == 1) && (bf16 == 0 || bf16 == 1), "%s: rms and bf16 are 0 or 1", name);
     AGB_CHECK_ARG(ptr ? B >= 1 : (!gate && !keep), "%s: a gate or a keep factor needs the plots' row ranges", name);
@@ -616,7 +620,7 @@ int agb_rownorm_fwd(const void* Z, long long ldz, const void* R, long long ldr, 
 }
 
 size_t agb_rownorm_bwd_workspace_bytes(int n, int C, int B, int next) {
-    if (n < 0 || C < 1 || C > RN_MAX_C || B < 0) return 0;
+    if (n < 0 || n > RN_MAX_N || C < 1 || C > RN_MAX_C || B < 0 || B > RN_MAX_B) return 0;
     const int runs = agb_cdiv(n, rn_rows(n, C)), blocks = rn_blocks(runs, B);
     const size_t slots = (size_t)runs + B + 1, more = blocks ? (size_t)blocks + B + 1 : 0;
     return (slots + more + B + 1) * (next ? 4 : 2) * (size_t)C * sizeof(float);
@@ -664,10 +668,10 @@ int agb_rownorm_bwd(const void* Z, long long ldz, const void* R, long long ldr, 
     }
     f.dw = dw; f.db = db; f.dgate = dgate; f.dscale = dscale; f.dw2 = dw2; f.db2 = db2;
     if (blocks) {
-        hipLaunchKernelGGL(k_rownorm_fold_slots, dim3(agb_cdiv(C, 32), blocks), dim3(1024), 0, st, f);
+        hipLaunchKernelGGL(k_rownorm_fold_slots, dim3(blocks, agb_cdiv(C, 32)), dim3(1024), 0, st, f);
         AGB_CHECK_LAUNCH("agb_rownorm_fold_slots");
     }
-    hipLaunchKernelGGL(k_rownorm_fold_plots, dim3(agb_cdiv(C, 32), ptr ? B + 1 : 1), dim3(1024), 0, st, f);
+    hipLaunchKernelGGL(k_rownorm_fold_plots, dim3(ptr ? B + 1 : 1, agb_cdiv(C, 32)), dim3(1024), 0, st, f);
     AGB_CHECK_LAUNCH("agb_rownorm_fold_plots");
     if (ptr && (dw || db || dscale || dw2 || db2)) {
         hipLaunchKernelGGL(k_rownorm_fold, dim3(agb_cdiv(C, 32)), dim3(1024), 0, st, f);

@@ -131,8 +131,9 @@ def muon_update(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight
         p <- (1 - lr weight_decay) p - lr adjust orthogonalize(u)
 
     params, momenta: fp32, contiguous, each taken as a matrix (``matrix_shape``); grads: fp32, bf16 or fp16 of the same shapes,
-    left as they are; clip_value limits each of their elements first.  All matrices go through the same launches.  A parameter or a momentum may
-    not be listed twice."""
+    left as they are; clip_value limits each of their elements first.  All matrices go through the same launches.  A parameter or a
+    momentum may not be listed twice, nor be a gradient.  In a captured graph lr and the list are fixed; what a model keeps of its
+    weights in other forms is renewed by sparse_ops.bump_weight_epoch() after a replay."""
     _update(params, grads, momenta, lr, 1.0 - lr * weight_decay, momentum, nesterov, steps, coefficients, eps, adjust, clip_value)
 
 
@@ -171,6 +172,8 @@ def _update(params, grads, momenta, lr, decay, momentum, nesterov, steps, coeffi
         seen.update((pp, mp))
         table += [g.data_ptr(), pp, mp, rows, cols, 1, cols, rows * cols, cols, rows * cols, TYPES[g.dtype]]
         sizes.append(shape)
+    if any(f in seen for f in table[0::_FIELDS]):
+        raise ValueError("muon_update: a gradient is a parameter or a momentum of the list")
     steplen = (ctypes.c_float * max(1, len(params)))(*(lr * adjust_factor(adjust, r, c) for r, c in sizes))
     if params:
         _run("agb_muon_update", table, len(params), params[0].device, steps, coef, float(eps), steplen,

@@ -392,6 +392,7 @@ _lib.declare("agb_rownorm_bwd", [_V, _L, _V, _L, _V, _L, _V, _L, _I, _I, _V, _V,
                                  _L, _V, _L, _V, _V, _V, _V, _V, _V, _V, _lib.ctypes.c_size_t, _I, _V])
 ROW_NORM_KINDS = {"layer": 0, "rms": 1}
 ROW_NORM_MAX_C = 4096
+ROW_NORM_MAX_N, ROW_NORM_MAX_PLOTS = 2_000_000_000, 10_000_000
 
 
 _ROW_TYPES = {torch.float32: 0, torch.bfloat16: 1}
@@ -494,8 +495,9 @@ def _check_rows(what, z, kind, act):
         raise ValueError(f"{what}: kind '{kind}': choose layer or rms")
     if act not in ACT_IDS:
         raise ValueError(f"{what}: act '{act}': choose none, relu or gelu")
-    if z.dim() != 2 or not 1 <= z.shape[1] <= ROW_NORM_MAX_C:
-        raise ValueError(f"{what}: rows [N, C] with 1 <= C <= {ROW_NORM_MAX_C} are normalised, got {list(z.shape)}")
+    if z.dim() != 2 or not 1 <= z.shape[1] <= ROW_NORM_MAX_C or z.shape[0] > ROW_NORM_MAX_N:
+        raise ValueError(f"{what}: rows [N, C] with N <= {ROW_NORM_MAX_N}, 1 <= C <= {ROW_NORM_MAX_C} are normalised, got "
+                         f"{list(z.shape)}")
     if z.dtype not in _ROW_TYPES:
         raise _lib.AgbError(f"{what}: rows are fp32 or bf16 (got {z.dtype})")
     return ROW_NORM_KINDS[kind], ACT_IDS[act], _ROW_TYPES[z.dtype]
@@ -579,6 +581,8 @@ def row_norm_join(z, r, weight=None, bias=None, eps=1e-6, kind="layer", act=None
             raise ValueError(f"{what}: ptr is int32 [B + 1] on {dev}, got {ptr.dtype} {list(ptr.shape)} on {ptr.device}")
         ptr = ptr.contiguous()
         plots = ptr.shape[0] - 1
+        if plots > ROW_NORM_MAX_PLOTS:
+            raise ValueError(f"{what}: {plots} plots (up to {ROW_NORM_MAX_PLOTS})")
         keep = _vector(what, "keep", keep, plots, dev)
         if keep is not None and keep.requires_grad:
             raise ValueError(f"{what}: keep factors are drawn, they have no gradient: pass a learned factor as gate")

@@ -78,6 +78,32 @@ def test_large_kernel_matrix(device):
 
 
 @pytest.mark.gpu
+def test_more_than_31_bits_of_elements(device):
+    """A polynomial of X X^T times X is X times a small matrix, which is taken in 64 bits here: rows at both ends, and where the
+    offsets pass 2^31."""
+    from dpcr_agb_amd.muon_ops import orthogonalize
+    rows, cols = 16_000_000, 136
+    x = torch.randn(rows, cols, device=device) * torch.exp(0.5 * torch.randn(cols, device=device))
+    got = orthogonalize(x)
+    g = torch.zeros(cols, cols, dtype=torch.float64, device=device)
+    for part in x.split(1 << 20):
+        g += part.double().T.contiguous() @ part.double()
+    norm = float(g.trace().sqrt()) + EPS
+    g = g / norm ** 2
+    q, s2 = torch.eye(cols, dtype=torch.float64, device=device), g
+    for a, b, c in [C] * 5:
+        step = a * torch.eye(cols, dtype=torch.float64, device=device) + b * s2 + c * (s2 @ s2)
+        q, s2 = q @ step, s2 @ step @ step
+    bound = iterate(torch.linalg.cholesky(g).T)[1]       # (the same singular values)
+    at = (1 << 31) // cols
+    for first in (0, at - 500, rows - 1000):
+        want = (x[first:first + 1000].double() / norm) @ q
+        # the bound is of all rows together; a thousand of them take their part of it, and five times that
+        err = float((got[first:first + 1000].double() - want).norm())
+        assert err <= 5 * (1000 / rows) ** 0.5 * bound + 2.0 ** -24 * float(want.norm()), (first, err)
+
+
+@pytest.mark.gpu
 def test_lists_equal_single_calls(device):
     """A list of unlike matrices (more than one table's worth, empty ones among them) gives what single calls give, bit for bit."""
     from dpcr_agb_amd.muon_ops import orthogonalize
@@ -331,6 +357,10 @@ def test_refuses_what_is_listed_twice(device):
         muon_update([p, p.clone()], [p.clone()] * 2, [m, m], lr=0.1)
     with pytest.raises(ValueError, match="twice"):
         muon_update([p], [p.clone()], [p], lr=0.1)
+    with pytest.raises(ValueError, match="gradient"):
+        muon_update([p], [m], [m], lr=0.1)
+    with pytest.raises(ValueError, match="gradient"):
+        muon_update([p, p.clone()], [m.clone(), p], [m, m.clone()], lr=0.1)
 
 
 def test_entry_points_validate_before_any_launch():

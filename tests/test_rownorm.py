@@ -151,6 +151,35 @@ def test_join_ragged_plots(device, n, plots):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [3000, 90000])
+def test_more_plots_than_a_grid_axis_takes(device, n):
+    check(make(n, 8, torch.float32, device, plots=70000, seed=n), "layer", "gelu", False)
+
+
+@pytest.mark.gpu
+def test_long_matrices_backwards(device):
+    """More than 2^31 elements: the rows' gradients at both ends are those of short matrices, column sums those of the parts."""
+    from dpcr_agb_amd import norm_ops
+    n, c = (1 << 31) // 64 + 5000, 64
+    z = torch.randn(n, c, device=device, dtype=torch.bfloat16).requires_grad_()
+    dy = torch.randn(n, c, device=device, dtype=torch.bfloat16)
+    w = torch.ones(c, device=device, requires_grad=True)
+    y = norm_ops.row_norm_act(z, w, None, kind="rms", act="gelu")
+    dz, dw = torch.autograd.grad([y], [z, w], [dy])
+    total, size = torch.zeros(c, dtype=torch.float64, device=device), torch.zeros(c, dtype=torch.float64, device=device)
+    for part in torch.arange(n, device=device).chunk(8):
+        a, b = int(part[0]), int(part[-1]) + 1
+        u = z[a:b].detach().requires_grad_()
+        v = norm_ops.row_norm_act(u, w, None, kind="rms", act="gelu")
+        du, part_w = torch.autograd.grad([v], [u, w], [dy[a:b]])
+        assert torch.equal(v, y[a:b]) and torch.equal(du, dz[a:b])
+        total += part_w.double()
+        size += 1 + part_w.double().abs()
+    # sums of n terms of size one in either order: 2^-24 of the partial sums, of which there are sqrt(n / 2048) times 2048 and more
+    assert bool(((dw.double() - total).abs() <= 64 * 2.0 ** -24 * (size + n ** 0.5)).all())
+
+
+@pytest.mark.gpu
 def test_rows_behind_the_last_plot_are_handed_on(device):
     t = make(300, 64, torch.float32, device, plots=4, behind=40, seed=3)
     check(t, "layer", "gelu", False)
@@ -330,6 +359,10 @@ def test_refusals():
         norm_ops.row_norm_act(torch.zeros(4, 0))
     with pytest.raises(ValueError):
         norm_ops.row_norm_act(torch.zeros(2, 4, 8))
+    with pytest.raises(ValueError, match="N <="):
+        norm_ops.row_norm_act(torch.zeros(1, 8).expand((1 << 32) + 4, 8))      # (as 32 bits: four rows)
+    with pytest.raises(ValueError, match="plots"):
+        norm_ops.row_norm_join(z, z, keep=torch.ones(1), ptr=torch.zeros(1, dtype=torch.int32).expand(20_000_001))
     with pytest.raises(ValueError, match="weight"):
         norm_ops.row_norm_act(z, torch.ones(7))
     with pytest.raises(_lib.AgbError, match="fp32"):
