@@ -212,14 +212,22 @@ __device__ __forceinline__ void rn_gelu(float u, float& y, float& slope) {
     slope = __builtin_fmaf(u * 0.39894228f, e, cdf);
 }
 
-// the plot of a row: how many of ptr[1 .. B] are <= row (B: behind the last plot), 64 looks at once
-__device__ __forceinline__ int rn_plot(const int32_t* ptr, int B, int row) {
-    int p = 0;
-    for (int base = 0; base < B; base += 64) {
-        const int i = base + (threadIdx.x & 63);
-        p += __popcll(__ballot(i < B && ptr[min(i, B - 1) + 1] <= row));
+// how many of 0 .. n - 1 `holds` holds for, if for none behind one that it does not hold for; 64 looks at once, a 64th of what is
+// left between them (whatever `holds` says: it ends, between 0 and n)
+template <typename F>
+__device__ __forceinline__ int rn_count(int n, F holds) {
+    int from = 0, end = n;
+    while (from < end) {
+        const int apart = (end - from + 63) >> 6, i = from + apart * (int)(threadIdx.x & 63) + apart - 1;
+        const int yes = __popcll(__ballot(i < end && holds(min(i, n - 1))));
+        from += yes * apart;
+        end = min(end, from + apart - 1);
     }
-    return __builtin_amdgcn_readfirstlane(p);
+    return __builtin_amdgcn_readfirstlane(from);
+}
+// the plot of a row: how many of ptr[1 .. B] are <= row (B: behind the last plot)
+__device__ __forceinline__ int rn_plot(const int32_t* ptr, int B, int row) {
+    return rn_count(B, [&](int i) { return ptr[i + 1] <= row; });
 }
 
 // f w and f b with f = keep[p] gate[p] scale of plot p; 0 behind the last plot (such a row is handed on as act(r))
@@ -262,7 +270,7 @@ __global__ __launch_bounds__(RN_THREADS) void k_rownorm(const RnArgs a) {
     int row0 = first;
     while (row0 < last) {
         const int p = a.ptr ? rn_plot(a.ptr, a.B, row0) : 0;
-        const int end = a.ptr && p < a.B ? min(last, a.ptr[p + 1]) : last;
+        const int end = a.ptr && p < a.B ? min(last, max(a.ptr[p + 1], row0 + 1)) : last;      // (it ends, whatever ptr holds)
         const bool live = !a.ptr || p < a.B;      // (rows behind the last plot: y = act(r), dz = 0 whatever z holds)
         float fw[N], fb[N], sums[BWD ? SUMS : 1][N];
         rn_factor<W, G, V>(a, p, lane, fw, fb);
@@ -439,13 +447,11 @@ __device__ __forceinline__ void rn_finish(const RnFold& a, int c, const float* s
 __global__ __launch_bounds__(1024) void k_rownorm_fold_slots(const RnFold a) {
     __shared__ float t[32][33];
     const int c = blockIdx.y * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5, first = blockIdx.x * 64;
-    int p = 0, s0, s1;
-    for (int base = 0; a.ptr && base <= a.B; base += 64) {      // the first plot that ends behind `first`, 64 looks at once
-        const int i = base + (threadIdx.x & 63);
-        rn_slots(a, min(i, a.B), s0, s1);
-        p += __popcll(__ballot(i <= a.B && s1 <= first));
-    }
-    p = __builtin_amdgcn_readfirstlane(p);
+    int s0, s1;
+    int p = !a.ptr ? 0 : rn_count(a.B + 1, [&](int i) {      // the first plot that ends behind `first`
+        rn_slots(a, i, s0, s1);
+        return s1 <= first;
+    });
     int look0 = 0, look1 = 0;      // lane i: the slots of plot p + i (of every 64 plots, one look)
     for (int i = 0; p <= a.B; ++p, i = (i + 1) & 63) {
         if (i == 0) rn_slots(a, min(p + (int)(threadIdx.x & 63), a.B), look0, look1);

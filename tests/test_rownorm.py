@@ -157,6 +157,23 @@ def test_more_plots_than_a_grid_axis_takes(device, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,plots", [(500, 63), (500, 64), (500, 65), (4000, 4096), (4000, 4097), (100, 5000)])
+def test_plots_around_the_searchs_steps(device, n, plots):
+    check(make(n, 16, torch.float32, device, plots=plots, seed=plots, behind=n % 7), "rms", "gelu", False)
+
+
+@pytest.mark.gpu
+def test_row_ranges_out_of_order_end_and_stay_inside(device):
+    """The values mean nothing then; the rows' places and the call's end do not depend on them."""
+    t = make(300, 32, torch.float32, device, plots=6, seed=1)
+    for ptr in ([0, 200, 50, 300, 20, 250, 300], [300, 200, 100, 90, 80, 70, 0], [0, 1 << 30, -5, 7, (1 << 31) - 1, -(1 << 31), 9]):
+        bad = dict(t, ptr=torch.tensor(ptr, dtype=torch.int32, device=device))
+        got = with_grads(call, bad, "layer", "gelu", False)
+        assert got["y"].shape == (300, 32) and torch.isfinite(got["y"]).all()
+    check(t, "layer", "gelu", False)
+
+
+@pytest.mark.gpu
 def test_long_matrices_backwards(device):
     """More than 2^31 elements: the rows' gradients at both ends are those of short matrices, column sums those of the parts."""
     from dpcr_agb_amd import norm_ops
