@@ -479,9 +479,9 @@ __global__ __launch_bounds__(1024) void k_rownorm_fold_plots(const RnFold a) {
     int s0, s1;
     rn_slots(a, p, s0, s1);
     const float* from = a.part;
+    const bool any = s1 > s0;
     if (a.blocks) {
         from = a.blocks;
-        const bool any = s1 > s0;
         s1 = any ? (s1 - 1) / 64 + p + 1 : 0;
         s0 = any ? s0 / 64 + p : 0;
     }
@@ -494,7 +494,7 @@ __global__ __launch_bounds__(1024) void k_rownorm_fold_plots(const RnFold a) {
     if (!a.ptr) { rn_finish(a, c, v); return; }
     for (int i = 0; i < a.sums; ++i) a.plots[((size_t)p * a.sums + i) * a.C + c] = v[i];
     if (a.dgate && p < a.B)
-        a.dgate[(size_t)p * a.C + c] = (a.keep ? a.keep[p] : 1.f) * (a.scale ? a.scale[c] : 1.f) *
+        a.dgate[(size_t)p * a.C + c] = !any ? 0.f : (a.keep ? a.keep[p] : 1.f) * (a.scale ? a.scale[c] : 1.f) *
                                        ((a.w ? a.w[c] : 1.f) * v[1] + (a.b ? a.b[c] : 0.f) * v[0]);
 }
 
@@ -504,6 +504,9 @@ __global__ __launch_bounds__(1024) void k_rownorm_fold(const RnFold a) {
     float v[4] = {0.f, 0.f, 0.f, 0.f};
     if (c < a.C)
         for (int p = k; p <= a.B; p += 32) {
+            int s0, s1;
+            rn_slots(a, p, s0, s1);
+            if (s0 >= s1) continue;      // (no rows: whatever its factors are, an average over no rows among them)
             const float* s = a.plots + (size_t)p * a.sums * a.C + c;
             const float f = p == a.B ? 0.f : (a.keep ? a.keep[p] : 1.f) * (a.gate ? a.gate[(size_t)p * a.C + c] : 1.f);
             if (p < a.B) { v[0] += f * s[0]; v[1] += f * s[a.C]; }

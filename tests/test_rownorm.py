@@ -293,6 +293,15 @@ def test_gradients_against_differences(device):
 
 
 @pytest.mark.gpu
+def test_factors_of_empty_plots_do_not_matter(device):
+    t = make(400, 48, torch.float32, device, plots=9, seed=4, want_h=True)
+    t["ptr"][3:6] = t["ptr"][3].clone()                  # plots 3 and 4 without rows
+    t["plot"] = torch.bucketize(torch.arange(400, device=device), t["ptr"][1:].long().contiguous(), right=True)
+    t["gate"][3], t["gate"][4], t["keep"][4] = float("nan"), float("inf"), float("nan")
+    check(t, "layer", "gelu", True)
+
+
+@pytest.mark.gpu
 def test_non_finite_rows_stay_in_their_rows(device):
     t = make(40, 64, torch.float32, device, plots=2, seed=2)
     clean = with_grads(call, t, "layer", "gelu", False)
