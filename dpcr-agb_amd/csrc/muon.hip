@@ -1399,7 +1399,7 @@ static int ns_run(const char* name, const long long* fields, int count, int step
     }
     for (const void* k : {(const void*)k_ns_gram<true>, (const void*)k_ns_poly<true>, (const void*)k_ns_apply<true>, (const void*)k_ns_last<true>,
                           (const void*)k_ns_last<false>}) {
-        const hipError_t e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, NS_LDS(128));
+        const hipError_t e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, plan.lds > NS_LDS(128) ? plan.lds : NS_LDS(128));
         if (e != hipSuccess) { agb_set_error("%s: %s", name, hipGetErrorString(e)); return AGB_ELAUNCH; }
     }
 #define NS_PRODUCT(kernel, which, wide, ...)                                                                                \

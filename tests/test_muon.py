@@ -116,6 +116,19 @@ def test_lists_equal_single_calls(device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("small", [(2, 512, 64), (5, 300, 40), (2, 128, 128)])
+@pytest.mark.parametrize("large", [(64, 700), (300, 700)])
+def test_stacks_beside_tiles(device, small, large):
+    """Matrices taken whole in the last launch of others, up to the most shared memory that one takes."""
+    from dpcr_agb_amd.muon_ops import orthogonalize
+    xs = [matrix(*large, device=device), matrix(*small, device=device, seed=1)]
+    for got, x in zip(orthogonalize(xs), xs):
+        assert torch.equal(got, orthogonalize(x))
+        for g, m in zip(got.reshape(-1, *got.shape[-2:]), x.reshape(-1, *x.shape[-2:])):
+            close(g, m)
+
+
+@pytest.mark.gpu
 def test_strided_rows(device):
     from dpcr_agb_amd.muon_ops import orthogonalize
     wide = matrix(90, 200, device=device)
