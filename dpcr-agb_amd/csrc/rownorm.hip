@@ -20,6 +20,7 @@
 // What a bf16 element may cost beside HBM is about 60 vector instructions (37 T lane-instructions/s against 1 T elements/s at 5
 // to 6 bytes): hence the fused parameters f w and f b, the one exponential that value and slope of the GELU share, no compares.
 #include "agb_common.h"
+#include "../../include/agb_hip.h"      // struct agb_rownorm_call
 
 #define RN_THREADS 256
 #define RN_MAX_C 4096
@@ -687,6 +688,30 @@ int agb_rownorm_bwd(const void* Z, long long ldz, const void* R, long long ldr, 
         AGB_CHECK_LAUNCH("agb_rownorm_fold");
     }
     return AGB_OK;
+}
+
+static int rn_check_call(const char* name, const agb_rownorm_call* c) {
+    AGB_CHECK_ARG(c, "%s: null pointer", name);
+    AGB_CHECK_ARG(c->n >= 0 && c->n <= RN_MAX_N && c->C >= 1 && c->C <= RN_MAX_C && c->B >= 0 && c->B <= RN_MAX_B,
+                  "%s: bad shape n=%lld C=%lld B=%lld", name, c->n, c->C, c->B);
+    AGB_CHECK_ARG((c->rms | c->bf16) >= 0 && (c->rms | c->bf16) <= 1 && c->act >= 0 && c->act <= ACT_GELU, "%s: rms, act or bf16",
+                  name);
+    return AGB_OK;
+}
+
+int agb_rownorm_fwd_call(const agb_rownorm_call* c, void* stream) {
+    if (int rc = rn_check_call("agb_rownorm_fwd", c)) return rc;
+    return agb_rownorm_fwd(c->Z, c->ldz, c->R, c->ldr, (int)c->n, (int)c->C, c->w, c->b, (float)c->eps, (int)c->rms, (int)c->act,
+                           c->gate, c->keep, c->ptr, (int)c->B, c->scale, c->w2, c->b2, (float)c->eps2, c->Y, c->ldy, c->H, c->ldh,
+                           (int)c->bf16, stream);
+}
+
+int agb_rownorm_bwd_call(const agb_rownorm_call* c, void* stream) {
+    if (int rc = rn_check_call("agb_rownorm_bwd", c)) return rc;
+    return agb_rownorm_bwd(c->Z, c->ldz, c->R, c->ldr, c->dY, c->lddy, c->dH, c->lddh, (int)c->n, (int)c->C, c->w, c->b,
+                           (float)c->eps, (int)c->rms, (int)c->act, c->gate, c->keep, c->ptr, (int)c->B, c->scale, c->w2, c->b2,
+                           (float)c->eps2, c->dZ, c->lddz, c->dR, c->lddr, c->dw, c->db, c->dgate, c->dscale, c->dw2, c->db2,
+                           c->workspace, c->workspace_bytes, (int)c->bf16, stream);
 }
 
 }  // extern "C"

@@ -1,6 +1,9 @@
 """autograd bindings of csrc/norm.hip: training-mode BatchNorm over [N, C] rows fused with the following
 activation, and the fused residual tail act(a * drop_path_scale[batch] + r); of csrc/layernorm.hip; and of csrc/rownorm.hip:
 row norms (layer / rms) before and after a residual block, fused with its activation, gate, residual scale and shortcut."""
+import functools
+import struct
+
 import torch
 
 from . import _lib
@@ -390,6 +393,8 @@ _lib.declare("agb_rownorm_fwd", [_V, _L, _V, _L, _I, _I, _V, _V, _F, _I, _I, _V,
 _lib.declare("agb_rownorm_bwd_workspace_bytes", [_I, _I, _I, _I])
 _lib.declare("agb_rownorm_bwd", [_V, _L, _V, _L, _V, _L, _V, _L, _I, _I, _V, _V, _F, _I, _I, _V, _V, _V, _I, _V, _V, _V, _F, _V,
                                  _L, _V, _L, _V, _V, _V, _V, _V, _V, _V, _lib.ctypes.c_size_t, _I, _V])
+_lib.declare("agb_rownorm_fwd_call", [_lib.ctypes.c_char_p, _V])
+_lib.declare("agb_rownorm_bwd_call", [_lib.ctypes.c_char_p, _V])
 ROW_NORM_KINDS = {"layer": 0, "rms": 1}
 ROW_NORM_MAX_C = 4096
 ROW_NORM_MAX_N, ROW_NORM_MAX_PLOTS = 2_000_000_000, 10_000_000
@@ -406,24 +411,39 @@ def _as_rows(t):
     return t if (c == 1 or t.stride(1) == 1) and (n == 1 or t.stride(0) >= c) else t.contiguous()
 
 
-def _ld(t):
+def _ld(t, n, c):
     """Row stride (of a single row: its width; the stride of an axis of length one says nothing)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return t.stride(0) if n > 1 else c
 
 
 def _at(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
+
+
+# struct agb_rownorm_call, as far as each direction reads it
+_FWD_CALL = struct.Struct("=8q2d14q").pack
+_BWD_CALL = struct.Struct("=8q2d30q").pack
+
+
+def _rows_like(t):
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+@functools.lru_cache(maxsize=256)
+def _row_norm_workspace(n, c, plots, has_h):
+    return _lib.size_call("agb_rownorm_bwd_workspace_bytes", n, c, plots, int(has_h))
 
 
 def _row_norm_forward(z, r, w, b, gate, scale, w2, b2, keep, ptr, cfg):
     """One launch.  (Everything has been checked: addresses are taken as they are.)"""
     eps, rms, act, eps2, want_h, bf16 = cfg
     n, c = z.shape
-    y = torch.empty((n, c), dtype=z.dtype, device=z.device)
-    h = torch.empty_like(y) if want_h else None
-    _lib.call("agb_rownorm_fwd", z.data_ptr(), _ld(z), _at(r), 0 if r is None else _ld(r), n, c, _at(w), _at(b), eps, rms, act,
-              _at(gate), _at(keep), _at(ptr), 0 if ptr is None else ptr.shape[0] - 1, _at(scale), _at(w2), _at(b2), eps2,
-              y.data_ptr(), c, _at(h), c, bf16, _lib.stream())
+    y = _rows_like(z)
+    h = _rows_like(z) if want_h else None
+    _lib.call("agb_rownorm_fwd_call", _FWD_CALL(
+        z.data_ptr(), _at(r), _ld(z, n, c), 0 if r is None else _ld(r, n, c), n, c, _at(w), _at(b), eps, eps2, rms, act, bf16,
+        0 if ptr is None else ptr.shape[0] - 1, _at(gate), _at(keep), _at(ptr), _at(scale), _at(w2), _at(b2), y.data_ptr(), _at(h),
+        c, c), _lib.stream())
     return y, h
 
 
@@ -435,23 +455,26 @@ def _row_norm_backward(z, r, w, b, gate, scale, w2, b2, keep, ptr, cfg, dy, dh, 
         return (None,) * 8
     eps, rms, act, eps2, _, bf16 = cfg
     n, c = z.shape
-    dev = z.device
     dy = None if dy is None else _as_rows(dy)
-    dh = None if dh is None else _as_rows(dh)
-    plots = 0 if ptr is None else ptr.shape[0] - 1
     has_h = dh is not None
-    dz = torch.empty((n, c), dtype=z.dtype, device=dev) if need[0] else None
+    dh = _as_rows(dh) if has_h else None
+    plots = 0 if ptr is None else ptr.shape[0] - 1
+    dz = _rows_like(z) if need[0] else None
     through = need[1] and act == 0 and not has_h           # dr = dy
-    dr = torch.empty((n, c), dtype=z.dtype, device=dev) if need[1] and not through else None
-    dw, db, dscale, dw2, db2 = (torch.empty(c, dtype=torch.float32, device=dev) if k else None
-                                for k in (need[2], need[3], need[5], need[6] and has_h, need[7] and has_h))
-    dgate = torch.empty((plots, c), dtype=torch.float32, device=dev) if need[4] else None
-    size = _lib.size_call("agb_rownorm_bwd_workspace_bytes", n, c, plots, int(has_h))
-    work = torch.empty(size, dtype=torch.uint8, device=dev)
-    _lib.call("agb_rownorm_bwd", z.data_ptr(), _ld(z), _at(r), 0 if r is None else _ld(r), _at(dy), 0 if dy is None else _ld(dy),
-              _at(dh), _ld(dh) if has_h else 0, n, c, _at(w), _at(b), eps, rms, act, _at(gate), _at(keep), _at(ptr), plots,
-              _at(scale), _at(w2), _at(b2), eps2, _at(dz), c, _at(dr), c, _at(dw), _at(db), _at(dgate), _at(dscale), _at(dw2),
-              _at(db2), work.data_ptr(), size, bf16, _lib.stream())
+    dr = _rows_like(r) if need[1] and not through else None
+    dw = torch.empty_like(w) if need[2] else None
+    db = torch.empty_like(b) if need[3] else None
+    dgate = torch.empty_like(gate) if need[4] else None
+    dscale = torch.empty_like(scale) if need[5] else None
+    dw2 = torch.empty_like(w2) if need[6] and has_h else None
+    db2 = torch.empty_like(b2) if need[7] and has_h else None
+    size = _row_norm_workspace(n, c, plots, has_h)
+    work = torch.empty(size, dtype=torch.uint8, device=z.device)
+    _lib.call("agb_rownorm_bwd_call", _BWD_CALL(
+        z.data_ptr(), _at(r), _ld(z, n, c), 0 if r is None else _ld(r, n, c), n, c, _at(w), _at(b), eps, eps2, rms, act, bf16, plots,
+        _at(gate), _at(keep), _at(ptr), _at(scale), _at(w2), _at(b2), 0, 0, 0, 0, _at(dy), _at(dh),
+        0 if dy is None else _ld(dy, n, c), _ld(dh, n, c) if has_h else 0, _at(dz), _at(dr), c, c, _at(dw), _at(db), _at(dgate),
+        _at(dscale), _at(dw2), _at(db2), work.data_ptr(), size), _lib.stream())
     return dz, (dy if through else dr), dw, db, dgate, dscale, dw2, db2
 
 
@@ -504,8 +527,8 @@ def _check_rows(what, z, kind, act):
 
 
 def _vector(what, name, v, n, device):
-    if v is None:
-        return None
+    if v is None or (v.shape == (n,) and v.dtype is torch.float32 and v.device == device and v.is_contiguous()):
+        return v
     if v.dim() != 1 or v.shape[0] != n:
         raise ValueError(f"{what}: {name}: expected [{n}], got {list(v.shape)}")
     return _param(what, name, v, device)

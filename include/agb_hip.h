@@ -442,6 +442,29 @@ int agb_rownorm_bwd(const void* Z, long long ldz, const void* R, long long ldr, 
                     const float* b2, float eps2, void* dZ, long long lddz, void* dR, long long lddr, float* dw, float* db,
                     float* dgate, float* dscale, float* dw2, float* db2, void* workspace, size_t workspace_bytes, int bf16,
                     void* stream);
+/* The same calls with their arguments in one record, which is read before they return (a binding packs it faster than it converts
+ * 24 or 43 arguments).  Every field has eight bytes; _fwd_call reads those up to ldh. */
+struct agb_rownorm_call {
+    const void *Z, *R;
+    long long ldz, ldr, n, C;
+    const float *w, *b;
+    double eps, eps2;
+    long long rms, act, bf16, B;
+    const float *gate, *keep;
+    const int32_t* ptr;
+    const float *scale, *w2, *b2;
+    void *Y, *H;
+    long long ldy, ldh;
+    const void *dY, *dH;
+    long long lddy, lddh;
+    void *dZ, *dR;
+    long long lddz, lddr;
+    float *dw, *db, *dgate, *dscale, *dw2, *db2;
+    void* workspace;
+    unsigned long long workspace_bytes;
+};
+int agb_rownorm_fwd_call(const struct agb_rownorm_call* c, void* stream);
+int agb_rownorm_bwd_call(const struct agb_rownorm_call* c, void* stream);
 
 /* ---------------------------------------------------------------------------------------------------------
  * KPConv index path.  Replaces the CPython extensions behind modules/KPConv/common.py:
