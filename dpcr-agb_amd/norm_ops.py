@@ -513,17 +513,21 @@ class RowNormJoinFunction(torch.autograd.Function):
         return (*_row_norm_backward(*ctx.saved_tensors, ctx.cfg, dy, dh, ctx.needs_input_grad), None, None)
 
 
+_MODES = {(k, a): (rms, act) for k, rms in ROW_NORM_KINDS.items() for a, act in ACT_IDS.items()}
+
+
 def _check_rows(what, z, kind, act):
+    mode, bf16, shape = _MODES.get((kind, act)), _ROW_TYPES.get(z.dtype), z.shape
+    if mode is not None and bf16 is not None and len(shape) == 2 and 1 <= shape[1] <= ROW_NORM_MAX_C and shape[0] <= ROW_NORM_MAX_N:
+        return mode[0], mode[1], bf16
     if kind not in ROW_NORM_KINDS:
         raise ValueError(f"{what}: kind '{kind}': choose layer or rms")
     if act not in ACT_IDS:
         raise ValueError(f"{what}: act '{act}': choose none, relu or gelu")
-    if z.dim() != 2 or not 1 <= z.shape[1] <= ROW_NORM_MAX_C or z.shape[0] > ROW_NORM_MAX_N:
+    if bf16 is not None:
         raise ValueError(f"{what}: rows [N, C] with N <= {ROW_NORM_MAX_N}, 1 <= C <= {ROW_NORM_MAX_C} are normalised, got "
-                         f"{list(z.shape)}")
-    if z.dtype not in _ROW_TYPES:
-        raise _lib.AgbError(f"{what}: rows are fp32 or bf16 (got {z.dtype})")
-    return ROW_NORM_KINDS[kind], ACT_IDS[act], _ROW_TYPES[z.dtype]
+                         f"{list(shape)}")
+    raise _lib.AgbError(f"{what}: rows are fp32 or bf16 (got {z.dtype})")
 
 
 def _vector(what, name, v, n, device):
@@ -544,8 +548,9 @@ def _param(what, name, v, device):
 
 def _on_device(z, run):
     """Launches go to the current stream of the current device: rows of another device bring theirs."""
-    _R(z)       # (refuses host tensors)
-    if z.device.index == _lib.current_device():
+    if not z.is_cuda:
+        _R(z)       # (refuses host tensors)
+    if z.get_device() == _lib.current_device():
         return run()
     with torch.cuda.device(z.device):
         return run()
