@@ -194,8 +194,8 @@ class Muon(AdaBelief):
     A parameter is a matrix with its leading axes merged: a convolution kernel [offsets, Cin, Cout] is [offsets * Cin, Cout].
     A group with ``muon=False`` (a head, an embedding) is left to AdaBelief altogether.  ``adjust``: muon_ops.adjust_factor; with
     "rms" the learning rate and weight decay of an Adam-like optimiser carry over.  ``clip_value`` limits gradient elements, in both
-    updates.  State: ``momentum_buffer`` of matrices, AdaBelief's of the others.  All matrices of a group go through the same
-    launches (20 to 30 in all, whatever their number)."""
+    updates.  Matrices' weight decay is always decoupled.  State: ``momentum_buffer`` of matrices, AdaBelief's of the others.  All
+    matrices of a group go through the same launches (20 to 30 in all, whatever their number).  Device parameters in fp32 only."""
 
     def __init__(self, params, lr=1e-3, momentum=0.95, nesterov=True, ns_steps=5, ns_coefficients=None, ns_eps=1e-7, adjust="rms",
                  **adabelief):
@@ -212,6 +212,14 @@ class Muon(AdaBelief):
         for group in self.param_groups:
             for k, v in mine.items():
                 group.setdefault(k, v)
+
+    def add_param_group(self, param_group):
+        from .muon_ops import _check_side, matrix_shape
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        for p in group["params"]:
+            if group.get("muon", True) and matrix_shape(p) is not None:
+                _check_side("Muon (a group with muon=False is left to AdaBelief)", *matrix_shape(p))
 
     @staticmethod
     def _is_matrix(p):

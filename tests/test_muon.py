@@ -376,6 +376,22 @@ def test_refuses_what_is_listed_twice(device):
         muon_update([p, p.clone()], [m.clone(), p], [m, m.clone()], lr=0.1)
 
 
+def test_optimiser_refuses_what_no_step_could_take():
+    from dpcr_agb_amd.optim import Muon
+    wide = torch.nn.Parameter(torch.empty(16385, 16385, device="meta"))
+    with pytest.raises(ValueError, match="muon=False"):
+        Muon([wide])
+    opt = Muon([{"params": [wide], "muon": False}])
+    with pytest.raises(ValueError, match="muon=False"):
+        opt.add_param_group({"params": [torch.nn.Parameter(torch.empty(2, 1 << 25, device="meta"))]})
+    with pytest.raises(ValueError, match="momentum"):
+        Muon([torch.nn.Parameter(torch.zeros(2, 2))], momentum=1.0)
+    with pytest.raises(ValueError, match="steps"):
+        Muon([torch.nn.Parameter(torch.zeros(2, 2))], ns_steps=0)
+    with pytest.raises(ValueError, match="adjust"):
+        Muon([torch.nn.Parameter(torch.zeros(2, 2))], adjust="spectral")
+
+
 def test_entry_points_validate_before_any_launch():
     import ctypes
     from dpcr_agb_amd import _lib, muon_ops
