@@ -15,7 +15,7 @@
 // run + plot — both only grow along the rows, so the slots are distinct and runs + plots + 1 of them are enough — folded in slot
 // order: no atomics, results repeat bit for bit.
 // Measured: norm + GELU of 211000 x 64 fp32 21 us forward, 31 backward (5.2 TB/s both); RMS norm + ReLU of 61007 x 512 bf16 23
-// and 36 (5.5, 5.3); join of 211000 x 256 bf16 78 and 111 (4.2, 4.9), folds 21; 50021 x 203 fp32, single channels, with the next
+// and 36 (5.5, 5.3); join of 211000 x 256 bf16 78 and 111 (4.2, 4.9), folds 20; 50021 x 203 fp32, single channels, with the next
 // norm 32 and 57 (5.1, 4.3).
 // What a bf16 element may cost beside HBM is about 60 vector instructions (37 T lane-instructions/s against 1 T elements/s at 5
 // to 6 bytes): hence the fused parameters f w and f b, the one exponential that value and slope of the GELU share, no compares.
@@ -420,17 +420,28 @@ __device__ __forceinline__ void rn_slots(const RnFold& a, int p, int& s0, int& s
     }
 }
 
-__device__ __forceinline__ float rn_fold32(float v, float (*t)[33]) {
+// up to four sums over the 32 rows of lanes at once: row k is left with sum k
+typedef float RnFoldBox[4][32][33];
+__device__ __forceinline__ float rn_fold32(const float* v, int sums, RnFoldBox& t) {
     const int c = threadIdx.x & 31, k = threadIdx.x >> 5;
     __syncthreads();
-    t[k][c] = v;
+    for (int i = 0; i < sums; ++i) t[i][k][c] = v[i];
     __syncthreads();
     float s = 0.f;
-    if (k == 0) {
+    if (k < sums) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) s += t[i][c];
+        for (int i = 0; i < 32; ++i) s += t[k][i][c];
     }
-    return s;          // (lane k == 0)
+    return s;
+}
+// ... and row 0 with all of them
+__device__ __forceinline__ void rn_fold32_all(float* v, int sums, RnFoldBox& t) {
+    const int c = threadIdx.x & 31, k = threadIdx.x >> 5;
+    const float s = rn_fold32(v, sums, t);
+    __syncthreads();
+    if (k < sums) t[k][0][c] = s;
+    __syncthreads();
+    for (int i = 0; i < sums; ++i) v[i] = t[i][0][c];
 }
 
 __device__ __forceinline__ void rn_finish(const RnFold& a, int c, const float* s) {
@@ -446,7 +457,7 @@ __device__ __forceinline__ void rn_finish(const RnFold& a, int c, const float* s
 
 // slots [64 x, 64 x + 64), plot by plot; 32 columns of blockIdx.y
 __global__ __launch_bounds__(1024) void k_rownorm_fold_slots(const RnFold a) {
-    __shared__ float t[32][33];
+    __shared__ RnFoldBox t;
     const int c = blockIdx.y * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5, first = blockIdx.x * 64;
     int s0, s1;
     int p = !a.ptr ? 0 : rn_count(a.B + 1, [&](int i) {      // the first plot that ends behind `first`
@@ -462,20 +473,19 @@ __global__ __launch_bounds__(1024) void k_rownorm_fold_slots(const RnFold a) {
         s0 = max(s0, first);
         s1 = min(s1, first + 64);
         if (s0 >= s1) continue;
-        for (int i = 0; i < a.sums; ++i) {
-            float v = 0.f;
-            if (c < a.C)
-                for (int s = s0 + k; s < s1; s += 32) v += a.part[((size_t)s * a.sums + i) * a.C + c];
-            v = rn_fold32(v, t);
-            if (k == 0 && c < a.C) a.blocks[((size_t)(blockIdx.x + p) * a.sums + i) * a.C + c] = v;
-        }
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (c < a.C)
+            for (int s = s0 + k; s < s1; s += 32)
+                for (int i = 0; i < a.sums; ++i) v[i] += a.part[((size_t)s * a.sums + i) * a.C + c];
+        const float sum = rn_fold32(v, a.sums, t);
+        if (k < a.sums && c < a.C) a.blocks[((size_t)(blockIdx.x + p) * a.sums + k) * a.C + c] = sum;
     }
 }
 
 // per plot (blockIdx.x; there may be more than the other grid axes take): the sum of its blocks, or slots -> plots[p][sums][C] and the gate's gradient; without plots straight to
 // the parameter gradients
 __global__ __launch_bounds__(1024) void k_rownorm_fold_plots(const RnFold a) {
-    __shared__ float t[32][33];
+    __shared__ RnFoldBox t;
     const int c = blockIdx.y * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5, p = blockIdx.x;
     int s0, s1;
     rn_slots(a, p, s0, s1);
@@ -490,7 +500,7 @@ __global__ __launch_bounds__(1024) void k_rownorm_fold_plots(const RnFold a) {
     if (c < a.C)
         for (int s = s0 + k; s < s1; s += 32)
             for (int i = 0; i < a.sums; ++i) v[i] += from[((size_t)s * a.sums + i) * a.C + c];
-    for (int i = 0; i < a.sums; ++i) v[i] = rn_fold32(v[i], t);
+    rn_fold32_all(v, a.sums, t);
     if (k || c >= a.C) return;
     if (!a.ptr) { rn_finish(a, c, v); return; }
     for (int i = 0; i < a.sums; ++i) a.plots[((size_t)p * a.sums + i) * a.C + c] = v[i];
@@ -500,7 +510,7 @@ __global__ __launch_bounds__(1024) void k_rownorm_fold_plots(const RnFold a) {
 }
 
 __global__ __launch_bounds__(1024) void k_rownorm_fold(const RnFold a) {
-    __shared__ float t[32][33];
+    __shared__ RnFoldBox t;
     const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
     if (c < a.C)
@@ -513,7 +523,7 @@ __global__ __launch_bounds__(1024) void k_rownorm_fold(const RnFold a) {
             if (p < a.B) { v[0] += f * s[0]; v[1] += f * s[a.C]; }
             if (a.sums == 4) { v[2] += s[2 * (size_t)a.C]; v[3] += s[3 * (size_t)a.C]; }
         }
-    for (int i = 0; i < a.sums; ++i) v[i] = rn_fold32(v[i], t);
+    rn_fold32_all(v, a.sums, t);
     if (k == 0 && c < a.C) rn_finish(a, c, v);
 }
 
