@@ -1217,7 +1217,6 @@ __global__ __launch_bounds__(NS_WIDE) void k_ns_last(const NsMat* tab, int count
 // fields of a matrix stack in the callers' table (int64 each)
 enum { NS_IN, NS_OUT, NS_MOM, NS_ROWS, NS_COLS, NS_BATCH, NS_IN_LD, NS_IN_BS, NS_OUT_LD, NS_OUT_BS, NS_TYPE, NS_FIELDS };
 #define NS_MAX_SIDE (1 << 24)
-#define NS_HALF_DEVICE 160
 
 struct NsPlan {
     size_t bytes;
@@ -1251,8 +1250,14 @@ static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
     // Products, measured: a workgroup of T = 128 has a CU to itself, for about 6 us and 0.65 for each 32 of the sum; of T = 64 a CU
     // holds two, which share what one alone reaches: 6 us and 0.22 for each 32 (a quarter of the work).  So 64 x 64 where the
     // tiles are few and 128 x 128 where they are many.
-    auto tiles_of = [](long long down, long long across, int T, int batch) { return agb_cdiv(down, T) * (long long)agb_cdiv(across, T) * batch; };
-    m.tile_x = m.kp >= 256 && tiles_of(m.np, m.kp, 128, m.batch) >= NS_HALF_DEVICE ? 128 : 64;
+    auto cost = [](int T, long long wgs, int sum) {      // us; `sum`: of how many products
+        const double rounds = (double)((wgs + 255) / 256), steps = sum / 32;
+        return T == 128 ? rounds * (6 + 0.65 * steps) : 5 + rounds * (1 + 0.22 * steps);
+    };
+    auto tiles_of = [&](int T) { return agb_cdiv(m.np, T) * (long long)agb_cdiv(m.kp, T) * m.batch; };
+    auto triangle_of = [&](int T) { const long long kt = agb_cdiv(m.kp, T); return kt * (kt + 1) / 2 * m.batch; };
+    // (X P of 1500 x 1500 by 128 x 128: 424 us a call instead of 491; of 3 x 515 x 1029 by 64 x 64: 238 instead of 251)
+    m.tile_x = m.kp >= 256 && cost(128, tiles_of(128), m.kp) <= cost(64, tiles_of(64), m.kp) ? 128 : 64;
     m.kt_x = agb_cdiv(m.kp, m.tile_x);
     m.nt_x = agb_cdiv(m.np, m.tile_x);
     // G: the tile and the number of chunks of n (none shorter than 256) that take least by those figures and the fold's, which
@@ -1263,12 +1268,10 @@ static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
     m.tile = 64;
     m.chunk = m.np;
     for (int T = 64; !whole && T <= (m.kp >= 256 ? 128 : 64); T *= 2) {
-        const long long kt = agb_cdiv(m.kp, T), tiles = kt * (kt + 1) / 2 * m.batch;
+        const long long tiles = triangle_of(T);
         for (int splits = 1; splits <= 64 && (splits == 1 || m.np / splits >= 256); ++splits) {
             const int chunk = agb_cdiv(agb_cdiv(m.np, splits), 64) * 64, real = agb_cdiv(m.np, chunk);
-            const double rounds = (double)((tiles * real + 255) / 256), sum = chunk / 32;
-            const double us = (T == 128 ? rounds * (6 + 0.65 * sum) : 5 + rounds * (1 + 0.22 * sum)) +
-                              (real > 1 ? 3 + (double)tiles * real * (T == 128 ? 0.04 : 0.02) : 0);
+            const double us = cost(T, tiles * real, chunk) + (real > 1 ? 3 + (double)tiles * real * (T == 128 ? 0.04 : 0.02) : 0);
             if (us < best) {
                 best = us;
                 m.tile = T;
@@ -1280,9 +1283,7 @@ static bool ns_plan(const long long* f, NsMat& m, char* ws, NsPlan& plan) {
     m.tri = m.kt * (m.kt + 1) / 2;
     const long long tiles = (long long)m.tri * m.batch;
     m.splits = agb_cdiv(m.np, m.chunk);
-    // P: k products a sum and few tiles: 64 x 64 as long as those fit the device twice
-    const int k64 = m.kp / 64;
-    m.tile_p = (long long)k64 * (k64 + 1) / 2 * m.batch <= 512 ? 64 : 128;
+    m.tile_p = m.kp >= 256 && cost(128, triangle_of(128), m.kp) <= cost(64, triangle_of(64), m.kp) ? 128 : 64;
     m.kt_p = agb_cdiv(m.kp, m.tile_p);
     m.tri_p = m.kt_p * (m.kt_p + 1) / 2;
     m.sums = agb_cdiv((long long)rows * cols, NS_CHUNK);
